@@ -377,15 +377,14 @@ def _own(s):
         return batch_spec.deltanet_tree(s["proj"][0], s["conv"][0], s["conv_w"][0], s["A_log"][0], s["dt_bias"][0], s["ssm"][0], s["slots"], s["pos"], s["parents"])
     if s["op"] == "commit":
         n, path = batch_spec.accept_tree(s["parents"], s["toks"], s["ids"])
-        batch_spec.deltanet_commit(list(s["proj"]), list(s["conv"]), list(s["conv_w"]), list(s["A_log"]), list(s["dt_bias"]), list(s["ssm"]), s["slots"], s["pos"],
-                                   path, n, dst_slots=s["dst_slots"])
-        batch.compact_rows([*s["K"], *s["V"]], s["table"], s["pos"], path, n, dst_table=s["dst_table"])
+        batch_spec.deltanet_commit(s["proj"], s["conv"], s["conv_w"], s["A_log"], s["dt_bias"], s["ssm"], s["slots"], s["pos"], path, n, dst_slots=s["dst_slots"])
+        batch.compact_rows([s["K"], s["V"]], s["table"], s["pos"], path, n, dst_table=s["dst_table"], stacked=True)
         return dict(n_path=n, path=path, ssm=s["ssm"], conv=s["conv"], K=s["K"], V=s["V"])
-    batch.copy_entries([*s["K"], *s["V"]], s["dst"], s["src"], rows=s["rows"])
+    batch.copy_entries([s["K"], s["V"]], s["dst"], s["src"], rows=s["rows"], stacked=True)
     if "ssm" not in s:
         return dict(K=s["K"], V=s["V"])
-    batch.copy_entries(list(s["ssm"]), s["s_dst"], s["s_src"])
-    batch.copy_entries(list(s["conv"]), s["s_dst"], s["s_src"])
+    batch.copy_entries([s["ssm"]], s["s_dst"], s["s_src"], stacked=True)
+    batch.copy_entries([s["conv"]], s["s_dst"], s["s_src"], stacked=True)
     return dict(K=s["K"], V=s["V"], ssm=s["ssm"], conv=s["conv"])
 
 
