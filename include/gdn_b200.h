@@ -242,6 +242,59 @@ GDN_API int gdn_state_copy(void* dst, const void* src, int elem_size, long long 
  *   device status 1). */
 GDN_API int gdn_hrec(void* hist, const void* rows, const int* slots, const int* pos, int B, int n_slots, int Lh, int H, void* stream);
 
+/* ---- speculative decoding with a tree of drafted tokens, and copies over many pools (no counterpart in the reference, whose
+ *      speculative mode verifies one chain) ----
+ * A tree: parents int32 [B, N], N <= 64.  Node i of sequence b hangs below node parents[b][i] < i; -1 = below the sequence's last
+ * cached token (a root; several are allowed); a smaller value = an unused node.  A parent that does not precede its child, or that
+ * is unused, makes the node (and what hangs below it) unused and sets device status 1. */
+
+/* Attention of all nodes of the trees over a paged KV cache: node i attends the cached keys 0 .. ctx_len[b]-1, itself and its
+ * ancestors; its k / v row is appended at position ctx_len[b] + i (rows of unused nodes are not written; their out rows are zero).
+ *   q, out bf16 [B*N, H, 256];  k_new, v_new bf16 [B*N, KV, 256];  H % KV == 0, H / KV <= 16
+ *   k_pages, v_pages bf16 [n_pages, KV, page_size, 256];  block_table int32 [B, max_pages];  ctx_len int32 [B]
+ *   workspace: at least gqa_tree_attn_workspace_bytes(B, N, H, KV) bytes, 16-byte aligned, contents need no initialisation, not shared by
+ *   calls that overlap on the GPU
+ *   A sequence whose ctx_len is negative, or whose last used node does not fit max_pages * page_size, is skipped (out rows zero,
+ *   status 1); a bad page number inside the context is reported and page 0 read in its place. */
+GDN_API int gqa_tree_attn(const void* q, const void* k_new, const void* v_new, void* k_pages, void* v_pages, const int* block_table, const int* ctx_len,
+                  const int* parents, void* out, void* workspace, size_t workspace_bytes, int B, int N, int H, int KV, int page_size, int max_pages,
+                  int n_pages, void* stream);
+GDN_API size_t gqa_tree_attn_workspace_bytes(int B, int N, int H, int KV);
+
+/* Gated delta rule for all nodes of the trees: node i continues the conv window and the state that its parent leaves (a root: those of
+ * the slot).  Only y is written (rows of unused nodes and of sequences with a bad slot: zero).  Conv, norms and gates in fp32, one
+ * rounding (y).
+ *   proj bf16 [B*N, row_stride >= 8224];  conv_pool, ssm_pool, slots, pos as for gdn_deltanet_b;  y bf16 [B*N, 2048] */
+GDN_API int gdn_tree_verify(const void* proj, long long row_stride, const void* conv_pool, const void* conv_w, const float* A_log, const float* dt_bias,
+                    const float* ssm_pool, const int* slots, const int* pos, const int* parents, int n_slots, void* y, int B, int N, void* stream);
+
+/* The path a target model confirms: the first root, then, as long as there is one, the lowest-numbered child whose token is the one the
+ * target chose after its parent.   toks, ids int32 [B, N]: token of every node, and the target's choice after it.
+ *   path int32 [B, N]: the nodes of the path in order, then -1;  n_path int32 [B] (0 for a tree without nodes) */
+GDN_API int gdn_tree_accept(const int* parents, const int* toks, const int* ids, int* path, int* n_path, int B, int N, void* stream);
+
+/* Advances recurrent state and conv window of n_layers layers along a path through each sequence's tree: state and window of slot
+ * slots[b] (window buffer pos[b] & 1) after the tokens path[b][0 .. n_path[b]-1] go to slot dst_slots[b] (window buffer
+ * (pos[b] + n_path[b]) & 1); dst_slots may equal slots.  A sequence with a bad index or path entry is skipped (status 1).  No
+ * dst_slots[b] may be a slot that another sequence of the call reads or writes with n_path > 0 (the result would depend on the order).
+ *   The `_host` arrays hold one device pointer per layer: proj bf16 [B*N, row_stride], conv_pool, conv_w, A_log, dt_bias, ssm_pool as for
+ *   gdn_deltanet_b.   path int32 [B, E]: nodes of the tree, 0 <= path < N */
+GDN_API int gdn_tree_commit(const void* const* proj_host, long long row_stride, void* const* conv_pool_host, const void* const* conv_w_host,
+                    const void* const* A_log_host, const void* const* dt_bias_host, void* const* ssm_pool_host, int n_layers, const int* slots,
+                    const int* dst_slots, const int* pos, const int* path, const int* n_path, int n_slots, int B, int N, int E, void* stream);
+
+/* Compaction of cached rows in n_pools pools [n_pages, heads, page_size, row_bytes]: row base[b] + keep[b][j] of sequence b (through
+ * block_table) moves to row base[b] + j (through dst_table), j < n_keep[b].  keep is strictly ascending; from the first entry that is not, or
+ * that is out of range, the rest of that sequence stays as it is (status 1).  dst_table equals block_table (in place), or the pages it
+ * names for the written rows are not read by the call.   block_table, dst_table int32 [B, max_pages];  keep int32 [B, L] */
+GDN_API int gdn_rows_compact(void* const* pools_host, int n_pools, int n_pages, int heads, int page_size, long long row_bytes, const int* block_table,
+                     const int* dst_table, int max_pages, const int* base, const int* keep, const int* n_keep, int B, int L, void* stream);
+
+/* Entry dst_host[i] <- entry src_host[i] of every pool [n_entries][n_sub][sub_bytes]; of each sub-block the first len_host[i] bytes (NULL: all).
+ * Indices are host arrays.  No dst may equal another dst or any src (unchecked here; the copies are unordered).  Sizes are even. */
+GDN_API int gdn_entries_copy(void* const* pools_host, int n_pools, long long n_entries, int n_sub, long long sub_bytes, const int* dst_host,
+                     const int* src_host, const long long* len_host, int n_pairs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,6 +5,7 @@ possible every operator raises.  Tensors cross the boundary as raw device pointe
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from ctypes import c_char_p, c_float, c_int, c_longlong, c_size_t, c_void_p, POINTER
 
@@ -48,6 +49,13 @@ SIGNATURES = {
     "gdn_gated_norm": (I, [P, P, LL, P, P, LL, P]),
     "gdn_state_copy": (I, [P, P, I, LL, LL, LL, I, LL, LL, P]),
     "gdn_hrec": (I, [P, P, P, P, I, I, I, I, P]),
+    "gqa_tree_attn": (I, [P, P, P, P, P, P, P, P, P, P, SZ, I, I, I, I, I, I, I, P]),
+    "gqa_tree_attn_workspace_bytes": (SZ, [I, I, I, I]),
+    "gdn_tree_verify": (I, [P, LL, P, P, P, P, P, P, P, P, I, P, I, I, P]),
+    "gdn_tree_accept": (I, [P, P, P, P, P, I, I, P]),
+    "gdn_tree_commit": (I, [P, LL, P, P, P, P, P, I, P, P, P, P, P, I, I, I, I, P]),
+    "gdn_rows_compact": (I, [P, I, I, I, I, LL, P, P, I, P, P, P, I, I, P]),
+    "gdn_entries_copy": (I, [P, I, LL, I, LL, P, P, P, I, P]),
 }
 
 
@@ -98,6 +106,22 @@ def require_cuda(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise RuntimeError("qwen_tailor_b200 operators run on CUDA tensors only (there is no CPU path)")
+
+
+def require_same_device(first, *rest):
+    """All tensors on CUDA and on one device (a launch reads them through plain pointers)."""
+    require_cuda(first, *rest)
+    for t in rest:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on {first.device} and {t.device} in one call")
+
+
+def on_device(device):
+    """Context in which ``device`` is the current one: kernels are launched on the device of their tensors, whatever the caller's is."""
+    return _HERE if device.index is None or device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def device_status() -> int:

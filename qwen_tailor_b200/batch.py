@@ -9,10 +9,14 @@ In-place writes are ordered against later readers by CUDA stream order.
 """
 from __future__ import annotations
 
+import ctypes
+from typing import Sequence
+
+import numpy as np
 import torch
 
 from . import _lib
-from ._lib import check, ptr, stream_ptr
+from ._lib import check, on_device, ptr, require_same_device, stream_ptr
 from .config import Cfg
 from .gated_delta import _f32
 from .kernels import _rows
@@ -90,6 +94,48 @@ def attn_paged_static(q, k_new, v_new, k_pages, v_pages, block_table, ctx_len, M
     return o
 
 
+def attn_tree(q, k_new, v_new, k_pages, v_pages, block_table, ctx_len, parents, out=None):
+    """GQA attention of a TREE of drafted tokens over a paged KV cache: the verify step of tree speculation, as ``attn_paged`` with M > 1
+    is that of a chain (no counterpart in the reference).
+
+    parents int32 [B, N], N <= 64: node i of sequence b hangs below node parents[b, i] < i; -1 = below the last cached token (a root,
+    several are allowed); a smaller value = an unused node.  q [B*N, H, 256], k_new / v_new [B*N, KV, 256] bf16 (normed and roped at
+    position ctx_len[b] + depth of the node), pages [n_pages, KV, page_size, 256] (any page size), block_table int32 [B, max_pages],
+    ctx_len int32 [B].  H is a multiple of KV, at most 16 query heads share one.
+    Node i attends the cached keys of its sequence, its ancestors and itself; its k / v rows are appended at ctx_len[b] + i (in place;
+    ``compact_rows`` moves the accepted ones together afterwards).  Rows of unused nodes are not appended and their output is zero.
+    One node per sequence (N = 1, parents = -1) is plain decode.  Returns o [B*N, H, 256] bf16 (``out``, if given).
+    A malformed tree, context or page number is reported by ``_lib.device_status()``."""
+    require_same_device(q, k_new, v_new, k_pages, v_pages, block_table, ctx_len, parents, out)
+    for name, t in (("block_table", block_table), ("ctx_len", ctx_len), ("parents", parents)):
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise ValueError(f"attn_tree: {name} must be contiguous int32")
+    for t in (q, k_new, v_new, k_pages, v_pages):
+        if t.dtype != torch.bfloat16 or not t.is_contiguous():
+            raise ValueError("attn_tree: q, k_new, v_new and the pages must be contiguous bf16")
+    if parents.dim() != 2 or q.dim() != 3 or k_pages.dim() != 4 or block_table.dim() != 2:
+        raise ValueError("attn_tree: parents [B, N], q [B*N, H, 256], pages [n_pages, KV, page_size, 256] and block_table [B, max_pages] expected")
+    (B, N), (R, H, D), (n_pages, KV, page_size, _) = parents.shape, q.shape, k_pages.shape
+    if not 1 <= N <= 64 or D != 256 or KV < 1 or H % KV or not 1 <= H // KV <= 16:
+        raise ValueError(f"attn_tree: 1 <= N <= 64 nodes, head_dim 256 and H a multiple of KV, at most 16 * KV, are supported (N={N}, H={H}, KV={KV}, D={D})")
+    if R != B * N or k_new.shape != (R, KV, D) or v_new.shape != k_new.shape or v_pages.shape != k_pages.shape or k_pages.shape[3] != D \
+            or block_table.shape[0] != B or ctx_len.shape != (B,):
+        raise ValueError(f"attn_tree: shapes do not agree: q {tuple(q.shape)}, k_new {tuple(k_new.shape)}, v_new {tuple(v_new.shape)}, pages {tuple(k_pages.shape)} / "
+                         f"{tuple(v_pages.shape)}, block_table {tuple(block_table.shape)}, ctx_len {tuple(ctx_len.shape)}, parents {tuple(parents.shape)}")
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
+        raise ValueError("attn_tree: out must be a contiguous bf16 tensor of q's shape")
+    if B == 0:
+        return out
+    lib = _lib.load()
+    with on_device(q.device):
+        ws = torch.empty((lib.gqa_tree_attn_workspace_bytes(B, N, H, KV),), dtype=torch.uint8, device=q.device)
+        check(lib.gqa_tree_attn(ptr(q), ptr(k_new), ptr(v_new), ptr(k_pages), ptr(v_pages), ptr(block_table), ptr(ctx_len), ptr(parents), ptr(out),
+                                ptr(ws), ws.numel(), B, N, H, KV, page_size, block_table.shape[1], n_pages, stream_ptr(q.device)), "attn_tree")
+    return out
+
+
 def attn_b(q, k, v, Kp, Vp, slots, pos, M=1):
     """q [R,H,D], k / v [R,KV,D] (normed + roped), pools [S+1,KV,Lmax,D]; R = B*M rows (row b*M+j = position pos[b]+j of slot
     slots[b]; slots / pos int32 [B]).  Returns o [R,H,D] bf16 and appends k / v at pos[b]+j (in place)  (batch.py:230-237).
@@ -120,6 +166,94 @@ def hrec(hist, Hn, slots, pos):
     assert hist.shape[2] == H and slots.numel() == B and pos.numel() == B
     check(_lib.load().gdn_hrec(ptr(hist), ptr(Hn), ptr(slots), ptr(pos), B, hist.shape[0], hist.shape[1], H, stream_ptr(hist.device)), "hrec")
     return hist
+
+
+def _pool_ptrs(who, pools, stacked):
+    """The pools of ``pools`` (each a contiguous bf16 or fp32 tensor, all of one shape; stacked: each holds several along a leading
+    layer dimension) as (first tensor, shape of one pool, device pointers)."""
+    pools = list(pools)
+    if not pools:
+        raise ValueError(f"{who}: no pools")
+    first = pools[0]
+    require_same_device(*pools)
+    ptrs = []
+    for t in pools:
+        if t.dtype not in (torch.bfloat16, torch.float32) or t.dtype != first.dtype or t.shape != first.shape or not t.is_contiguous():
+            raise ValueError(f"{who}: pools must be contiguous bf16 or fp32 tensors of one shape")
+        if stacked:
+            step = t.stride(0) * t.element_size()
+            ptrs += [t.data_ptr() + i * step for i in range(t.shape[0])]
+        else:
+            ptrs.append(t.data_ptr())
+    shape = first.shape[1:] if stacked else first.shape
+    if len(shape) < 2 or not all(shape):
+        raise ValueError(f"{who}: pools of shape {tuple(shape)}")
+    return first, tuple(shape), (ctypes.c_void_p * len(ptrs))(*ptrs), len(ptrs)
+
+
+def copy_entries(pools, dst: Sequence[int], src: Sequence[int], rows=None, stacked=False):
+    """pool[dst[i]] = pool[src[i]] for every pool and i, in place, in one launch (no counterpart in the reference, which copies layer by
+    layer with ``blit``): K/V pages, recurrent states or conv windows of all layers when a sequence is forked, checkpointed or moved.
+
+    pools: contiguous tensors [n_entries, ...] of one shape and type (bf16 or fp32); stacked=True: each has a leading layer dimension.
+    dst, src: host integers.  One source may be copied to many entries; no dst may repeat or be a src (ValueError).
+    rows (an int, or one per pair): only the first rows of every head of pages [n_entries, heads, page_size, dim] are copied.
+    Every 160 pairs take one launch."""
+    first, shape, ptrs, n_pools = _pool_ptrs("copy_entries", pools, stacked)
+    d, s = np.ascontiguousarray(dst, dtype=np.int32), np.ascontiguousarray(src, dtype=np.int32)
+    if d.ndim != 1 or d.shape != s.shape:
+        raise ValueError(f"copy_entries: {d.shape} destinations for {s.shape} sources")
+    n = d.size
+    if n == 0:
+        return
+    if min(d.min(), s.min()) < 0 or max(d.max(), s.max()) >= shape[0]:
+        raise ValueError(f"copy_entries: an entry outside [0, {shape[0]})")
+    targets = set(d.tolist())
+    if len(targets) < n or not targets.isdisjoint(s.tolist()):
+        raise ValueError("copy_entries: a destination is named twice, or is a source too")
+    item = first.element_size()
+    n_sub, sub_bytes, lens = 1, int(np.prod(shape[1:])) * item, None
+    if rows is not None:
+        if len(shape) != 4:
+            raise ValueError(f"copy_entries: rows needs pools [n_entries, heads, page_size, dim], got entries of {tuple(shape[1:])}")
+        r = np.asarray(rows, dtype=np.int64)
+        if r.ndim > 1 or (r.ndim == 1 and r.size != n) or r.min() < 0 or r.max() > shape[2]:
+            raise ValueError(f"copy_entries: rows must be one number or {n}, from 0 to {shape[2]}")
+        n_sub, sub_bytes = shape[1], shape[2] * shape[3] * item
+        lens = np.ascontiguousarray(np.broadcast_to(r * (shape[3] * item), (n,)), dtype=np.int64)
+    with on_device(first.device):
+        check(_lib.load().gdn_entries_copy(ptrs, n_pools, shape[0], n_sub, sub_bytes, d.ctypes.data, s.ctypes.data, lens.ctypes.data if lens is not None else None, n,
+                                           stream_ptr(first.device)), "copy_entries")
+
+
+def compact_rows(pools, block_table, base, keep, n_keep, dst_table=None, stacked=False):
+    """Row base[b] + keep[b, j] of sequence b moves to row base[b] + j for j < n_keep[b], in every pool and head, in one launch: the K/V
+    rows of an accepted path move together behind the context (base = ctx_len, keep / n_keep from ``accept_tree``), or any subset of a
+    sequence's rows to its front (base = 0).  No counterpart in the reference.
+
+    pools: page pools [n_pages, heads, page_size, dim] (bf16 or fp32; K and V of all layers), stacked=True: with a leading layer
+    dimension.  block_table int32 [B, max_pages]; base, n_keep int32 [B]; keep int32 [B, L], strictly ascending.  All on the device.
+    dst_table: the rows are written through this table instead (pages that the call does not read, or the same table): the
+    source keeps its rows.  From the first keep entry that is out of order or range the rest of a sequence is left alone and
+    ``_lib.device_status()`` reports it."""
+    first, shape, ptrs, n_pools = _pool_ptrs("compact_rows", pools, stacked)
+    dst_table = block_table if dst_table is None else dst_table
+    require_same_device(first, block_table, base, keep, n_keep, dst_table)
+    for name, t in (("block_table", block_table), ("dst_table", dst_table), ("base", base), ("keep", keep), ("n_keep", n_keep)):
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise ValueError(f"compact_rows: {name} must be contiguous int32")
+    if len(shape) != 4 or keep.dim() != 2 or block_table.dim() != 2:
+        raise ValueError("compact_rows: pools [n_pages, heads, page_size, dim], block_table [B, max_pages] and keep [B, L] expected")
+    B, L = keep.shape
+    if block_table.shape[0] != B or dst_table.shape != block_table.shape or base.shape != (B,) or n_keep.shape != (B,):
+        raise ValueError(f"compact_rows: shapes do not agree: block_table {tuple(block_table.shape)}, dst_table {tuple(dst_table.shape)}, base {tuple(base.shape)}, "
+                         f"keep {tuple(keep.shape)}, n_keep {tuple(n_keep.shape)}")
+    if block_table.shape[1] == 0:
+        raise ValueError("compact_rows: an empty block table")
+    n_pages, heads, page_size, dim = shape
+    with on_device(first.device):
+        check(_lib.load().gdn_rows_compact(ptrs, n_pools, n_pages, heads, page_size, dim * first.element_size(), ptr(block_table), ptr(dst_table),
+                                           block_table.shape[1], ptr(base), ptr(keep), ptr(n_keep), B, L, stream_ptr(first.device)), "compact_rows")
 
 
 class Pools:

@@ -10,10 +10,12 @@ Rollback after a verify is an index choice: the next round passes ``sel = n_new`
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
-from ._lib import check, ptr, stream_ptr
+from ._lib import check, on_device, ptr, require_same_device, stream_ptr
 from .batch import CD, DK, DV, HV, blit
 from .config import Cfg
 from .gated_delta import _f32
@@ -44,6 +46,114 @@ def accept_length(toks, ids):
     k = toks.shape[1] - 1
     eq = (toks[:, 1:] == ids[:, :k]).to(torch.int32)
     return torch.cumprod(eq, dim=1).sum(dim=1).to(torch.int32)
+
+
+def accept_tree(parents, toks, ids):
+    """The path of a tree that the target confirms, found on the device (``accept_length`` for trees): from the first root, as long as
+    there is one, to the lowest-numbered child whose token the target chose after its parent.
+
+    parents int32 [B, N] as for ``attn_tree``, N <= 64; toks int32 [B, N] the nodes' tokens (those of roots are taken as confirmed); ids
+    int32 [B, N] the target's token after every node.  Returns n_path int32 [B] and path int32 [B, N] (the path's nodes in order, then
+    -1): what ``deltanet_commit`` and ``compact_rows`` take.  The round's next token is ids[b, path[b, n_path[b] - 1]]."""
+    require_same_device(parents, toks, ids)
+    for t in (parents, toks, ids):
+        if t.dtype != torch.int32 or not t.is_contiguous() or t.dim() != 2 or t.shape != parents.shape:
+            raise ValueError("accept_tree: parents, toks and ids must be contiguous int32 [B, N]")
+    B, N = parents.shape
+    if not 1 <= N <= 64:
+        raise ValueError(f"accept_tree: 1 <= N <= 64 nodes, got {N}")
+    path = torch.empty_like(parents)
+    n_path = torch.empty((B,), dtype=torch.int32, device=parents.device)
+    with on_device(parents.device):
+        check(_lib.load().gdn_tree_accept(ptr(parents), ptr(toks), ptr(ids), ptr(path), ptr(n_path), B, N, stream_ptr(parents.device)), "accept_tree")
+    return n_path, path
+
+
+def deltanet_tree(proj, conv_pool, conv_w, A_log, dt_bias, ssm_pool, slots, pos, parents, out=None):
+    """Speculative verify of a TREE of drafted tokens on slot pools (no counterpart in the reference, whose ``deltanet_bm`` verifies a
+    chain and writes a state snapshot after every token).  Nothing in the pools changes: ``deltanet_commit`` advances them along the
+    path that was accepted.
+
+    proj [B*N, 8224] bf16 (row b*N+i = node i of sequence b, row stride a multiple of 4 elements); parents int32 [B, N] as for
+    ``attn_tree``, N <= 64; conv_pool, ssm_pool, slots, pos as for ``deltanet_b``.  Node i continues the conv window and the state that
+    its parent leaves.  Returns y [B*N, 2048] bf16; rows of unused nodes are zero.  Conv, silu, norms and gates are computed in fp32
+    and rounded nowhere before y; the chained kernels round to bf16 after each step, so the two agree to bf16 rounding."""
+    require_same_device(proj, conv_pool, conv_w, A_log, dt_bias, ssm_pool, slots, pos, parents, out)
+    proj, stride = _rows(proj)
+    if parents.dtype != torch.int32 or parents.dim() != 2 or not parents.is_contiguous():
+        raise ValueError("deltanet_tree: parents must be contiguous int32 [B, N]")
+    B, N = parents.shape
+    _check_pools("deltanet_tree", conv_pool, ssm_pool)
+    _check_index("deltanet_tree", B, slots=slots, pos=pos)
+    if not 1 <= N <= 64 or proj.shape[0] != B * N or stride % 4:
+        raise ValueError(f"deltanet_tree: 1 <= N <= 64 nodes and proj [B*N, 8224] with a row stride that is a multiple of 4 expected (B={B}, N={N}, proj {tuple(proj.shape)}, stride {stride})")
+    if out is None:
+        out = torch.empty((B * N, HV * DV), dtype=torch.bfloat16, device=proj.device)
+    elif out.dtype != torch.bfloat16 or not out.is_contiguous() or tuple(out.shape) != (B * N, HV * DV):
+        raise ValueError("deltanet_tree: out must be contiguous bf16 [B*N, 2048]")
+    cw = conv_w.to(torch.bfloat16).reshape(-1).contiguous()
+    with on_device(proj.device):
+        check(_lib.load().gdn_tree_verify(ptr(proj), stride, ptr(conv_pool), ptr(cw), ptr(_f32(A_log)), ptr(_f32(dt_bias)), ptr(ssm_pool), ptr(slots), ptr(pos),
+                                          ptr(parents), ssm_pool.shape[0], ptr(out), B, N, stream_ptr(proj.device)), "deltanet_tree")
+    return out
+
+
+def _check_pools(who, conv_pool, ssm_pool):
+    if ssm_pool.dtype != torch.float32 or not ssm_pool.is_contiguous() or ssm_pool.shape[1:] != (HV, DV, DK) or conv_pool.dtype != torch.bfloat16 \
+            or not conv_pool.is_contiguous() or conv_pool.shape != (2 * ssm_pool.shape[0], 3, CD):
+        raise ValueError(f"{who}: contiguous slot pools ssm fp32 [S, 16, 128, 128] and conv bf16 [2 S, 3, 6144] expected, got {tuple(ssm_pool.shape)} and {tuple(conv_pool.shape)}")
+
+
+def _check_index(who, B, **arrays):
+    for name, t in arrays.items():
+        if t.dtype != torch.int32 or t.shape != (B,) or not t.is_contiguous():
+            raise ValueError(f"{who}: {name} must be contiguous int32 [{B}]")
+
+
+def _layers(x):
+    """Device pointers of the layers of ``x``: a sequence of tensors, or one tensor with a leading layer dimension."""
+    if isinstance(x, torch.Tensor):
+        step = x.stride(0) * x.element_size()
+        return [x.data_ptr() + i * step for i in range(x.shape[0])]
+    return [t.data_ptr() for t in x]
+
+
+def deltanet_commit(projs, conv_pools, conv_ws, A_logs, dt_biases, ssm_pools, slots, pos, path, n_path, dst_slots=None):
+    """Advances the recurrent state and the conv window of every GatedDeltaNet layer along an accepted path, in one launch (no
+    counterpart in the reference).  Per layer, as a sequence of tensors or as one tensor with a leading layer dimension:
+    projs [B*N, 8224] bf16 (what ``deltanet_tree`` was called with), conv_pools / ssm_pools (slot pools), conv_ws bf16, A_logs and
+    dt_biases fp32.  slots, pos int32 [B]; path int32 [B, E], n_path int32 [B] from ``accept_tree`` (E may be smaller than N if no path is
+    longer).  The state after the path goes to slot dst_slots[b] (default: in place), the window to its buffer (pos + n_path) & 1.
+    No destination may be another sequence's slot in the same call.  n_path = 0 leaves a slot as it is (or copies it to its destination)."""
+    args = [projs, conv_pools, conv_ws, A_logs, dt_biases, ssm_pools]
+    L = len(ssm_pools)
+    if L == 0 or any(len(x) != L for x in args):
+        raise ValueError(f"deltanet_commit: every argument needs one entry per layer, got {[len(x) for x in args]}")
+    firsts = [x[0] for x in args]
+    proj, stride = _rows(firsts[0])
+    dst_slots = slots if dst_slots is None else dst_slots
+    require_same_device(*firsts, slots, pos, path, n_path, dst_slots)
+    _check_pools("deltanet_commit", firsts[1], firsts[5])
+    if path.dtype != torch.int32 or path.dim() != 2 or not path.is_contiguous():
+        raise ValueError("deltanet_commit: path must be contiguous int32 [B, E]")
+    B, E = path.shape
+    _check_index("deltanet_commit", B, slots=slots, pos=pos, n_path=n_path, dst_slots=dst_slots)
+    if firsts[2].dtype != torch.bfloat16 or firsts[2].numel() != CD * 4 or any(t.dtype != torch.float32 or t.numel() != HV for t in firsts[3:5]):
+        raise ValueError("deltanet_commit: conv_ws bf16 [6144*4], A_logs and dt_biases fp32 [16] per layer expected")
+    for x, first in zip(args, firsts):
+        if not (first.is_contiguous() or x is projs):
+            raise ValueError("deltanet_commit: weights and pools must be contiguous")
+        if not isinstance(x, torch.Tensor):
+            for t in x:
+                if t.shape != first.shape or t.dtype != first.dtype or t.stride() != first.stride() or t.device != first.device:
+                    raise ValueError("deltanet_commit: the layers' tensors must have one shape, type, layout and device")
+    N = proj.shape[0] // B if B else 1
+    if B and (N < 1 or proj.shape[0] != B * N):
+        raise ValueError(f"deltanet_commit: proj has {proj.shape[0]} rows for {B} sequences")
+    table = [(ctypes.c_void_p * L)(*_layers(x)) for x in args]
+    with on_device(proj.device):
+        check(_lib.load().gdn_tree_commit(table[0], stride, *table[1:], L, ptr(slots), ptr(dst_slots), ptr(pos), ptr(path), ptr(n_path), firsts[5].shape[0], B, N, E,
+                                          stream_ptr(proj.device)), "deltanet_commit")
 
 
 class SpecPools:

@@ -346,4 +346,159 @@ int gdn_hrec(void* hist, const void* rows, const int* slots, const int* pos, int
     return launch_hrec(hist, rows, slots, pos, B, n_slots, Lh, H, status, static_cast<cudaStream_t>(stream));
 }
 
+static int tree_common(const char* who, const int* parents, int B, int N) {
+    REQUIRE(parents || B == 0, GDN_E_NULL, "%s: null parents", who);
+    REQUIRE(B >= 0 && N >= 1 && N <= 64, GDN_E_SHAPE, "%s: B=%d N=%d (1 <= N <= 64 nodes)", who, B, N);
+    return GDN_OK;
+}
+
+size_t gqa_tree_attn_workspace_bytes(int B, int N, int H, int KV) {
+    if (B <= 0 || N <= 0 || H <= 0 || KV <= 0 || H % KV) return 0;
+    return tree_attn_workspace_bytes(B, N, H, KV);
+}
+
+int gqa_tree_attn(const void* q, const void* k_new, const void* v_new, void* k_pages, void* v_pages, const int* block_table, const int* ctx_len,
+                  const int* parents, void* out, void* workspace, size_t workspace_bytes, int B, int N, int H, int KV, int page_size, int max_pages,
+                  int n_pages, void* stream) {
+    int rc = tree_common("gqa_tree_attn", parents, B, N);
+    if (rc) return rc;
+    REQUIRE(H > 0 && KV > 0 && H % KV == 0 && H / KV <= 16, GDN_E_SHAPE, "gqa_tree_attn: H=%d KV=%d (H a multiple of KV, at most 16 query heads on one)", H, KV);
+    REQUIRE(page_size > 0 && max_pages > 0 && n_pages > 0, GDN_E_SHAPE, "gqa_tree_attn: page_size=%d max_pages=%d n_pages=%d", page_size, max_pages, n_pages);
+    if (B == 0) return GDN_OK;
+    REQUIRE(q && k_new && v_new && k_pages && v_pages && block_table && ctx_len && out && workspace, GDN_E_NULL, "gqa_tree_attn: null pointer");
+    REQUIRE(aligned16(q) && aligned16(k_new) && aligned16(v_new) && aligned16(k_pages) && aligned16(v_pages) && aligned16(out) && aligned16(workspace),
+            GDN_E_ALIGN, "gqa_tree_attn: tensors must be 16-byte aligned");
+    const size_t need = tree_attn_workspace_bytes(B, N, H, KV);
+    REQUIRE(workspace_bytes >= need, GDN_E_SHAPE, "gqa_tree_attn: workspace %zu < %zu bytes", workspace_bytes, need);
+    TreeAttnArgs a{};
+    a.q = static_cast<const __nv_bfloat16*>(q); a.k_new = static_cast<const __nv_bfloat16*>(k_new); a.v_new = static_cast<const __nv_bfloat16*>(v_new);
+    a.k_pages = static_cast<__nv_bfloat16*>(k_pages); a.v_pages = static_cast<__nv_bfloat16*>(v_pages);
+    a.block_table = block_table; a.ctx_len = ctx_len; a.parents = parents; a.out = static_cast<__nv_bfloat16*>(out);
+    a.B = B; a.N = N; a.H = H; a.KV = KV; a.page_size = page_size; a.max_pages = max_pages; a.n_pages = n_pages;
+    a.status = status_ptr();
+    REQUIRE(a.status, GDN_E_LAUNCH, "gqa_tree_attn: no CUDA device");
+    return launch_tree_attn(a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int gdn_tree_verify(const void* proj, long long row_stride, const void* conv_pool, const void* conv_w, const float* A_log, const float* dt_bias,
+                    const float* ssm_pool, const int* slots, const int* pos, const int* parents, int n_slots, void* y, int B, int N, void* stream) {
+    int rc = tree_common("gdn_tree_verify", parents, B, N);
+    if (rc) return rc;
+    REQUIRE(row_stride >= PW && row_stride % 4 == 0, GDN_E_SHAPE, "gdn_tree_verify: proj row stride %lld (need >= 8224 and a multiple of 4)", row_stride);
+    REQUIRE(n_slots > 0, GDN_E_SHAPE, "gdn_tree_verify: empty pool");
+    if (B == 0) return GDN_OK;
+    REQUIRE(proj && conv_pool && conv_w && A_log && dt_bias && ssm_pool && slots && pos && y, GDN_E_NULL, "gdn_tree_verify: null pointer");
+    REQUIRE(aligned16(ssm_pool) && ((uintptr_t)proj | (uintptr_t)conv_pool | (uintptr_t)conv_w | (uintptr_t)y) % 8 == 0, GDN_E_ALIGN,
+            "gdn_tree_verify: the state must be 16-byte aligned, rows 8-byte aligned");
+    TreeDeltaArgs a{};
+    a.proj = static_cast<const __nv_bfloat16*>(proj); a.row_stride = row_stride;
+    a.conv_pool = static_cast<const __nv_bfloat16*>(conv_pool); a.conv_w = static_cast<const __nv_bfloat16*>(conv_w);
+    a.A_log = A_log; a.dt_bias = dt_bias; a.ssm_pool = ssm_pool; a.slots = slots; a.pos = pos; a.parents = parents;
+    a.y = static_cast<__nv_bfloat16*>(y); a.B = B; a.N = N; a.n_slots = n_slots;
+    a.status = status_ptr();
+    REQUIRE(a.status, GDN_E_LAUNCH, "gdn_tree_verify: no CUDA device");
+    return launch_tree_verify(a, static_cast<cudaStream_t>(stream));
+}
+
+int gdn_tree_accept(const int* parents, const int* toks, const int* ids, int* path, int* n_path, int B, int N, void* stream) {
+    int rc = tree_common("gdn_tree_accept", parents, B, N);
+    if (rc) return rc;
+    if (B == 0) return GDN_OK;
+    REQUIRE(toks && ids && path && n_path, GDN_E_NULL, "gdn_tree_accept: null pointer");
+    int* status = status_ptr();
+    REQUIRE(status, GDN_E_LAUNCH, "gdn_tree_accept: no CUDA device");
+    return launch_tree_accept(parents, toks, ids, path, n_path, status, B, N, static_cast<cudaStream_t>(stream));
+}
+
+int gdn_tree_commit(const void* const* proj_host, long long row_stride, void* const* conv_pool_host, const void* const* conv_w_host,
+                    const void* const* A_log_host, const void* const* dt_bias_host, void* const* ssm_pool_host, int n_layers, const int* slots,
+                    const int* dst_slots, const int* pos, const int* path, const int* n_path, int n_slots, int B, int N, int E, void* stream) {
+    REQUIRE(n_layers >= 0 && B >= 0 && N >= 1 && E >= 0 && n_slots > 0, GDN_E_SHAPE, "gdn_tree_commit: n_layers=%d B=%d N=%d E=%d n_slots=%d", n_layers, B, N, E, n_slots);
+    REQUIRE(row_stride >= PW, GDN_E_SHAPE, "gdn_tree_commit: proj row stride %lld < 8224", row_stride);
+    if (B == 0 || n_layers == 0) return GDN_OK;
+    REQUIRE(proj_host && conv_pool_host && conv_w_host && A_log_host && dt_bias_host && ssm_pool_host && slots && dst_slots && pos && n_path && (path || E == 0),
+            GDN_E_NULL, "gdn_tree_commit: null pointer");
+    for (int l = 0; l < n_layers; l++) {
+        REQUIRE(proj_host[l] && conv_pool_host[l] && conv_w_host[l] && A_log_host[l] && dt_bias_host[l] && ssm_pool_host[l], GDN_E_NULL,
+                "gdn_tree_commit: null pointer in layer %d", l);
+        REQUIRE(aligned16(ssm_pool_host[l]) && (uintptr_t)conv_w_host[l] % 8 == 0, GDN_E_ALIGN, "gdn_tree_commit: layer %d: the state must be 16-byte aligned", l);
+    }
+    int* status = status_ptr();
+    REQUIRE(status, GDN_E_LAUNCH, "gdn_tree_commit: no CUDA device");
+    for (int l0 = 0; l0 < n_layers; l0 += TREE_MAX_LAYERS) {
+        TreeCommitArgs a{};
+        const int cnt = n_layers - l0 < TREE_MAX_LAYERS ? n_layers - l0 : TREE_MAX_LAYERS;
+        for (int l = 0; l < cnt; l++) {
+            a.proj[l] = static_cast<const __nv_bfloat16*>(proj_host[l0 + l]); a.conv_pool[l] = static_cast<__nv_bfloat16*>(conv_pool_host[l0 + l]);
+            a.conv_w[l] = static_cast<const __nv_bfloat16*>(conv_w_host[l0 + l]); a.A_log[l] = static_cast<const float*>(A_log_host[l0 + l]);
+            a.dt_bias[l] = static_cast<const float*>(dt_bias_host[l0 + l]); a.ssm_pool[l] = static_cast<float*>(ssm_pool_host[l0 + l]);
+        }
+        a.row_stride = row_stride; a.slots = slots; a.dst_slots = dst_slots; a.pos = pos; a.path = path; a.n_path = n_path;
+        a.status = status; a.B = B; a.N = N; a.E = E; a.n_slots = n_slots;
+        const int rc = launch_tree_commit(a, cnt, static_cast<cudaStream_t>(stream));
+        if (rc) return rc;
+    }
+    return GDN_OK;
+}
+
+int gdn_rows_compact(void* const* pools_host, int n_pools, int n_pages, int heads, int page_size, long long row_bytes, const int* block_table,
+                     const int* dst_table, int max_pages, const int* base, const int* keep, const int* n_keep, int B, int L, void* stream) {
+    REQUIRE(n_pools >= 0 && n_pages > 0 && heads > 0 && page_size > 0 && max_pages > 0 && row_bytes > 0 && row_bytes % 2 == 0 && B >= 0 && L >= 0, GDN_E_SHAPE,
+            "gdn_rows_compact: n_pools=%d n_pages=%d heads=%d page_size=%d max_pages=%d row_bytes=%lld B=%d L=%d", n_pools, n_pages, heads, page_size, max_pages,
+            row_bytes, B, L);
+    REQUIRE((long long)B * heads < (1ll << 31), GDN_E_SHAPE, "gdn_rows_compact: B=%d heads=%d", B, heads);
+    if (n_pools == 0 || B == 0 || L == 0) return GDN_OK;
+    REQUIRE(pools_host && block_table && dst_table && base && keep && n_keep, GDN_E_NULL, "gdn_rows_compact: null pointer");
+    int* status = status_ptr();
+    REQUIRE(status, GDN_E_LAUNCH, "gdn_rows_compact: no CUDA device");
+    for (int p0 = 0; p0 < n_pools; p0 += RC_MAX_POOLS) {
+        RowsArgs a{};
+        const int cnt = n_pools - p0 < RC_MAX_POOLS ? n_pools - p0 : RC_MAX_POOLS;
+        for (int p = 0; p < cnt; p++) {
+            REQUIRE(pools_host[p0 + p] && (uintptr_t)pools_host[p0 + p] % 2 == 0, GDN_E_NULL, "gdn_rows_compact: null or odd pool %d", p0 + p);
+            a.pool[p] = pools_host[p0 + p];
+        }
+        a.table = block_table; a.dst_table = dst_table; a.base = base; a.keep = keep; a.n_keep = n_keep; a.status = status;
+        a.row_bytes = row_bytes; a.B = B; a.L = L; a.heads = heads; a.page_size = page_size; a.max_pages = max_pages; a.n_pages = n_pages;
+        const int rc = launch_rows_compact(a, cnt, static_cast<cudaStream_t>(stream));
+        if (rc) return rc;
+    }
+    return GDN_OK;
+}
+
+int gdn_entries_copy(void* const* pools_host, int n_pools, long long n_entries, int n_sub, long long sub_bytes, const int* dst_host, const int* src_host,
+                     const long long* len_host, int n_pairs, void* stream) {
+    REQUIRE(n_pools >= 0 && n_entries > 0 && n_sub > 0 && sub_bytes > 0 && sub_bytes % 2 == 0 && n_pairs >= 0, GDN_E_SHAPE,
+            "gdn_entries_copy: n_pools=%d n_entries=%lld n_sub=%d sub_bytes=%lld n_pairs=%d", n_pools, n_entries, n_sub, sub_bytes, n_pairs);
+    if (n_pools == 0 || n_pairs == 0) return GDN_OK;
+    REQUIRE(pools_host && dst_host && src_host, GDN_E_NULL, "gdn_entries_copy: null pointer");
+    for (int p = 0; p < n_pools; p++) REQUIRE(pools_host[p] && (uintptr_t)pools_host[p] % 2 == 0, GDN_E_NULL, "gdn_entries_copy: null or odd pool %d", p);
+    for (int i = 0; i < n_pairs; i++) {
+        REQUIRE(dst_host[i] >= 0 && dst_host[i] < n_entries && src_host[i] >= 0 && src_host[i] < n_entries, GDN_E_INDEX,
+                "gdn_entries_copy: pair %d copies entry %d to %d of %lld", i, src_host[i], dst_host[i], n_entries);
+        REQUIRE(!len_host || (len_host[i] >= 0 && len_host[i] <= sub_bytes && len_host[i] % 2 == 0), GDN_E_SHAPE, "gdn_entries_copy: pair %d: %lld of %lld bytes", i,
+                len_host[i], sub_bytes);
+    }
+    for (int p0 = 0; p0 < n_pools; p0 += EC_MAX_POOLS)
+        for (int i0 = 0; i0 < n_pairs; i0 += EC_MAX_PAIRS) {
+            EntriesArgs a{};
+            const int pools = n_pools - p0 < EC_MAX_POOLS ? n_pools - p0 : EC_MAX_POOLS;
+            a.n_pairs = n_pairs - i0 < EC_MAX_PAIRS ? n_pairs - i0 : EC_MAX_PAIRS;
+            for (int p = 0; p < pools; p++) a.pool[p] = pools_host[p0 + p];
+            for (int i = 0; i < a.n_pairs; i++) {
+                a.dst[i] = dst_host[i0 + i]; a.src[i] = src_host[i0 + i];
+                a.len[i] = len_host ? len_host[i0 + i] : sub_bytes;
+            }
+            // whole entries are one run of bytes
+            a.entry_bytes = n_sub * sub_bytes; a.sub_bytes = sub_bytes; a.n_sub = n_sub;
+            if (!len_host) {
+                a.n_sub = 1; a.sub_bytes = a.entry_bytes;
+                for (int i = 0; i < a.n_pairs; i++) a.len[i] = a.entry_bytes;
+            }
+            const int rc = launch_entries_copy(a, pools, static_cast<cudaStream_t>(stream));
+            if (rc) return rc;
+        }
+    return GDN_OK;
+}
+
 }  // extern "C"

@@ -121,4 +121,68 @@ int launch_hrec(void* hist, const void* rows, const int* slots, const int* pos, 
 int launch_state_copy(void* dst, const void* src, int elem_size, long long n, long long d0, long long s0, int ny, long long dstride,
                       long long sstride, cudaStream_t st);
 
+constexpr int EC_MAX_POOLS = 64, EC_MAX_PAIRS = 160;              // per launch: the arguments fit the 4 KiB every launch may carry
+struct EntriesArgs {
+    void* pool[EC_MAX_POOLS];
+    int dst[EC_MAX_PAIRS], src[EC_MAX_PAIRS];
+    long long len[EC_MAX_PAIRS];      // bytes of each sub-block to copy
+    long long entry_bytes, sub_bytes; // an entry = n_sub sub-blocks
+    int n_sub, n_pairs;
+};
+int launch_entries_copy(const EntriesArgs& a, int n_pools, cudaStream_t st);
+
+constexpr int RC_MAX_POOLS = 64;
+struct RowsArgs {
+    void* pool[RC_MAX_POOLS];         // [n_pages, heads, page_size, row_bytes]
+    const int *table, *dst_table;     // [B, max_pages]
+    const int *base, *keep, *n_keep;  // [B], [B, L], [B]
+    int* status;
+    long long row_bytes;
+    int B, L, heads, page_size, max_pages, n_pages;
+};
+int launch_rows_compact(const RowsArgs& a, int n_pools, cudaStream_t st);
+
+// ---- tree_delta.cu ----
+struct TreeDeltaArgs {
+    const __nv_bfloat16* proj;        // [B*N, row_stride]
+    long long row_stride;
+    const __nv_bfloat16* conv_pool;   // [n_slots*2, 3, 6144]; buffer pos & 1 of the slot is read
+    const __nv_bfloat16* conv_w;      // [6144*4]
+    const float *A_log, *dt_bias;     // [16]
+    const float* ssm_pool;            // [n_slots, 16, 128, 128]
+    const int *slots, *pos, *parents; // [B], [B], [B, N]
+    __nv_bfloat16* y;                 // [B*N, 2048]
+    int* status;
+    int B, N, n_slots;
+};
+int launch_tree_verify(const TreeDeltaArgs& a, cudaStream_t st);
+
+constexpr int TREE_MAX_LAYERS = 32;
+struct TreeCommitArgs {
+    const __nv_bfloat16* proj[TREE_MAX_LAYERS];
+    __nv_bfloat16* conv_pool[TREE_MAX_LAYERS];
+    const __nv_bfloat16* conv_w[TREE_MAX_LAYERS];
+    const float* A_log[TREE_MAX_LAYERS];
+    const float* dt_bias[TREE_MAX_LAYERS];
+    float* ssm_pool[TREE_MAX_LAYERS];
+    long long row_stride;
+    const int *slots, *dst_slots, *pos, *path, *n_path;      // [B] each, path [B, E]
+    int* status;
+    int B, N, E, n_slots;
+};
+int launch_tree_commit(const TreeCommitArgs& a, int n_layers, cudaStream_t st);
+int launch_tree_accept(const int* parents, const int* toks, const int* ids, int* path, int* n_path, int* status, int B, int N, cudaStream_t st);
+
+// ---- tree_attn.cu ----
+struct TreeAttnArgs {
+    const __nv_bfloat16 *q, *k_new, *v_new;     // q [B*N,H,256]; k_new, v_new [B*N,KV,256]
+    __nv_bfloat16 *k_pages, *v_pages;           // [n_pages, KV, page_size, 256]
+    const int *block_table, *ctx_len, *parents; // [B, max_pages], [B], [B, N]
+    __nv_bfloat16* out;                         // [B*N,H,256]
+    int* status;
+    int B, N, H, KV, page_size, max_pages, n_pages;
+};
+size_t tree_attn_workspace_bytes(int B, int N, int H, int KV);
+int launch_tree_attn(const TreeAttnArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t st);
+
 }  // namespace gdn

@@ -13,7 +13,8 @@ from typing import List, Optional, Sequence
 import numpy as np
 import torch
 
-from .batch import CD, DK, DV, HV, attn_paged, blit, deltanet_b
+from .batch import CD, DK, DV, HV, attn_paged, attn_tree, blit, compact_rows, copy_entries, deltanet_b
+from .batch_spec import deltanet_commit, deltanet_tree
 from .config import Cfg
 from .prefix_cache import PagePool
 
@@ -70,6 +71,27 @@ class PagedPools:
         self.length[slot] = 0
         self._sync_row(slot)
 
+    def trim(self, slot: int):
+        """Give back the pages behind the slot's last cached token (a tree round reserves room for every node and keeps a few)."""
+        keep = -(-int(self.length[slot]) // self.pages.page_size)
+        if len(self.owned[slot]) > keep:
+            self.pages.release(self.owned[slot][keep:])
+            del self.owned[slot][keep:]
+            self._sync_row(slot)
+
+    def fork(self, slot: int, slots: Sequence[int]):
+        """The free slots ``slots`` continue the sequence in ``slot`` independently (parallel samples of one prompt): full K/V pages are
+        shared, the last page, the recurrent states and the conv windows of all layers are copied, one launch each."""
+        slots = list(slots)
+        if len(set(slots)) < len(slots) or not all(0 <= s < self.S and s != slot and not self.owned[s] for s in slots) or not 0 <= slot < self.S:
+            raise ValueError(f"fork: slot {slot} into {slots}: the destinations must be different free slots")
+        for s, pages in zip(slots, self.pages.fork(self.owned[slot], int(self.length[slot]), len(slots))):
+            self.owned[s] = pages
+            self.length[s] = self.length[slot]
+            self._sync_row(s)
+        copy_entries(self.ssm, slots, [slot] * len(slots))
+        copy_entries([c.view(self.S + 1, 2, 3, CD) for c in self.conv], slots, [slot] * len(slots))
+
     # ---- admission --------------------------------------------------------------------------------
     def _load_recurrent(self, slot: int, conv: Sequence[torch.Tensor], ssm: Sequence[torch.Tensor], pos: int):
         par = pos & 1                                                # the conv window of a slot alternates between two halves
@@ -117,6 +139,23 @@ class PagedPools:
         pool through the block table and appends the step's rows.  ``reserve`` must have made room for ctx_len + M tokens."""
         table = self.table.index_select(0, slots.long())
         return attn_paged(q, k_new, v_new, self.pages.K[layer], self.pages.V[layer], table, ctx_len, M=M, max_ctx=self.Lmax)
+
+    # ---- a round of tree speculation: attn_tree / deltanet_tree per layer, accept_tree, commit_tree, then advance and trim ----
+    def deltanet_tree(self, layer: int, proj, conv_w, A_log, dt_bias, slots: torch.Tensor, pos: torch.Tensor, parents: torch.Tensor, out=None):
+        """``batch_spec.deltanet_tree`` on this pool's conv / ssm of GatedDeltaNet layer ``layer``."""
+        return deltanet_tree(proj, self.conv[layer], conv_w, A_log, dt_bias, self.ssm[layer], slots, pos, parents, out=out)
+
+    def attn_tree(self, layer: int, q, k_new, v_new, slots: torch.Tensor, ctx_len: torch.Tensor, parents: torch.Tensor, out=None):
+        """``batch.attn_tree`` of full-attention layer ``layer``.  ``reserve`` must have made room for ctx_len + N tokens."""
+        table = self.table.index_select(0, slots.long())
+        return attn_tree(q, k_new, v_new, self.pages.K[layer], self.pages.V[layer], table, ctx_len, parents, out=out)
+
+    def commit_tree(self, projs, conv_ws, A_logs, dt_biases, slots: torch.Tensor, pos: torch.Tensor, path: torch.Tensor, n_path: torch.Tensor):
+        """Settles a round on the device, all layers in two launches: states and conv windows advance along the accepted path
+        (``deltanet_commit``, per-layer arguments as there), the K/V rows of the path move together behind the context
+        (``compact_rows``).  pos int32 [B] = tokens cached before the round.  The host follows with ``advance(slot, n_path)``."""
+        deltanet_commit(projs, self.conv, conv_ws, A_logs, dt_biases, self.ssm, slots, pos, path, n_path)
+        compact_rows(self.pages.K + self.pages.V, self.table.index_select(0, slots.long()), pos, path, n_path)
 
     def advance(self, slot: int, n: int):
         """Book-keeping after a step appended ``n`` rows to ``slot``."""

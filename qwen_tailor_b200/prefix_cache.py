@@ -80,12 +80,38 @@ class PagePool:
             if self.refs[p] == 0:
                 self.free.append(int(p))
 
+    def copy_pages(self, dst: Sequence[int], src: Sequence[int], n_rows: int):
+        """Rows [0, n_rows) of every (layer, K/V, head) of page src[i] -> page dst[i], for all i in one launch."""
+        if self.K[0].is_cuda:
+            from .batch import copy_entries
+            copy_entries(self.K + self.V, dst, src, rows=None if n_rows == self.page_size else n_rows)
+            return
+        row, per_head = self.head_dim, self.page_size * self.head_dim
+        for d, s in zip(dst, src):
+            for pool in self.K + self.V:
+                _copy_flat(pool, pool, n_rows * row, d * self.kv_heads * per_head, s * self.kv_heads * per_head, ny=self.kv_heads, dstride=per_head,
+                           sstride=per_head)
+
     def copy_rows(self, dst_page: int, src_page: int, n_rows: int):
         """Rows [0, n_rows) of every (layer, K/V, head) of src_page -> dst_page."""
-        row, per_head = self.head_dim, self.page_size * self.head_dim
-        for pool in self.K + self.V:
-            _copy_flat(pool, pool, n_rows * row, dst_page * self.kv_heads * per_head, src_page * self.kv_heads * per_head, ny=self.kv_heads,
-                       dstride=per_head, sstride=per_head)
+        self.copy_pages([dst_page], [src_page], n_rows)
+
+    def fork(self, pages: Sequence[int], n_tokens: int, n: int) -> List[List[int]]:
+        """Page lists of ``n`` new sequences that continue the ``n_tokens`` rows in ``pages`` independently: full pages are shared
+        (reference counts), a partly filled last page is copied for each, all copies in one launch.  The caller owns one reference
+        on every returned page.  MemoryError, with nothing changed, if the copies do not fit."""
+        full, tail = divmod(n_tokens, self.page_size)
+        if len(pages) * self.page_size < n_tokens:
+            raise ValueError(f"fork: {len(pages)} pages do not hold {n_tokens} rows")
+        if tail and self.available() < n:
+            raise MemoryError("prefix cache: the K/V page pool is exhausted")
+        forks = []
+        for _ in range(n):
+            self.retain(pages[:full])
+            forks.append(list(pages[:full]) + ([self.alloc()] if tail else []))
+        if tail and n:
+            self.copy_pages([f[full] for f in forks], [pages[full]] * n, tail)
+        return forks
 
     def write_rows(self, page: int, row0: int, kv: Sequence, src_row0: int, n_rows: int):
         """Rows [src_row0, src_row0 + n_rows) of dense buffers kv = [(K, V)] ([1, heads, L, dim]) -> rows [row0, ...) of ``page``."""

@@ -1,0 +1,573 @@
+"""GPU: operators for trees of drafted tokens and the cache copies around them, against the definitions in 64 bits (oracle/tree_oracle.py)."""
+import numpy as np
+import pytest
+import torch
+
+from conftest import bf16_dev, f32_dev, host, i32_dev
+from oracle import tree_oracle as tree
+from qwen_tailor_b200 import Cfg, _lib, synth
+from qwen_tailor_b200.batch import attn_paged, attn_tree, compact_rows, copy_entries
+from qwen_tailor_b200.batch_spec import accept_tree, deltanet_bm, deltanet_commit, deltanet_tree
+from qwen_tailor_b200.paged_pools import PagedPools
+
+pytestmark = pytest.mark.gpu
+
+HALF = 2.0 ** -8                # a rounding to bf16, relative to the value
+# attention before that rounding: scores are fp32 sums of 256 products (|q||k| / 16 <= ~24 here; 2^-21 of that at worst is < 2^-16 in the exponent), exp and
+# weights that are exact to 2^-16: together below 2^-14 of the same sums taken over |V|
+ATTN_ABS = 2.0 ** -14
+# y of the tree rule before its rounding: every product is exact to 2^-16 of its factors' norms; a path sums at most 64 terms weighted by |q.k| <= 0.09
+DELTA_ABS = 2.0 ** -12
+
+
+def random_tree(rng, N, used=None, kind="random"):
+    """parents [N]; nodes from `used` on are unused."""
+    used = N if used is None else used
+    p = np.full(N, -2, np.int32)
+    for i in range(used):
+        p[i] = {"chain": i - 1, "star": -1 if i == 0 else 0, "forest": -1 if i < 3 else rng.integers(0, i), "random": -1 if i == 0 else rng.integers(0, i)}[kind]
+    return p
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------------------------------------------------
+def attn_case(rng, ctx, N, page, H=8, KV=2, scale=1.0):
+    ctx = np.asarray(ctx, np.int64)
+    need = -(-(ctx + N) // page)
+    total = int(need.sum()) + 1
+    order = rng.permutation(total - 1) + 1
+    table = np.zeros((len(ctx), int(need.max()) + 1), np.int32)
+    o = 0
+    for b, n in enumerate(need):
+        table[b, :n] = order[o:o + n]
+        o += n
+    r = lambda *s: synth.bf16r(rng.standard_normal(s) * scale)  # noqa: E731
+    B = len(ctx)
+    return dict(q=r(B * N, H, 256), k_new=r(B * N, KV, 256), v_new=r(B * N, KV, 256), k_pages=r(total, KV, page, 256), v_pages=r(total, KV, page, 256), table=table,
+                ctx=ctx.astype(np.int32))
+
+
+def to_dev(c, dev):
+    return {k: i32_dev(v, dev) if v.dtype == np.int32 else bf16_dev(v, dev) for k, v in c.items()}
+
+
+def run_attn(d, parents):
+    return attn_tree(d["q"], d["k_new"], d["v_new"], d["k_pages"], d["v_pages"], d["table"], d["ctx"], parents)
+
+
+def context(c, b, X):
+    n, P = int(c["ctx"][b]), X.shape[2]
+    return np.concatenate([X[p] for p in c["table"][b]], axis=1)[:, :n] if n else np.zeros((X.shape[1], 0, 256), np.float32)
+
+
+def check_attn(c, parents, out, K1, V1, skip=()):
+    N, P = parents.shape[1], c["k_pages"].shape[2]
+    want_K, want_V = c["k_pages"].copy(), c["v_pages"].copy()
+    for b in range(len(c["ctx"])):
+        r = slice(b * N, (b + 1) * N)
+        ref, mag = tree.attn_tree(c["q"][r], c["k_new"][r], c["v_new"][r], context(c, b, c["k_pages"]), context(c, b, c["v_pages"]), parents[b])
+        err = np.abs(out[r] - ref)
+        assert (err <= HALF * np.abs(ref) + ATTN_ABS * mag + 1e-30).all(), (b, float((err - HALF * np.abs(ref)).max()), float(mag.max()))
+        for i, line in enumerate(tree.lines(parents[b])):
+            if line:
+                at = int(c["ctx"][b]) + i
+                want_K[c["table"][b, at // P], :, at % P], want_V[c["table"][b, at // P], :, at % P] = c["k_new"][b * N + i], c["v_new"][b * N + i]
+    assert np.array_equal(K1, want_K) and np.array_equal(V1, want_V), "only the rows of used nodes are appended"
+
+
+@pytest.mark.parametrize("ctx,N,page,kind,H,KV", [
+    ([0], 1, 64, "chain", 8, 2), ([1, 0, 63, 64, 65], 1, 64, "chain", 8, 2), ([700], 8, 64, "random", 8, 2), ([130, 0, 5, 64, 257], 13, 64, "forest", 8, 2),
+    ([511, 1025], 16, 128, "star", 8, 2), ([300, 77, 1], 33, 64, "random", 8, 2), ([64, 191, 1000], 64, 64, "chain", 8, 2), ([1300, 64], 64, 256, "random", 8, 2),
+    ([100, 47, 48, 0], 13, 48, "random", 8, 2), ([37, 90], 7, 1, "random", 8, 2), ([530, 3], 20, 37, "random", 8, 2), ([200, 64], 21, 16, "random", 8, 2),
+    ([150, 300], 31, 64, "random", 16, 2), ([150, 300], 11, 64, "random", 4, 4), ([129], 40, 64, "random", 24, 4), ([333, 10], 9, 64, "random", 32, 2),
+    ([90, 200], 64, 32, "random", 3, 3), ([5000, 2], 5, 64, "random", 8, 2),
+])
+def test_attn_tree(dev, ctx, N, page, kind, H, KV):
+    rng = np.random.default_rng(N * 1000 + page)
+    c = attn_case(rng, ctx, N, page, H, KV)
+    parents = np.stack([random_tree(rng, N, max(1, N - (3 * b) % 5), kind) for b in range(len(ctx))])
+    d = to_dev(c, dev)
+    out = run_attn(d, i32_dev(parents, dev))
+    assert out.shape == d["q"].shape and out.dtype == torch.bfloat16
+    check_attn(c, parents, host(out), host(d["k_pages"]), host(d["v_pages"]))
+    assert _lib.device_status() == 0
+
+
+def test_attn_tree_peaked_scores_and_many_sequences(dev):
+    """Large scores (one key takes almost all the weight, found late in the context) and more sequences than blocks."""
+    rng = np.random.default_rng(5)
+    ctx = rng.integers(0, 200, 90)
+    c = attn_case(rng, ctx, 3, 64, scale=3.0)
+    parents = np.stack([random_tree(rng, 3) for _ in ctx])
+    d = to_dev(c, dev)
+    out = host(run_attn(d, i32_dev(parents, dev)))
+    for b in range(len(ctx)):
+        r = slice(b * 3, b * 3 + 3)
+        ref, mag = tree.attn_tree(c["q"][r], c["k_new"][r], c["v_new"][r], context(c, b, c["k_pages"]), context(c, b, c["v_pages"]), parents[b])
+        # scores nine times as large: 9 x the exponent's error, 2^-13 + 2^-16 < 2^-12 of the sums over |V|
+        assert (np.abs(out[r] - ref) <= HALF * np.abs(ref) + 2.0 ** -12 * mag).all()
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("N", [3, 40])
+def test_attn_tree_nothing_leaks_from_masked_places(dev, N):
+    """NaN and infinities behind the context in its last page, in unused pages, in unused nodes and in siblings change nothing where
+    they are masked; where a node does see them it gets them."""
+    rng = np.random.default_rng(6)
+    ctx = [70, 5, 64, 0]
+    c = attn_case(rng, ctx, N, 64)
+    parents = np.stack([random_tree(rng, N, N - 1, "star") for _ in ctx])
+    clean = to_dev(c, dev)
+    ref = host(run_attn(clean, i32_dev(parents, dev)))
+    for X in (c["k_pages"], c["v_pages"]):
+        X[0] = np.nan
+        for b, n in enumerate(ctx):
+            seen = np.zeros((c["table"].shape[1], 64), bool)
+            seen.reshape(-1)[:n] = True
+            for p in range(-(-(n + N) // 64)):
+                X[c["table"][b, p]][:, ~seen[p]] = [np.nan, np.inf, -np.inf][b % 3]
+    for b in range(4):
+        c["k_new"][b * N + 1], c["v_new"][b * N + 1] = np.nan, [np.inf, np.nan][b % 2]      # node 1: a leaf of the star
+        c["k_new"][b * N + N - 1], c["v_new"][b * N + N - 1] = np.inf, np.nan                   # unused
+        c["q"][b * N + N - 1] = np.nan
+    d = to_dev(c, dev)
+    got = host(run_attn(d, i32_dev(parents, dev)))
+    for b in range(4):
+        for i in range(N):
+            if i != 1:
+                assert np.array_equal(got[b * N + i], ref[b * N + i]), (b, i)
+        assert np.isnan(got[b * N + 1]).all()
+        assert not got[b * N + N - 1].any()
+    # a finite key with a non-finite value: exactly the dimensions of the nodes that see it
+    c["k_new"][1], c["v_new"][1] = c["k_new"][0], c["v_new"][0]
+    c["v_new"][1][:, 7] = np.inf
+    got = host(run_attn(to_dev(c, dev), i32_dev(parents, dev)))
+    assert np.isposinf(got[1][:, 7]).all() and np.isfinite(np.delete(got[1], 7, 1)).all()
+    assert np.array_equal(got[0], ref[0]) and np.array_equal(got[2:N], ref[2:N])
+    assert _lib.device_status() == 0
+
+
+def test_attn_tree_reports_and_skips_what_is_malformed(dev):
+    rng = np.random.default_rng(7)
+    ctx = [40, 50, 60, 70]
+    c = attn_case(rng, ctx, 6, 64)
+    parents = np.stack([random_tree(rng, 6, kind="chain") for _ in ctx])
+    parents[1] = [-1, 0, 5, 1, 2, 0]                                 # node 2 hangs below a later node; 4 below 2
+    d = to_dev(c, dev)
+    out = host(run_attn(d, i32_dev(parents, dev)))
+    assert _lib.device_status() == 1
+    check_attn(c, parents, out, host(d["k_pages"]), host(d["v_pages"]))
+    assert not out[8].any() and not out[10].any()
+    # a context that does not fit its table, and a negative one: those sequences give zeros and write nothing
+    parents[1] = random_tree(rng, 6)
+    for bad in (c["table"].shape[1] * 64 - 5, -1, 2 ** 31 - 1):
+        c2 = dict(c, ctx=np.array([40, 50, bad, 70], np.int32))
+        d = to_dev(c2, dev)
+        out = host(run_attn(d, i32_dev(parents, dev)))
+        assert _lib.device_status() == 1
+        none = parents.copy()
+        none[2] = -2
+        check_attn(dict(c2, ctx=np.array([40, 50, 0, 70], np.int32)), none, out, host(d["k_pages"]), host(d["v_pages"]))
+    # a page number outside the pool: reported, nothing faults, the other sequences are right
+    c2 = dict(c, table=c["table"].copy())
+    c2["table"][3, 0] = 10 ** 6
+    d = to_dev(c2, dev)
+    out = host(run_attn(d, i32_dev(parents, dev)))
+    assert _lib.device_status() == 1
+    for b in range(3):
+        r = slice(6 * b, 6 * b + 6)
+        ref, mag = tree.attn_tree(c["q"][r], c["k_new"][r], c["v_new"][r], context(c, b, c["k_pages"]), context(c, b, c["v_pages"]), parents[b])
+        assert (np.abs(out[r] - ref) <= HALF * np.abs(ref) + ATTN_ABS * mag).all()
+
+
+def test_attn_tree_refusals(dev):
+    rng = np.random.default_rng(8)
+    c = attn_case(rng, [10, 20], 4, 64)
+    parents = np.stack([random_tree(rng, 4)] * 2)
+    d = to_dev(c, dev)
+    p = i32_dev(parents, dev)
+    run_attn(d, p)
+    for change in (dict(q=d["q"].float()), dict(q=d["q"][:, :7]), dict(q=d["q"][:7]), dict(k_new=d["k_new"][:, :1]), dict(table=d["table"].long()), dict(ctx=d["ctx"][:1]),
+                   dict(v_pages=d["v_pages"][:2]), dict(q=d["q"][..., :128].contiguous()), dict(table=d["table"][:1])):
+        with pytest.raises(ValueError):
+            run_attn({**d, **change}, p)
+    with pytest.raises(ValueError):
+        run_attn(d, p.long())
+    with pytest.raises(ValueError):
+        run_attn(d, torch.full((2, 65), -1, dtype=torch.int32, device=dev))
+    with pytest.raises(RuntimeError):
+        run_attn({**d, "q": d["q"].cpu()}, p)
+    with pytest.raises(ValueError):
+        attn_tree(d["q"], d["k_new"], d["v_new"], d["k_pages"], d["v_pages"], d["table"], d["ctx"], p, out=d["q"].float())
+    empty = attn_tree(d["q"][:0], d["k_new"][:0], d["v_new"][:0], d["k_pages"], d["v_pages"], d["table"][:0], d["ctx"][:0], p[:0])
+    assert empty.shape == (0, 8, 256)
+
+
+def test_attn_tree_of_a_chain_is_attn_paged(dev):
+    rng = np.random.default_rng(9)
+    ctx = [700, 64, 0, 129]
+    c = attn_case(rng, ctx, 4, 64)
+    a, b = to_dev(c, dev), to_dev(c, dev)
+    got = host(run_attn(a, i32_dev(np.tile(np.arange(4) - 1, (4, 1)), dev)))
+    ref = host(attn_paged(b["q"], b["k_new"], b["v_new"], b["k_pages"], b["v_pages"], b["table"], b["ctx"], M=4))
+    assert np.abs(got - ref).max() <= 2 * HALF * np.abs(ref).max()                # two roundings of values of one size
+    assert torch.equal(a["k_pages"], b["k_pages"]) and torch.equal(a["v_pages"], b["v_pages"])
+
+
+def test_attn_tree_captured_on_other_streams_and_repeatable(dev):
+    """Two captured graphs replayed in turn, a second stream, and the same bits every time."""
+    rng = np.random.default_rng(10)
+    cases = [(attn_case(rng, [900, 1500], 12, 64), 12), (attn_case(rng, [3000], 40, 64), 40)]
+    refs, graphs, outs, devs, ps = [], [], [], [], []
+    for c, N in cases:
+        d, p = to_dev(c, dev), i32_dev(np.stack([random_tree(rng, N) for _ in c["ctx"]]), dev)
+        refs.append(run_attn(d, p).clone())
+        devs.append(d), ps.append(p)
+        out = torch.empty_like(d["q"])
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            attn_tree(d["q"], d["k_new"], d["v_new"], d["k_pages"], d["v_pages"], d["table"], d["ctx"], p, out=out)
+        graphs.append(g), outs.append(out)
+    for _ in range(3):
+        for g, out, ref in zip(graphs, outs, refs):
+            out.fill_(7)
+            g.replay()
+            assert torch.equal(out, ref)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [run_attn(d, p) for d, p in zip(devs, ps)]
+    here = [run_attn(d, p) for d, p in zip(devs, ps)]                 # overlaps the other stream's calls (the appended rows are the same)
+    torch.cuda.synchronize()
+    for g, h, ref in zip(got, here, refs):
+        assert torch.equal(g, ref) and torch.equal(h, ref)
+    assert _lib.device_status() == 0
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# the gated delta rule
+# ---------------------------------------------------------------------------------------------------------------------
+def delta_case(rng, B, N, n_slots, layers=1):
+    A, dtb = zip(*(synth.layer_params(rng) for _ in range(layers)))
+    return dict(proj=synth.bf16r(rng.standard_normal((layers, B * N, 8224))), conv=synth.bf16r(rng.standard_normal((layers, n_slots * 2, 3, 6144))),
+                conv_w=np.stack([synth.conv_weights(rng) for _ in range(layers)]), A_log=np.stack(A), dt_bias=np.stack(dtb),
+                ssm=(rng.standard_normal((layers, n_slots, 16, 128, 128)) * 0.1).astype(np.float32),
+                slots=rng.permutation(n_slots)[:B].astype(np.int32), pos=rng.integers(0, 1000, B).astype(np.int32))
+
+
+def delta_dev(c, dev):
+    f32 = ("ssm", "A_log", "dt_bias")
+    return {k: i32_dev(v, dev) if v.dtype == np.int32 else f32_dev(v, dev) if k in f32 else bf16_dev(v, dev) for k, v in c.items()}
+
+
+def run_delta(d, parents, proj=None):
+    return deltanet_tree(d["proj"][0] if proj is None else proj, d["conv"][0], d["conv_w"][0], d["A_log"][0], d["dt_bias"][0], d["ssm"][0], d["slots"], d["pos"], parents)
+
+
+@pytest.mark.parametrize("B,N,kind", [(1, 1, "chain"), (3, 2, "chain"), (2, 8, "random"), (2, 13, "forest"), (2, 16, "star"), (1, 17, "random"), (2, 32, "random"), (1, 33, "chain"),
+                                      (2, 64, "random"), (1, 64, "chain"), (1, 63, "star"), (20, 5, "random")])
+def test_deltanet_tree(dev, B, N, kind):
+    rng = np.random.default_rng(B * 100 + N)
+    c = delta_case(rng, B, N, B + 2)
+    parents = np.stack([random_tree(rng, N, max(1, N - (2 * b) % 3), kind) for b in range(B)])
+    d = delta_dev(c, dev)
+    wide = torch.full((B * N, 8256), float("nan"), dtype=torch.bfloat16, device=dev)      # rows of a wider buffer
+    wide[:, :8224] = d["proj"][0]
+    keep = d["ssm"].clone(), d["conv"].clone()
+    for proj in (None, wide[:, :8224]):
+        y = host(run_delta(d, i32_dev(parents, dev), proj))
+        for b in range(min(B, 4)):
+            s, par = int(c["slots"][b]), int(c["pos"][b]) & 1
+            ref = tree.deltanet_tree(c["proj"][0, b * N:(b + 1) * N], c["conv"][0, 2 * s + par], c["conv_w"][0], c["A_log"][0], c["dt_bias"][0], c["ssm"][0, s], parents[b])
+            got = y[b * N:(b + 1) * N]
+            scale = np.abs(ref).reshape(N, 16, 128).max((0, 2)).repeat(128)
+            assert (np.abs(got - ref) <= HALF * np.abs(ref) + DELTA_ABS * scale).all(), (b, float((np.abs(got - ref) - HALF * np.abs(ref)).max()), float(scale.min()))
+            assert not got[[i for i, line in enumerate(tree.lines(parents[b])) if not line]].any()
+    assert torch.equal(d["ssm"], keep[0]) and torch.equal(d["conv"], keep[1]), "a verify changes nothing in the pools"
+    assert _lib.device_status() == 0
+
+
+def test_deltanet_tree_malformed_trees_slots_and_masked_nans(dev):
+    rng = np.random.default_rng(31)
+    c = delta_case(rng, 4, 6, 5)
+    parents = np.stack([random_tree(rng, 6, kind="star") for _ in range(4)])
+    d = delta_dev(c, dev)
+    good = host(run_delta(d, i32_dev(parents, dev))).reshape(4, 6, -1)
+    assert _lib.device_status() == 0
+    for field, bad in (("slots", 5), ("slots", -1), ("pos", -3)):
+        x = c[field].copy()
+        x[2] = bad
+        y = host(run_delta({**d, field: i32_dev(x, dev)}, i32_dev(parents, dev))).reshape(4, 6, -1)
+        assert _lib.device_status() == 1
+        assert not y[2].any() and np.array_equal(np.delete(y, 2, 0), np.delete(good, 2, 0))
+    p = parents.copy()
+    p[1] = [-1, 4, 0, 1, 0, 0]                                       # node 1 below a later node, node 3 below node 1
+    y = host(run_delta(d, i32_dev(p, dev))).reshape(4, 6, -1)
+    assert _lib.device_status() == 1
+    assert not y[1, [1, 3]].any() and np.allclose(y[1, [0, 2, 4, 5]], good[1, [0, 2, 4, 5]], atol=2 * HALF * np.abs(good[1]).max())
+    x = c["proj"].copy()
+    x[0, 0 * 6 + 3] = np.nan                                         # a leaf
+    x[0, 1 * 6 + 5] = np.inf                                         # an unused node
+    p = parents.copy()
+    p[1, 5] = -2
+    y = host(run_delta(d, i32_dev(p, dev), bf16_dev(x[0], dev))).reshape(4, 6, -1)
+    assert np.isnan(y[0, 3]).any() and np.array_equal(np.delete(y[0], 3, 0), np.delete(good[0], 3, 0)) and np.array_equal(y[1, :5], good[1, :5]) and not y[1, 5].any()
+    assert _lib.device_status() == 0
+    with pytest.raises(ValueError):
+        run_delta(d, i32_dev(parents, dev).long())
+    with pytest.raises(ValueError):
+        run_delta(d, torch.full((1, 65), -1, dtype=torch.int32, device=dev))
+    with pytest.raises(ValueError):
+        run_delta({**d, "slots": d["slots"][:3]}, i32_dev(parents, dev))
+    with pytest.raises(ValueError):
+        run_delta({**d, "ssm": d["ssm"][:, :3]}, i32_dev(parents, dev))
+    assert run_delta({**d, "slots": d["slots"][:0], "pos": d["pos"][:0]}, i32_dev(parents[:0], dev), d["proj"][0][:0]).shape == (0, 2048)
+
+
+def test_deltanet_tree_of_a_chain_agrees_with_deltanet_bm(dev):
+    rng = np.random.default_rng(32)
+    c = delta_case(rng, 2, 4, 3)
+    c["pos"][:] = [4, 7]
+    d = delta_dev(c, dev)
+    y = host(run_delta(d, i32_dev(np.tile(np.arange(4) - 1, (2, 1)), dev)))
+    ssm = torch.zeros(2, 4, 16, 128, 128, device=dev)
+    conv = torch.zeros(4, 4, 3, 6144, dtype=torch.bfloat16, device=dev)
+    for b in range(2):
+        s = int(c["slots"][b])
+        ssm[b, 0], conv[2 * b, 0] = d["ssm"][0, s], d["conv"][0, 2 * s + int(c["pos"][b]) % 2]
+    zero = i32_dev([0, 0], dev)
+    ref = host(deltanet_bm(d["proj"][0], conv, d["conv_w"][0], d["A_log"][0], d["dt_bias"][0], ssm, i32_dev([0, 1], dev), zero, zero, 4))
+    # the chained kernel rounds conv, silu, norm (twice) and gates to bf16: six roundings of 2^-9 each on factors of y
+    assert np.linalg.norm(y - ref) <= 6 * HALF * np.linalg.norm(ref)
+
+
+@pytest.mark.parametrize("B,N,lengths,layers", [(1, 1, [1], 1), (3, 8, [1, 4, 0], 3), (4, 40, [2, 40, 17, 16], 2), (2, 6, [2, 3], 34)])
+def test_deltanet_commit(dev, B, N, lengths, layers):
+    rng = np.random.default_rng(N + layers)
+    c = delta_case(rng, B, N, 2 * B + 1, layers)
+    path = np.full((B, N), -1, np.int32)
+    for b, n in enumerate(lengths):
+        path[b, :n] = np.sort(rng.permutation(N)[:n])
+    free = np.setdiff1d(np.arange(2 * B + 1), c["slots"])[:B].astype(np.int32)
+    for stacked, dst in ((True, None), (False, free), (True, np.where(np.arange(B) % 2, c["slots"], free).astype(np.int32))):
+        d = delta_dev(c, dev)
+        args = [d[k] if stacked else list(d[k]) for k in ("proj", "conv", "conv_w", "A_log", "dt_bias", "ssm")]
+        deltanet_commit(*args, d["slots"], d["pos"], i32_dev(path, dev), i32_dev(lengths, dev), dst_slots=None if dst is None else i32_dev(dst, dev))
+        ssm, conv = host(d["ssm"]), host(d["conv"])
+        want_ssm, want_conv = c["ssm"].astype(np.float64), c["conv"].copy()
+        for l in range(0, layers, 1 if layers < 5 else 11):
+            for b, n in enumerate(lengths):
+                s, t, pos = int(c["slots"][b]), int(c["slots"][b] if dst is None else dst[b]), int(c["pos"][b])
+                S, win = tree.commit(c["proj"][l, b * N:(b + 1) * N], c["conv"][l, 2 * s + (pos & 1)], c["conv_w"][l], c["A_log"][l], c["dt_bias"][l], c["ssm"][l, s], path[b, :n])
+                # fp32 sums of 128 products per step, at most 40 steps
+                assert np.abs(ssm[l, t] - S).max() <= 2.0 ** -16 * np.abs(S).max()
+                want_ssm[l, t], want_conv[l, 2 * t + ((pos + n) & 1)] = ssm[l, t], win
+            assert np.array_equal(ssm[l], want_ssm[l].astype(np.float32)) and np.array_equal(conv[l], want_conv[l]), "other slots and buffers stay as they are"
+    assert _lib.device_status() == 0
+
+
+def test_deltanet_commit_skips_what_is_out_of_range(dev):
+    rng = np.random.default_rng(41)
+    c = delta_case(rng, 3, 4, 4)
+    path, n = np.tile(np.arange(4, dtype=np.int32), (3, 1)), np.array([2, 2, 2], np.int32)
+    d = delta_dev(c, dev)
+    run = lambda d, path, n, **k: deltanet_commit(d["proj"], d["conv"], d["conv_w"], d["A_log"], d["dt_bias"], d["ssm"], d["slots"], d["pos"], i32_dev(path, dev), i32_dev(n, dev), **k)  # noqa: E731
+    run(d, path, n)
+    good = d["ssm"].clone(), d["conv"].clone()
+    s = int(c["slots"][1])
+    p_bad, n_bad = path.copy(), n.copy()
+    p_bad[1, 1], n_bad[1] = 4, 5
+    for change, kw in ((dict(path=p_bad), {}), (dict(n=n_bad), {}), ({}, dict(dst_slots=i32_dev([c["slots"][0], 9, c["slots"][2]], dev)))):
+        d = delta_dev(c, dev)
+        run(d, **{"path": path, "n": n, **change}, **kw)
+        assert _lib.device_status() == 1
+        ssm, conv = d["ssm"][0], d["conv"][0]
+        other = [i for i in range(4) if i != s]
+        assert torch.equal(ssm[other], good[0][0][other]) and np.array_equal(host(ssm)[s], c["ssm"][0, s]) and np.array_equal(host(conv)[2 * s:2 * s + 2], c["conv"][0, 2 * s:2 * s + 2])
+    with pytest.raises(ValueError):
+        deltanet_commit([], [], [], [], [], [], d["slots"], d["pos"], i32_dev(path, dev), i32_dev(n, dev))
+    with pytest.raises(ValueError):
+        run(d, path[:2], n)
+    with pytest.raises(ValueError):
+        run({**d, "conv_w": d["conv_w"].float()}, path, n)
+    with pytest.raises(ValueError):
+        run({**d, "proj": d["proj"][:, :11]}, path, n)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# accepting and copying
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("N,kind", [(1, "chain"), (7, "random"), (32, "star"), (33, "forest"), (64, "random"), (64, "chain")])
+def test_accept_tree(dev, N, kind):
+    rng = np.random.default_rng(N)
+    B = 37
+    parents = np.stack([random_tree(rng, N, int(rng.integers(0, N + 1)), kind) for _ in range(B)])
+    toks, ids = rng.integers(0, 3, (B, N)), rng.integers(0, 3, (B, N))
+    for b in range(0, B, 3):                                         # chains that are confirmed to the end
+        toks[b] = ids[b][np.maximum(parents[b], 0)]
+    n, path = accept_tree(i32_dev(parents, dev), i32_dev(toks, dev), i32_dev(ids, dev))
+    n, path = host(n), host(path)
+    for b in range(B):
+        want = tree.accept(parents[b], toks[b], ids[b])
+        assert n[b] == len(want) and path[b].tolist() == want + [-1] * (N - len(want))
+    assert _lib.device_status() == 0
+
+
+def test_accept_tree_malformed(dev):
+    parents = np.array([[-1, 2, 0, 1], [-1, -2, 1, 0]], np.int32)
+    z = i32_dev(np.zeros((2, 4)), dev)
+    n, path = accept_tree(i32_dev(parents, dev), z, z)
+    assert _lib.device_status() == 1
+    assert host(path).tolist() == [[0, 2, -1, -1], [0, 3, -1, -1]] and host(n).tolist() == [2, 2]
+    with pytest.raises(ValueError):
+        accept_tree(z.long(), z, z)
+    with pytest.raises(ValueError):
+        accept_tree(z, z[:1], z)
+    assert accept_tree(z[:0], z[:0], z[:0])[1].shape == (0, 4)
+
+
+@pytest.mark.parametrize("page,dim,dtype,L,elsewhere", [(64, 256, torch.bfloat16, 8, False), (16, 256, torch.bfloat16, 100, False), (5, 6, torch.bfloat16, 40, False), (8, 40, torch.float32, 33, True),
+                                                        (64, 256, torch.bfloat16, 70, True)])
+def test_compact_rows(dev, page, dim, dtype, L, elsewhere):
+    rng = np.random.default_rng(L)
+    base = np.array([0, 3, 77, page, 2 * page - 1], np.int32)
+    B, width = len(base), (77 + 2 * L) // page + 2
+    order = rng.permutation(2 * B * width) + 1
+    table, other = order[:B * width].reshape(B, width).astype(np.int32), order[B * width:].reshape(B, width).astype(np.int32)
+    pools = [torch.randn(2 * B * width + 1, 3, page, dim, device=dev).to(dtype) for _ in range(3)]
+    n_keep = np.array([L, 0, L // 2, 1, L - 1], np.int32)
+    keep = np.stack([np.sort(rng.permutation(2 * L)[:L]) for _ in base]).astype(np.int32)
+    keep[3] = np.arange(L)
+    want = [host(p).copy() for p in pools]
+    to = other if elsewhere else table
+    for X in want:
+        src = X.copy()
+        for b in range(B):
+            for j in range(n_keep[b]):
+                f, t = int(base[b] + keep[b, j]), int(base[b]) + j
+                X[to[b, t // page], :, t % page] = src[table[b, f // page], :, f % page]
+    compact_rows(pools, i32_dev(table, dev), i32_dev(base, dev), i32_dev(keep, dev), i32_dev(n_keep, dev), dst_table=i32_dev(other, dev) if elsewhere else None)
+    assert all(np.array_equal(host(p), X) for p, X in zip(pools, want))
+    assert _lib.device_status() == 0
+
+
+def test_compact_rows_stops_at_a_bad_entry(dev):
+    table = np.array([[1, 2], [3, 4], [5, 99], [6, 7]], np.int32)
+    pool = torch.arange(8 * 4 * 8, device=dev).float().view(8, 1, 4, 8)
+    want = host(pool).copy()
+    keep = np.array([[1, 3, 2], [1, 8, 9], [2, 4, 5], [2, 3, 5]], np.int32)      # out of order; beyond the table; a bad page; fine
+    for b, rows in ((0, [(0, 1), (1, 3)]), (1, [(0, 1)]), (2, [(0, 2)]), (3, [(0, 2), (1, 3), (2, 5)])):
+        for t, f in rows:
+            want[table[b, t // 4], :, t % 4] = host(pool)[table[b, f // 4], :, f % 4]
+    compact_rows([pool], i32_dev(table, dev), i32_dev([0] * 4, dev), i32_dev(keep, dev), i32_dev([3] * 4, dev))
+    assert _lib.device_status() == 1 and np.array_equal(host(pool), want)
+    for n, base in ((-1, 0), (4, 0), (3, -1)):
+        compact_rows([pool], i32_dev(table, dev), i32_dev([0, 0, 0, base], dev), i32_dev(keep, dev), i32_dev([0, 0, 0, n], dev))
+        assert _lib.device_status() == 1 and np.array_equal(host(pool), want)
+    t = i32_dev(table, dev)
+    z = i32_dev([0] * 4, dev)
+    for args in (([pool.half()], t, z, i32_dev(keep, dev), z), ([pool], t.long(), z, i32_dev(keep, dev), z), ([pool], t[:3], z, i32_dev(keep, dev), z), ([pool, pool[:3]], t, z, i32_dev(keep, dev), z),
+                 ([], t, z, i32_dev(keep, dev), z)):
+        with pytest.raises(ValueError):
+            compact_rows(*args)
+
+
+@pytest.mark.parametrize("shape,dtype,rows,stacked", [((40, 2, 64, 256), torch.bfloat16, None, False), ((40, 2, 64, 256), torch.bfloat16, 37, True), ((400, 2, 8, 16), torch.bfloat16, "each", False),
+                                                      ((9, 16, 128, 128), torch.float32, None, True), ((30, 3, 5, 3), torch.bfloat16, 2, False), ((30, 7), torch.float32, None, False), ((30, 3, 5, 3), torch.float32, 0, False)])
+def test_copy_entries(dev, shape, dtype, rows, stacked):
+    rng = np.random.default_rng(shape[0])
+    n = shape[0] // 2 - 1
+    order = rng.permutation(shape[0])
+    dst, src = order[:n].tolist(), rng.choice(order[n:], n).tolist()        # sources repeat
+    pools = [torch.randn((3, *shape) if stacked else shape, device=dev).to(dtype) for _ in range(2)]
+    want = [p.clone() for p in pools]
+    each = rng.integers(0, shape[2] + 1, n).tolist() if rows == "each" else [rows] * n
+    for X in want:
+        for Y in (X if stacked else [X]):
+            for d, s, r in zip(dst, src, each):
+                if r is None:
+                    Y[d] = Y[s]
+                else:
+                    Y[d, :, :r] = Y[s, :, :r]
+    copy_entries(pools, dst, src, rows=each if rows == "each" else rows, stacked=stacked)
+    assert all(torch.equal(p, X) for p, X in zip(pools, want))
+
+
+def test_copy_entries_refusals(dev):
+    p = torch.zeros(6, 2, 4, 8, device=dev)
+    copy_entries([p], [], [])
+    for dst, src, kw in (([1, 1], [0, 0], {}), ([1, 2], [0, 1], {}), ([6], [0], {}), ([0], [-1], {}), ([0, 1], [2], {}), ([1], [0], dict(rows=5)), ([1], [0], dict(rows=[1, 2])), ([1], [0], dict(rows=-1))):
+        with pytest.raises(ValueError):
+            copy_entries([p], dst, src, **kw)
+    for pools in ([], [p.half()], [p, p[:3]], [p.transpose(2, 3)]):
+        with pytest.raises(ValueError):
+            copy_entries(pools, [1], [0])
+    with pytest.raises(ValueError):
+        copy_entries([p.view(6, 64)], [1], [0], rows=1)
+    assert not p.any()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# together
+# ---------------------------------------------------------------------------------------------------------------------
+def test_rounds_of_tree_speculation_on_paged_pools(dev):
+    """Fork a prompt into two slots; three rounds of verify, accept and commit over all layers; the caches hold exactly the accepted tokens:
+    states and windows as the token-by-token rule leaves them, K/V rows in order, and the next round's attention sees them."""
+    rng = np.random.default_rng(77)
+    cfg = Cfg(layers=4)                                              # three GatedDeltaNet layers and a full-attention layer
+    nl, N, ctx0 = cfg.n_linear, 10, 61
+    pools = PagedPools(cfg, 4, 256, n_pages=30)
+    c = delta_case(rng, 1, 1, 1, nl)
+    kv = synth.bf16r(rng.standard_normal((2, 1, 2, ctx0, 256)))
+    state = dict(kv=[(bf16_dev(kv[0], dev), bf16_dev(kv[1], dev))], conv=[bf16_dev(x[:1], dev) for x in c["conv"]], ssm=[f32_dev(x[:1], dev) for x in c["ssm"]])
+    pools.admit(2, state, ctx0)
+    pools.fork(2, [0, 3])
+    seqs = [3, 2, 0]
+    B = len(seqs)
+    hist = [(kv[0, 0], kv[1, 0]) for _ in seqs]                      # K, V [2, n, 256] of every sequence
+    S = [[x[0].astype(np.float64) for x in c["ssm"]] for _ in seqs]
+    win = [[x[0].astype(np.float64) for x in c["conv"]] for _ in seqs]
+    weights = bf16_dev(c["conv_w"], dev), f32_dev(c["A_log"], dev), f32_dev(c["dt_bias"], dev)
+    slots = i32_dev(seqs, dev)
+    for _ in range(3):
+        lengths = [int(pools.length[s]) for s in seqs]
+        for s, n in zip(seqs, lengths):
+            pools.reserve(s, n + N)
+        pos = i32_dev(lengths, dev)
+        parents = np.stack([random_tree(rng, N, N - b) for b in range(B)])
+        proj = synth.bf16r(rng.standard_normal((nl, B * N, 8224)))
+        q, k, v = (synth.bf16r(rng.standard_normal((B * N, h, 256))) for h in (8, 2, 2))
+        ids = rng.integers(0, 2, (B, N)).astype(np.int32)
+        toks = rng.integers(0, 2, (B, N)).astype(np.int32)
+        p = i32_dev(parents, dev)
+        projs = [bf16_dev(x, dev) for x in proj]
+        ys = [host(pools.deltanet_tree(l, projs[l], weights[0][l], weights[1][l], weights[2][l], slots, pos, p)) for l in range(nl)]
+        o = host(pools.attn_tree(0, bf16_dev(q, dev), bf16_dev(k, dev), bf16_dev(v, dev), slots, pos, p))
+        n_path, path = accept_tree(p, i32_dev(toks, dev), i32_dev(ids, dev))
+        pools.commit_tree(projs, list(weights[0]), list(weights[1]), list(weights[2]), slots, pos, path, n_path)
+        for b, s in enumerate(seqs):
+            r = slice(b * N, (b + 1) * N)
+            ref, mag = tree.attn_tree(q[r], k[r], v[r], *hist[b], parents[b])
+            assert (np.abs(o[r] - ref) <= HALF * np.abs(ref) + ATTN_ABS * mag + 1e-30).all()
+            want = tree.accept(parents[b], toks[b], ids[b])
+            assert host(path)[b, :int(n_path[b])].tolist() == want
+            hist[b] = tuple(np.concatenate([h, x[r][want].transpose(1, 0, 2)], 1) for h, x in zip(hist[b], (k, v)))
+            pools.advance(s, len(want))
+            pools.trim(s)
+            n = int(pools.length[s])
+            for X, h in zip((pools.pages.K[0], pools.pages.V[0]), hist[b]):
+                rows = np.concatenate([host(X[pg]) for pg in pools.owned[s]], 1)
+                assert np.array_equal(rows[:, :n], h), "the accepted rows lie behind the context in order"
+            assert len(pools.owned[s]) == -(-n // 64)
+            for l in range(nl):
+                ref = tree.deltanet_tree(proj[l, r], win[b][l], c["conv_w"][l], c["A_log"][l], c["dt_bias"][l], S[b][l], parents[b])
+                scale = np.abs(ref).reshape(N, 16, 128).max((0, 2)).repeat(128)
+                assert (np.abs(ys[l][r] - ref) <= HALF * np.abs(ref) + DELTA_ABS * scale).all()
+                S[b][l], win[b][l] = tree.commit(proj[l, r], win[b][l], c["conv_w"][l], c["A_log"][l], c["dt_bias"][l], S[b][l], want)
+                assert np.abs(host(pools.ssm[l][s]) - S[b][l]).max() <= 2.0 ** -16 * np.abs(S[b][l]).max()
+                assert np.array_equal(host(pools.conv[l][2 * s + n % 2]), win[b][l])
+    for s in seqs:
+        pools.release(s)
+    assert pools.pages.available() == pools.pages.n_pages - 1
+    assert _lib.device_status() == 0
