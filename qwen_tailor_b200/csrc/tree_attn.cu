@@ -1,74 +1,767 @@
-// Attention of a tree of drafted tokens over a paged cache (see gqa_tree_attn in the header).
+// GQA attention, head_dim 256, of a tree of drafted tokens over a paged bf16 KV cache, on the Blackwell tensor cores.
+//
+// Node i of sequence b hangs below node parents[b][i] < i (or, -1, below the last cached token) and attends the cached keys
+// 0 .. ctx_len[b] - 1, its ancestors and itself:  softmax(q_i K^T / 16) V.  The chained verify (gqa_decode_tc.cu) has at most 16 query rows
+// per KV head; a tree has up to 64 nodes x (H / KV) query heads, so here the rows fill the 128 of a tensor-core tile and a K / V tile is
+// read once for all of them.  Bound: HBM (2 KiB per key and pair of KV heads) up to about 128 rows per KV head, the tensor pipe beyond.
+//
+// Work: a (sequence, KV head, row tile) triple is a "pair"; its keys come in 128-key tiles, the last tile holding the nodes themselves
+// (from the call's k_new / v_new).  The tiles of all pairs laid end to end are cut into equal ranges, one per SM, so that one long
+// sequence occupies the whole GPU as well as many short ones; a pair that is cut leaves fp32 partials, which a second small kernel
+// joins (overlapping its launch with this kernel's end).  Every block derives the plan from ctx_len itself.
+//
+// Roles: warps 0-3 softmax (one thread per query row; warps without rows sleep), warp 4 issues the MMAs, warp 5 is the TMA producer,
+// warp 6 appends the nodes' rows to the cache.  Per tile
+//     S [128 x 128]  = Q K^T      16 MMAs; K travels in slabs of 64 dims x 128 keys
+//     P              = 2^(S sc - m), written over S in tensor memory as bf16 hi + lo pairs (weights exact to 2^-17, as in the chained
+//                      and prefill kernels; hi alone would put an error of the size of the output's own rounding on every weight)
+//     O [128 x 256] += P V        16 MMAs; V travels in chunks of 32 keys x 256 dims, read N-major
+// with S / P double buffered, so the scores of the next tile (also of the next pair's first one) are formed while the softmax of this
+// one runs.  The running maximum is only raised when a tile exceeds it by more than 2^8, which keeps rescales of O rare.
+//
+// Pages: the boxes of the page maps hold gcd(page_size, 128) keys (K) and gcd(page_size, 32) keys (V), so a box never crosses a page and any
+// page size works; pages of a multiple of 32 / 128 keys take the fewest copies.  (The 128-byte swizzle goes by shared-memory address bits,
+// so small boxes side by side form the same image as one large box.)
+//
+// Masked places never reach the sums: scores are replaced, not multiplied; value rows behind the context and of unused nodes are zeroed in
+// shared memory; non-finite values of a node are zeroed there too (their weight is 0 for nodes that do not see it, and 0 x NaN is NaN)
+// and added back in the epilogue of the rows that do see it.
+// Every wait is bounded; one that gives up sets the device status word and the block runs out its loops.
+#include <cstring>
 #include "gqa_common.cuh"
+#include "sm100_prims.cuh"
 
 namespace gdn {
 
-// one warp per (sequence, node, query head)
-__global__ void __launch_bounds__(128) tree_attn_kernel(const TreeAttnArgs a) {
-    const int lane = threadIdx.x & 31, item = blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (item >= a.B * a.N * a.H) return;
-    const int h = item % a.H, i = item / a.H % a.N, b = item / a.H / a.N, kvh = h / (a.H / a.KV);
-    const int ctx = a.ctx_len[b];
-    const int* par = a.parents + (size_t)b * a.N;
-    uint4* out = reinterpret_cast<uint4*>(a.out + (size_t)item * ATT_D);
-    unsigned long long line = 0;
-    for (int at = i; at >= 0;) {
-        line |= 1ull << at;
-        const int p = par[at];
-        if (p >= at || (p < -1 && at != i)) { if (lane == 0) atomicExch(a.status, 1); }
-        if (p >= at || p < -1) { line = 0; break; }
-        at = p;
+using namespace sm100;
+
+constexpr int TA_THREADS = 224, TA_TK = 128;
+constexpr int TA_MAX_B = 256;                                         // sequences per launch (the plan lives in shared memory)
+constexpr int TA_SLOT = 16384, TA_NK = 5, TA_NV = 5;                  // K slab: 128 keys x 64 dims; V chunk: 32 keys x 256 dims
+constexpr int TA_Q_BYTES = 65536;                                     // 128 rows, or two buffers of up to 64 rows
+constexpr int TA_SMEM = TA_Q_BYTES + (TA_NK + TA_NV) * TA_SLOT;
+constexpr uint32_t TAM_O = 0, TAM_SP0 = 256;
+constexpr float TA_RAISE = 8.f;                                       // log2 units
+enum {
+    AB_QFULL = 0, AB_QEMPTY = 2, AB_KFULL = 4, AB_KEMPTY = AB_KFULL + TA_NK, AB_VFULL = AB_KEMPTY + TA_NK, AB_VEMPTY = AB_VFULL + TA_NV,
+    AB_SDONE = AB_VEMPTY + TA_NV, AB_PREADY = AB_SDONE + 2, AB_PFREE = AB_PREADY + 2, AB_ODONE = AB_PFREE + 2, AB_OFREE, AB_NODES, AB_DRAIN, AB_COUNT
+};
+
+struct TreeAttnPlan {
+    TreeAttnArgs a;
+    float* part;                 // [2 * G][64 column groups][rows][4]: partial O; then [2 * G][rows][2]: (m, l)
+    float* part_ml;
+    int* info;                   // [G][2]: the pair that starts in block g and goes on in the next ones, and its number of partials (0: none)
+    int G;                       // blocks
+    int group, nodes, rows;      // query heads per KV head, nodes per row tile, rows per tile
+    int row_tiles, q_bufs, q_slab;       // row tiles per (sequence, KV head); Q buffers; bytes of a Q slab (64 dims of all rows)
+    int k_box, v_box;            // keys per copy
+};
+
+struct TreeSeg { int b, kvh, rt, t0, n, tiles, ctx; bool more; };     // tiles [t0, t0 + n) of a pair with `tiles` of them; more: the block's range goes on
+
+// {i, ancestors} of nodes lane and lane + 32 of one tree, as bit masks (0 = unused); par0 / par1: their parents (-2 beyond N)
+__device__ __forceinline__ void warp_lines(int par0, int par1, unsigned long long& l0, unsigned long long& l1, bool& bad) {
+    const int lane = threadIdx.x & 31;
+    const bool late0 = par0 >= lane, late1 = par1 >= lane + 32;      // a parent that does not precede its child
+    if (late0) par0 = -2;
+    if (late1) par1 = -2;
+    bad = late0 || late1;
+    int at0 = par0 < -1 ? -2 : par0, at1 = par1 < -1 ? -2 : par1;    // >= 0: still walking, -1: reached the root, -2: unused
+    l0 = 1ull << lane; l1 = 1ull << (lane + 32);
+    const bool in0 = par0 >= -1, in1 = par1 >= -1;
+    while (__any_sync(0xffffffffu, at0 >= 0 || at1 >= 0)) {
+        if (at0 >= 0) l0 |= 1ull << at0;
+        if (at1 >= 0) l1 |= 1ull << at1;
+        const int a0 = __shfl_sync(0xffffffffu, par0, at0 & 31), b0 = __shfl_sync(0xffffffffu, par1, at0 & 31);
+        const int a1 = __shfl_sync(0xffffffffu, par0, at1 & 31), b1 = __shfl_sync(0xffffffffu, par1, at1 & 31);
+        if (at0 >= 0) at0 = at0 < 32 ? a0 : b0;
+        if (at1 >= 0) at1 = at1 < 32 ? a1 : b1;
     }
-    const long long rows = (long long)a.max_pages * a.page_size;
-    int last = a.N - 1;                                              // the last node in use
-    while (last >= 0 && par[last] < -1) last--;
-    if (ctx < 0 || (long long)ctx + last >= rows) { line = 0; if (lane == 0) atomicExch(a.status, 1); }
-    if (!line) { out[lane] = make_uint4(0, 0, 0, 0); return; }
-    float q[8], o[8] = {}, m = -INFINITY, l = 0.f;
-    auto unpack = [](uint4 u, float* f) {
-        unpack_bf16x4(make_uint2(u.x, u.y), f);
-        unpack_bf16x4(make_uint2(u.z, u.w), f + 4);
+    if (at0 != -1) l0 = 0;
+    if (at1 != -1) l1 = 0;
+    bad = bad || (in0 && !l0) || (in1 && !l1);
+}
+
+__device__ __forceinline__ unsigned long long shfl64(unsigned long long v, int src) {
+    return (unsigned long long)__shfl_sync(0xffffffffu, (uint32_t)v, src) | (unsigned long long)__shfl_sync(0xffffffffu, (uint32_t)(v >> 32), src) << 32;
+}
+
+__device__ __forceinline__ bool bf16_not_finite(uint32_t bits) { return (bits & 0x7f80u) == 0x7f80u; }
+
+// tile range [lo, hi) of block g when G blocks share N tiles
+__device__ __forceinline__ long long range_lo(int g, int G, long long N) { return (long long)g * N / G; }
+
+__global__ void __launch_bounds__(TA_THREADS, 1)
+tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmKn, const __grid_constant__ CUtensorMap tmVn) {
+    extern __shared__ __align__(1024) unsigned char smem[];
+    __shared__ uint64_t bars[AB_COUNT];
+    __shared__ long long s_cum[TA_MAX_B + 1];                        // tiles of all pairs of the sequences before
+    __shared__ unsigned long long s_badv[2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int s_abort;
+    const TreeAttnArgs& a = p.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t sbase = smem_addr(smem);
+    if (sbase & 1023u) { if (tid == 0) atomicExch(a.status, 4); return; }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");               // nothing an earlier kernel wrote is read before this
+
+    // ---- plan ----
+    const long long cap = (long long)a.max_pages * a.page_size;
+    const int PP = a.KV * p.row_tiles;
+    // context of sequence b as the kernel uses it, -1 = skipped (negative, or the nodes do not fit the table)
+    auto context = [&](int b) -> int {
+        const int ctx = a.ctx_len[b];
+        if (ctx < 0 || ctx > cap) return -1;
+        if ((long long)ctx + a.N > cap) {                            // (rare: only then do the tree's unused nodes matter)
+            int last = a.N - 1;
+            while (last >= 0 && a.parents[(size_t)b * a.N + last] < -1) last--;
+            if ((long long)ctx + last >= cap) return -1;
+        }
+        return ctx;
     };
-    unpack(reinterpret_cast<const uint4*>(a.q + (size_t)item * ATT_D)[lane], q);
-    auto step = [&](const uint4 ku, const uint4 vu) {
-        float k[8], v[8], s = 0.f;
-        unpack(ku, k); unpack(vu, v);
+    if (warp == 0) {
+        long long run = 0;
+        for (int b0 = 0; b0 < a.B; b0 += 32) {
+            const int b = b0 + lane;
+            int ctx = 0;
+            if (b < a.B) {
+                ctx = context(b);
+                if (ctx < 0) { if (blockIdx.x == 0) atomicExch(a.status, 1); ctx = 0; }
+            }
+            long long x = b < a.B ? (long long)((ctx + TA_TK - 1) / TA_TK + 1) * PP : 0;
+            const long long own = x;
 #pragma unroll
-        for (int c = 0; c < 8; c++) s = fmaf(q[c], k[c], s);
-        s = warp_sum(s) * 0.0625f;
-        const float mn = fmaxf(m, s), al = mn == -INFINITY ? 1.f : expf(m - mn), p = mn == -INFINITY ? 0.f : expf(s - mn);
-        m = mn; l = l * al + p;
-#pragma unroll
-        for (int c = 0; c < 8; c++) o[c] = fmaf(p, v[c], o[c] * al);
+            for (int o = 1; o < 32; o <<= 1) { const long long y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
+            if (b < a.B) s_cum[b] = run + x - own;
+            run += __shfl_sync(0xffffffffu, x, 31);
+        }
+        if (lane == 0) s_cum[a.B] = run;
+    }
+    auto bar = [&](int i) -> uint32_t { return smem_addr(&bars[i]); };
+    const int n_warps = (p.rows + 31) / 32;                          // softmax warps with rows
+    if (tid == 32) {
+        for (int i = 0; i < AB_COUNT; i++) mbar_init(bar(i), (i >= AB_PREADY && i < AB_PREADY + 2) || i == AB_OFREE || i == AB_NODES ? n_warps : 1);
+        s_abort = 0;
+        s_badv[0] = s_badv[1] = 0;
+        fence_barrier_init();
+        tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV); tma_prefetch_desc(&tmKn); tma_prefetch_desc(&tmVn);
+    }
+    if (warp == 4) { tmem_alloc(smem_addr(&tmem_slot), 512); tmem_relinquish(); }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tb = tmem_slot;
+    const long long N_all = s_cum[a.B];
+    const int G = (int)min((long long)gridDim.x, N_all);
+    const long long lo = (int)blockIdx.x < G ? range_lo(blockIdx.x, G, N_all) : 0, hi = (int)blockIdx.x < G ? range_lo(blockIdx.x + 1, G, N_all) : 0;
+
+    auto aborted = [&]() -> bool { return *(volatile int*)&s_abort != 0; };
+    auto wait = [&](int b, uint32_t parity) -> bool {                // bounded; a failure tells the whole block to stop computing
+        const uint32_t addr = bar(b);
+        for (uint32_t i = 0; i < 2000000u; i++) {
+            if (mbar_test_wait(addr, parity & 1u)) return true;
+            if ((i & 63u) == 63u && aborted()) return false;
+            __nanosleep(20);
+        }
+        atomicExch(&s_abort, 1);
+        atomicExch(a.status, 2);
+        return false;
     };
-    const int* table = a.block_table + (size_t)b * a.max_pages;
-    for (int t = 0; t < ctx; t++) {
-        int page = table[t / a.page_size];
-        if (page < 0 || page >= a.n_pages) { if (lane == 0) atomicExch(a.status, 1); page = 0; }
-        const size_t off = (((size_t)page * a.KV + kvh) * a.page_size + t % a.page_size) * ATT_D;
-        step(reinterpret_cast<const uint4*>(a.k_pages + off)[lane], reinterpret_cast<const uint4*>(a.v_pages + off)[lane]);
+    // the same for a whole warp: every lane gets the same answer, whatever a lane saw of an abort
+    auto warp_wait = [&](int b, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(b, parity)); };
+    // the part of the block's range that starts at tile x: it ends with the pair or with the range
+    auto segment = [&](long long x) -> TreeSeg {
+        int l = 0, r = a.B - 1;
+        while (l < r) { const int m = (l + r + 1) >> 1; if (s_cum[m] <= x) l = m; else r = m - 1; }
+        TreeSeg s;
+        s.b = l;
+        s.tiles = (int)((s_cum[l + 1] - s_cum[l]) / PP);
+        const long long off = x - s_cum[l];
+        const int pr = (int)(off / s.tiles);
+        s.t0 = (int)(off % s.tiles);
+        s.kvh = pr / p.row_tiles; s.rt = pr % p.row_tiles;
+        s.n = (int)min((long long)(s.tiles - s.t0), hi - x);
+        s.more = x + s.n < hi;
+        s.ctx = context(l);
+        return s;
+    };
+    const uint32_t sQ = sbase, sK = sbase + TA_Q_BYTES, sV = sK + TA_NK * TA_SLOT;
+    // keys of tile t of a segment's pair (the last tile holds the nodes)
+    auto limit_of = [&](const TreeSeg& s, int t) -> int { return t == s.tiles - 1 ? a.N : min(TA_TK, s.ctx - t * TA_TK); };
+
+    if (warp == 5) {
+        // ================= producer =================
+        uint64_t stream_policy;                                      // the cache is read once per row tile: first to leave L2 unless a second row tile follows
+        if (p.row_tiles == 1) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(stream_policy));
+        else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(stream_policy));
+        uint32_t nk = 0, nv = 0, nseg = 0;
+        bool okp = true;
+        for (long long x = lo; x < hi && okp; nseg++) {
+            const TreeSeg s = segment(x);
+            x += s.n;
+            const int qb = nseg % p.q_bufs;
+            if (nseg >= (uint32_t)p.q_bufs && !warp_wait(AB_QEMPTY + qb, nseg / p.q_bufs - 1)) { okp = false; break; }
+            if (lane == 0) {
+                mbar_expect_tx(bar(AB_QFULL + qb), p.rows * 512);
+                for (int j = 0; j < 4; j++)
+                    tma_load_3d(sQ + qb * (TA_Q_BYTES / 2) + j * p.q_slab, &tmQ, bar(AB_QFULL + qb), 64 * j, s.kvh * p.group, s.b * a.N + s.rt * p.nodes);
+            }
+            // page numbers: two windows of 32 table entries, one entry per lane, the later one requested while the earlier is used
+            const int* table = a.block_table + (size_t)s.b * a.max_pages;
+            const int pages = (int)((max(s.ctx, 0) + (long long)a.page_size - 1) / a.page_size);      // entries that hold context
+            auto entry = [&](int e) -> int {
+                if (e >= pages) return 0;
+                const int pg = table[e];
+                if (pg < 0 || pg >= a.n_pages) { atomicExch(a.status, 1); return 0; }      // reported; page 0 is read in its place
+                return pg;
+            };
+            int wk = (int)((long long)s.t0 * TA_TK / a.page_size), wv = wk;
+            int k_cur = entry(wk + lane), k_nxt = entry(wk + 32 + lane);
+            int v_cur = k_cur, v_nxt = k_nxt;
+            auto page_of = [&](int e, int& w, int& cur, int& nxt) -> int {
+                while (e >= w + 32) { w += 32; cur = nxt; nxt = entry(w + 32 + lane); }
+                return __shfl_sync(0xffffffffu, cur, e - w);
+            };
+            auto load_k = [&](int t) -> bool {
+                const int limit = limit_of(s, t);
+                const bool nodes = t == s.tiles - 1;
+                const int boxes = (limit + p.k_box - 1) / p.k_box;
+                for (int j = 0; j < 4; j++, nk++) {
+                    const int slot = nk % TA_NK;
+                    if (nk >= (uint32_t)TA_NK && !warp_wait(AB_KEMPTY + slot, nk / TA_NK - 1)) return false;
+                    if (lane == 0) {
+                        mbar_expect_tx(bar(AB_KFULL + slot), nodes ? 64 * 128 : boxes * p.k_box * 128);
+                        if (nodes) tma_load_3d(sK + slot * TA_SLOT, &tmKn, bar(AB_KFULL + slot), 64 * j, s.kvh, s.b * a.N);
+                    }
+                    if (nodes) continue;
+                    // (the windows only move forwards, so a slab walks the tile's boxes from a copy of them)
+                    int w = wk, cur = k_cur, nxt = k_nxt;
+                    for (int i = 0; i < boxes; i++) {
+                        const int key = t * TA_TK + i * p.k_box;
+                        const int page = page_of(key / a.page_size, w, cur, nxt);
+                        if (lane == 0)
+                            asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5, %6}], [%2], %7;"
+                                         ::"r"(sK + slot * TA_SLOT + i * p.k_box * 128), "l"(&tmK), "r"(bar(AB_KFULL + slot)), "r"(64 * j), "r"(key % a.page_size), "r"(s.kvh), "r"(page), "l"(stream_policy) : "memory");
+                    }
+                    if (j == 3) { wk = w; k_cur = cur; k_nxt = nxt; }
+                }
+                return true;
+            };
+            auto load_v = [&](int t) -> bool {
+                const int limit = limit_of(s, t);
+                const bool nodes = t == s.tiles - 1;
+                for (int c = 0; c < (limit + 31) / 32; c++, nv++) {
+                    const int slot = nv % TA_NV;
+                    if (nv >= (uint32_t)TA_NV && !warp_wait(AB_VEMPTY + slot, nv / TA_NV - 1)) return false;
+                    const int boxes = nodes ? 0 : (min(32, limit - 32 * c) + p.v_box - 1) / p.v_box;
+                    if (lane == 0) {
+                        mbar_expect_tx(bar(AB_VFULL + slot), nodes ? TA_SLOT : boxes * p.v_box * 512);
+                        if (nodes)
+                            for (int j = 0; j < 4; j++) tma_load_3d(sV + slot * TA_SLOT + j * 4096, &tmVn, bar(AB_VFULL + slot), 64 * j, s.kvh, s.b * a.N + 32 * c);
+                    }
+                    for (int i = 0; i < boxes; i++) {
+                        const int key = t * TA_TK + 32 * c + i * p.v_box;
+                        const int page = page_of(key / a.page_size, wv, v_cur, v_nxt);
+                        if (lane == 0)
+                            for (int j = 0; j < 4; j++)
+                                asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5, %6}], [%2], %7;"
+                                             ::"r"(sV + slot * TA_SLOT + j * 4096 + i * p.v_box * 128), "l"(&tmV), "r"(bar(AB_VFULL + slot)), "r"(64 * j), "r"(key % a.page_size), "r"(s.kvh), "r"(page), "l"(stream_policy) : "memory");
+                    }
+                }
+                return true;
+            };
+            okp = load_k(s.t0);
+            for (int t = s.t0; t < s.t0 + s.n && okp; t++) {
+                if (t + 1 < s.t0 + s.n) okp = load_k(t + 1);
+                if (okp) okp = load_v(t);
+            }
+        }
+        if (!okp && lane == 0) {                                     // gave up: the copies in flight have to land before the block leaves
+            for (int i = 0; i < TA_NK; i++) if (nk > (uint32_t)i) mbar_wait(bar(AB_KFULL + i), ((nk - 1 - i) / TA_NK) & 1, 100000u);
+            for (int i = 0; i < TA_NV; i++) if (nv > (uint32_t)i) mbar_wait(bar(AB_VFULL + i), ((nv - 1 - i) / TA_NV) & 1, 100000u);
+            for (int i = 0; i < p.q_bufs; i++) if (nseg + 1 > (uint32_t)i) mbar_wait(bar(AB_QFULL + i), ((nseg - i) / p.q_bufs) & 1, 100000u);
+        }
+    } else if (warp == 4) {
+        // ================= MMA issuer =================
+        if (lane == 0) {
+            constexpr uint32_t I_QK = idesc_bf16(128, 128, 0, 0), I_QN = idesc_bf16(128, 64, 0, 0);
+            constexpr uint32_t I_PV = idesc_bf16(128, 256, 0, 1);    // B = V read N-major (dims contiguous)
+            constexpr uint32_t HI = smem_desc_hi_sw128(1024);
+            uint32_t nk = 0, nv = 0, n = 0, nseg = 0;                // slabs, chunks, tiles and segments so far
+            bool ok = true;
+            // the P V product of tile m with `limit` keys; first / last: of its segment (the ps-th)
+            auto issue_pv = [&](uint32_t m, int limit, bool first, bool last, uint32_t ps) -> bool {
+                const uint32_t sp = tb + TAM_SP0 + (m & 1) * 128;
+                if (!wait(AB_PREADY + (m & 1), m >> 1)) return false;
+                if (first && ps > 0 && !wait(AB_OFREE, ps - 1)) return false;      // the epilogue before has read O
+                bool fresh = first;
+                for (int c = 0; 32 * c < limit; c++, nv++) {
+                    const int slot = nv % TA_NV;
+                    if (!wait(AB_VFULL + slot, nv / TA_NV)) return false;
+                    tc_fence_after_sync();
+                    const uint32_t vlo = smem_desc_lo(sV + slot * TA_SLOT, 4096);
+                    const int steps = limit - 32 * c > 16 ? 2 : 1;
+                    for (int part = 0; part < 2; part++)             // hi, lo
+                        for (int ks = 0; ks < steps; ks++) {
+                            const uint32_t acol = sp + 32 * c + 16 * part + 8 * ks;
+                            if (fresh) mma_ts_w<false>(tb + TAM_O, acol, vlo + ks * 128, HI, I_PV);
+                            else mma_ts_w<true>(tb + TAM_O, acol, vlo + ks * 128, HI, I_PV);
+                            fresh = false;
+                        }
+                    mma_commit(bar(AB_VEMPTY + slot));
+                }
+                mma_commit(bar(AB_PFREE + (m & 1)));
+                if (last) mma_commit(bar(AB_ODONE));
+                return true;
+            };
+            int p_limit = 0;
+            bool p_have = false, p_first = false, p_last = false;
+            uint32_t p_seg = 0;
+            for (long long x = lo; x < hi && ok; nseg++) {
+                const TreeSeg s = segment(x);
+                x += s.n;
+                const int qb = nseg % p.q_bufs;
+                if (!wait(AB_QFULL + qb, nseg / p.q_bufs)) { ok = false; break; }
+                const uint32_t qlo = smem_desc_lo(sQ + qb * (TA_Q_BYTES / 2), 16);
+                for (int t = s.t0; t < s.t0 + s.n && ok; t++, n++) {
+                    // the buffer of tile n held P of tile n - 2, whose product was issued before: MMAs of one thread run in order
+                    const uint32_t sp = tb + TAM_SP0 + (n & 1) * 128;
+                    const uint32_t idesc = t == s.tiles - 1 ? I_QN : I_QK;
+                    for (int j = 0; j < 4 && ok; j++, nk++) {
+                        const int slot = nk % TA_NK;
+                        if (!wait(AB_KFULL + slot, nk / TA_NK)) { ok = false; break; }
+                        tc_fence_after_sync();
+                        const uint32_t klo = smem_desc_lo(sK + slot * TA_SLOT, 16);
+#pragma unroll
+                        for (int kk = 0; kk < 4; kk++) {
+                            if (j == 0 && kk == 0) mma_ss_w<false>(sp, qlo + kk * 2, HI, klo + kk * 2, HI, idesc);
+                            else mma_ss_w<true>(sp, qlo + j * (p.q_slab >> 4) + kk * 2, HI, klo + kk * 2, HI, idesc);
+                        }
+                        mma_commit(bar(AB_KEMPTY + slot));
+                    }
+                    if (!ok) break;
+                    mma_commit(bar(AB_SDONE + (n & 1)));
+                    if (t == s.t0 + s.n - 1) mma_commit(bar(AB_QEMPTY + qb));
+                    if (p_have) ok = issue_pv(n - 1, p_limit, p_first, p_last, p_seg);
+                    p_have = true; p_limit = limit_of(s, t); p_first = t == s.t0; p_last = t == s.t0 + s.n - 1; p_seg = nseg;
+                }
+            }
+            if (ok && p_have) ok = issue_pv(n - 1, p_limit, p_first, p_last, p_seg);
+            if (!ok) { mma_commit(bar(AB_DRAIN)); mbar_wait(bar(AB_DRAIN), 0, 100000u); }      // gave up: nothing may run on after the block
+        }
+    } else if (warp == 6) {
+        // ================= append: the nodes' rows into the cache, by the block that has a pair's first tile =================
+        for (long long x = lo; x < hi;) {
+            const TreeSeg s = segment(x);
+            x += s.n;
+            if (s.t0 != 0 || s.rt != 0 || s.ctx < 0) continue;
+            const int* par = a.parents + (size_t)s.b * a.N;
+            unsigned long long l0, l1;
+            bool bad;
+            warp_lines(lane < a.N ? par[lane] : -2, lane + 32 < a.N ? par[lane + 32] : -2, l0, l1, bad);
+            if (bad) atomicExch(a.status, 1);
+            const unsigned long long used = __ballot_sync(0xffffffffu, l0 != 0) | (unsigned long long)__ballot_sync(0xffffffffu, l1 != 0) << 32;
+            const int* table = a.block_table + (size_t)s.b * a.max_pages;
+            for (int i = 0; i < a.N; i++) {
+                if (!(used >> i & 1)) continue;
+                const int at = s.ctx + i;
+                const int page = table[at / a.page_size];
+                if (page < 0 || page >= a.n_pages) { if (lane == 0) atomicExch(a.status, 1); continue; }
+                const size_t src = (((size_t)s.b * a.N + i) * a.KV + s.kvh) * ATT_D, dst = (((size_t)page * a.KV + s.kvh) * a.page_size + at % a.page_size) * ATT_D;
+                reinterpret_cast<uint4*>(a.k_pages + dst)[lane] = reinterpret_cast<const uint4*>(a.k_new + src)[lane];
+                reinterpret_cast<uint4*>(a.v_pages + dst)[lane] = reinterpret_cast<const uint4*>(a.v_new + src)[lane];
+            }
+        }
+    } else if (warp < n_warps) {
+        // ================= softmax and epilogue: thread = row = node * group + head =================
+        const float sc = 0.0625f * 1.4426950408889634f;              // 256^-1/2, scores kept in log2 units
+        const int row = tid, local = row / p.group;
+        const uint32_t tl = tb + ((uint32_t)(warp * 32) << 16);      // this warp's TMEM lanes
+        uint32_t n = 0, nv = 0, nseg = 0, node_tiles = 0;
+        bool ok = true;
+        for (long long x = lo; x < hi; nseg++) {
+            const TreeSeg s = segment(x);
+            x += s.n;
+            const int node = s.rt * p.nodes + local;
+            const bool real = row < p.rows && node < a.N;
+            const bool has_nodes = s.t0 + s.n == s.tiles;
+            int par0 = -2, par1 = -2;                                // requested early, used at the last tile
+            if (has_nodes && s.ctx >= 0) {
+                const int* par = a.parents + (size_t)s.b * a.N;
+                if (lane < a.N) par0 = par[lane];
+                if (lane + 32 < a.N) par1 = par[lane + 32];
+            }
+            unsigned long long line = 0, badv = 0;
+            float m_run = -INFINITY, l_run = 0.f;
+            for (int t = s.t0; t < s.t0 + s.n && ok; t++, n++) {
+                const int limit = limit_of(s, t), chunks = (limit + 31) / 32;
+                const bool nodes = t == s.tiles - 1;
+                const uint32_t sp = tl + TAM_SP0 + (n & 1) * 128;
+                if (!warp_wait(AB_SDONE + (n & 1), n >> 1)) { ok = false; break; }
+                tc_fence_after_sync();
+                unsigned long long used = 0;                         // (nodes tile) nodes in use
+                if (nodes) {                                         // the ancestors of this row's node
+                    unsigned long long l0, l1;
+                    bool bad;
+                    warp_lines(par0, par1, l0, l1, bad);
+                    used = __ballot_sync(0xffffffffu, l0 != 0) | (unsigned long long)__ballot_sync(0xffffffffu, l1 != 0) << 32;
+                    const unsigned long long x0 = shfl64(l0, node & 31), x1 = shfl64(l1, node & 31);
+                    line = real ? (node < 32 ? x0 : x1) : 0;
+                }
+                float sv[128];
+                {
+                    uint32_t r0[32], r1[32], r2[32], r3[32];
+                    tmem_ld32(sp, r0); tmem_ld32(sp + 32, r1);
+                    if (!nodes) { tmem_ld32(sp + 64, r2); tmem_ld32(sp + 96, r3); }
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        sv[i] = __uint_as_float(r0[i]); sv[32 + i] = __uint_as_float(r1[i]);
+                        sv[64 + i] = nodes ? -INFINITY : __uint_as_float(r2[i]); sv[96 + i] = nodes ? -INFINITY : __uint_as_float(r3[i]);
+                    }
+                }
+                if (nodes) {
+#pragma unroll
+                    for (int i = 0; i < 64; i++) sv[i] = (line >> i & 1) ? sv[i] : -INFINITY;
+                } else if (limit < TA_TK) {
+#pragma unroll
+                    for (int i = 0; i < 128; i++) sv[i] = i < limit ? sv[i] : -INFINITY;
+                }
+                float mt = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 128; i += 4) mt = fmaxf(mt, fmaxf(fmaxf(sv[i], sv[i + 1]), fmaxf(sv[i + 2], sv[i + 3])));
+                mt *= sc;                                            // (sc > 0: the maximum of the scaled scores)
+                // raise the reference only when it is far behind (or not set yet); O is rescaled then -- all lanes take part in the
+                // tensor-memory round trip, each with its own factor
+                const bool raise = mt > m_run + TA_RAISE || (m_run == -INFINITY && mt != -INFINITY);
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float m_new = raise ? mt : m_run;
+                    const float alpha = (m_run == -INFINITY) ? 0.f : exp2f(m_run - m_new);
+                    l_run *= alpha;
+                    m_run = m_new;
+                    if (t > s.t0) {                                  // O holds the tiles before this one: P V of tile n - 1 must have landed
+                        if (!warp_wait(AB_PFREE + ((n - 1) & 1), (n - 1) >> 1)) { ok = false; break; }
+                        tc_fence_after_sync();
+#pragma unroll 1
+                        for (int c0 = 0; c0 < 256; c0 += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(tl + TAM_O + c0, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                            tmem_st32(tl + TAM_O + c0, o);
+                        }
+                        tmem_wait_st();
+                    }
+                }
+                // p = 2^(s sc - m) (a masked score gives 0) as bf16 hi + lo, written over the scores group by group: the 32 score
+                // columns of keys 32 g .. 32 g + 31 become 16 columns of hi pairs and 16 columns of lo pairs
+                const float nm = (m_run == -INFINITY) ? 0.f : -m_run;
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    if (g >= chunks) continue;
+                    uint32_t ph[16], pl[16];
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        float p0, p1;
+                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(fmaf(sv[32 * g + i], sc, nm)));
+                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(fmaf(sv[32 * g + i + 1], sc, nm)));
+                        l_run += p0 + p1;
+                        ph[i >> 1] = pack_bf16x2(p0, p1);
+                        pl[i >> 1] = pack_bf16x2(p0 - __uint_as_float(ph[i >> 1] << 16), p1 - __uint_as_float(ph[i >> 1] & 0xffff0000u));
+                    }
+                    tmem_st16(sp + 32 * g, ph);
+                    tmem_st16(sp + 32 * g + 16, pl);
+                }
+                tmem_wait_st();
+                if (nodes || (limit & 15)) {
+                    // value rows that nobody may see, and a node's non-finite values, are zeroed before the product reads them.  These warps
+                    // do not wait for every phase of the V ring, and a parity cannot tell a phase from the one two before: once the
+                    // product of the tile before is done, the chunks before this tile's have all been consumed.
+                    if (n > 0 && !warp_wait(AB_PFREE + ((n - 1) & 1), (n - 1) >> 1)) { ok = false; break; }
+                    unsigned long long seen_bad = 0;
+                    // (nodes: all rows of its chunks; the last context tile: the rows behind the context, up to the next multiple of 16 keys)
+                    for (int c = nodes ? 0 : chunks - 1; c < chunks && ok; c++) {
+                        const int slot = (nv + c) % TA_NV;
+                        if (!warp_wait(AB_VFULL + slot, (nv + c) / TA_NV)) { ok = false; break; }
+                        const int r0 = nodes ? 0 : limit & 31, r1 = nodes ? 32 : (r0 + 15) & ~15;
+                        for (int i = row; i < (r1 - r0) * 32; i += n_warps * 32) {
+                            const int r = r0 + (i >> 5), k = 32 * c + r, ch = i & 31;
+                            uint4* at = reinterpret_cast<uint4*>(smem + TA_Q_BYTES + TA_NK * TA_SLOT + slot * TA_SLOT + (ch >> 3) * 4096 + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+                            if (!nodes || !(used >> k & 1)) { *at = make_uint4(0, 0, 0, 0); continue; }
+                            const uint4 v = *at;
+                            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                            bool hit = false;
+#pragma unroll
+                            for (int q = 0; q < 4; q++) {
+                                if (bf16_not_finite(w[q])) { w[q] &= 0xffff0000u; hit = true; }
+                                if (bf16_not_finite(w[q] >> 16)) { w[q] &= 0xffffu; hit = true; }
+                            }
+                            if (hit) { seen_bad |= 1ull << k; *at = make_uint4(w[0], w[1], w[2], w[3]); }
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    if (nodes) {
+                        if (seen_bad) atomicOr(&s_badv[node_tiles & 1], seen_bad);
+                        __threadfence_block();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bar(AB_NODES));
+                        ok = warp_wait(AB_NODES, node_tiles) && ok;
+                        badv = *(volatile unsigned long long*)&s_badv[node_tiles & 1];
+                        if (tid == 0) s_badv[(node_tiles + 1) & 1] = 0;      // (last read before this barrier)
+                        node_tiles++;
+                    }
+                    if (!ok) break;
+                }
+                nv += chunks;
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(AB_PREADY + (n & 1)));
+            }
+            if (!ok) break;
+            // ---- epilogue: O / l, or a partial (m, l, O) where the pair goes on in another block ----
+            if (!warp_wait(AB_ODONE, nseg)) break;
+            tc_fence_after_sync();
+            const bool whole = s.n == s.tiles;
+            const int slot = 2 * (int)blockIdx.x + (s.t0 == 0 ? 1 : 0);
+            float* part = p.part + (size_t)slot * (64 * 4) * p.rows;
+            const float inv = l_run == 0.f ? 1.f : 1.f / l_run;
+            __nv_bfloat16* orow = a.out + (((size_t)s.b * a.N + node) * a.H + s.kvh * p.group + (row - local * p.group)) * ATT_D;
+            const unsigned long long add = line & badv;
+#pragma unroll 1
+            for (int c0 = 0; c0 < 256; c0 += 32) {
+                uint32_t u[32];
+                tmem_ld32(tl + TAM_O + c0, u);
+                tmem_wait_ld();
+                if (add) {
+                    for (unsigned long long r = add; r; r &= r - 1) {
+                        const __nv_bfloat16* v = a.v_new + (((size_t)s.b * a.N + (__ffsll((long long)r) - 1)) * a.KV + s.kvh) * ATT_D + c0;
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            const float f = __bfloat162float(v[i]);
+                            if (!isfinite(f)) u[i] = __float_as_uint(__uint_as_float(u[i]) + f);
+                        }
+                    }
+                }
+                if (real && whole) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        uint4 v;
+                        v.x = pack_bf16x2(__uint_as_float(u[i]) * inv, __uint_as_float(u[i + 1]) * inv);
+                        v.y = pack_bf16x2(__uint_as_float(u[i + 2]) * inv, __uint_as_float(u[i + 3]) * inv);
+                        v.z = pack_bf16x2(__uint_as_float(u[i + 4]) * inv, __uint_as_float(u[i + 5]) * inv);
+                        v.w = pack_bf16x2(__uint_as_float(u[i + 6]) * inv, __uint_as_float(u[i + 7]) * inv);
+                        if (!line) v = make_uint4(0, 0, 0, 0);       // an unused node
+                        *reinterpret_cast<uint4*>(orow + c0 + i) = v;
+                    }
+                } else if (row < p.rows && !whole) {
+                    // partials are stored column group by column group, rows side by side: a warp writes 512 contiguous bytes
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<float4*>(part + ((size_t)((c0 + i) >> 2) * p.rows + row) * 4) =
+                            make_float4(__uint_as_float(u[i]), __uint_as_float(u[i + 1]), __uint_as_float(u[i + 2]), __uint_as_float(u[i + 3]));
+                }
+            }
+            if (row < p.rows && !whole) *reinterpret_cast<float2*>(p.part_ml + ((size_t)slot * p.rows + row) * 2) = make_float2(m_run, l_run);
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(AB_OFREE));
+            if (tid == 0 && !s.more) {
+                // the pair that starts in this block and goes on in the next ones is joined by the merge kernel
+                const long long first = hi - s.n - s.t0;
+                int parts = 0;
+                if (s.t0 == 0 && !whole) {
+                    parts = 1;
+                    while (range_lo(blockIdx.x + parts, G, N_all) < first + s.tiles) parts++;
+                }
+                p.info[2 * blockIdx.x] = (s.b * a.KV + s.kvh) * p.row_tiles + s.rt;
+                p.info[2 * blockIdx.x + 1] = parts;
+            }
+        }
     }
-    for (unsigned long long r = line; r; r &= r - 1) {
-        const size_t off = (((size_t)b * a.N + (__ffsll((long long)r) - 1)) * a.KV + kvh) * ATT_D;
-        step(reinterpret_cast<const uint4*>(a.k_new + off)[lane], reinterpret_cast<const uint4*>(a.v_new + off)[lane]);
+    if (tid == 0 && (lo >= hi || aborted())) p.info[2 * blockIdx.x + 1] = 0;
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 4) tmem_dealloc(tb, 512);
+}
+
+// Joins the partials of the pair that starts in main block blockIdx.x and is cut: 32 rows per block (rows side by side in memory), eight
+// warps taking 32 columns each.
+constexpr int TM_THREADS = 256;
+
+__global__ void __launch_bounds__(TM_THREADS) tree_attn_merge_kernel(const __grid_constant__ TreeAttnPlan p) {
+    __shared__ float s_w[149][32];
+    __shared__ __align__(16) __nv_bfloat16 s_out[32][ATT_D + 8];
+    __shared__ unsigned char s_live[32];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int g = blockIdx.x, parts = p.info[2 * g + 1];
+    if (parts == 0) return;
+    const TreeAttnArgs& a = p.a;
+    const int pair = p.info[2 * g], rt = pair % p.row_tiles, kvh = pair / p.row_tiles % a.KV, b = pair / p.row_tiles / a.KV;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.y * 32 + lane;
+    const bool in = row < p.rows;
+    const int node = rt * p.nodes + row / p.group;
+    auto slot = [&](int k) -> int { return k == 0 ? 2 * g + 1 : 2 * (g + k); };
+    if (warp == 0) {
+        // the rows' common maximum, the partials' weights over the row's sum
+        float mx = -INFINITY, sum = 0.f;
+        for (int k = 0; k < parts; k++) if (in) mx = fmaxf(mx, p.part_ml[((size_t)slot(k) * p.rows + row) * 2]);
+        for (int k = 0; k < parts; k++) {
+            const float2 ml = in ? *reinterpret_cast<const float2*>(p.part_ml + ((size_t)slot(k) * p.rows + row) * 2) : make_float2(-INFINITY, 0.f);
+            const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mx);
+            sum = fmaf(w, ml.y, sum);
+            s_w[k][lane] = w;
+        }
+        const float inv = sum == 0.f ? 1.f : 1.f / sum;
+        for (int k = 0; k < parts; k++) s_w[k][lane] *= inv;
+    } else if (warp == 1) {
+        unsigned long long l0, l1;
+        bool bad;
+        const int* par = a.parents + (size_t)b * a.N;
+        warp_lines(lane < a.N ? par[lane] : -2, lane + 32 < a.N ? par[lane + 32] : -2, l0, l1, bad);
+        const unsigned long long x0 = shfl64(l0, node & 31), x1 = shfl64(l1, node & 31);
+        s_live[lane] = in && node < a.N && (node < 32 ? x0 : x1) != 0;
     }
-    const float inv = l == 0.f ? 1.f : 1.f / l;
-    out[lane] = make_uint4(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv), pack_bf16x2(o[4] * inv, o[5] * inv), pack_bf16x2(o[6] * inv, o[7] * inv));
-    if (h % (a.H / a.KV) == 0) {                                     // the node's rows into the cache
-        const int page = table[(ctx + i) / a.page_size];
-        if (page < 0 || page >= a.n_pages) { if (lane == 0) atomicExch(a.status, 1); return; }
-        const size_t src = (((size_t)b * a.N + i) * a.KV + kvh) * ATT_D, dst = (((size_t)page * a.KV + kvh) * a.page_size + (ctx + i) % a.page_size) * ATT_D;
-        reinterpret_cast<uint4*>(a.k_pages + dst)[lane] = reinterpret_cast<const uint4*>(a.k_new + src)[lane];
-        reinterpret_cast<uint4*>(a.v_pages + dst)[lane] = reinterpret_cast<const uint4*>(a.v_new + src)[lane];
+    __syncthreads();
+    float4 acc[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (in) {
+#pragma unroll 2
+        for (int k = 0; k < parts; k++) {
+            const float w = s_w[k][lane];
+            const float4* src = reinterpret_cast<const float4*>(p.part) + ((size_t)slot(k) * 64 + warp * 8) * p.rows + row;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float4 o = __ldcg(src + (size_t)i * p.rows);
+                acc[i].x = fmaf(w, o.x, acc[i].x); acc[i].y = fmaf(w, o.y, acc[i].y); acc[i].z = fmaf(w, o.z, acc[i].z); acc[i].w = fmaf(w, o.w, acc[i].w);
+            }
+        }
+    }
+    const bool live = s_live[lane];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        *reinterpret_cast<uint2*>(&s_out[lane][warp * 32 + 4 * i]) = live ? make_uint2(pack_bf16x2(acc[i].x, acc[i].y), pack_bf16x2(acc[i].z, acc[i].w)) : make_uint2(0, 0);
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * 32; i += TM_THREADS) {
+        const int r = i >> 5, gr = blockIdx.y * 32 + r, nd = rt * p.nodes + gr / p.group;
+        if (gr < p.rows && nd < a.N)
+            reinterpret_cast<uint4*>(a.out + (((size_t)b * a.N + nd) * a.H + kvh * p.group + gr % p.group) * ATT_D)[i & 31] = *reinterpret_cast<const uint4*>(&s_out[r][(i & 31) * 8]);
     }
 }
 
-size_t tree_attn_workspace_bytes(int, int, int, int) { return 16; }
+// ---- host side ----
+static int tree_sms() {
+    static int sms[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return 148; }
+    if (!sms[dev]) {
+        int n = 0;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) { cudaGetLastError(); n = 148; }
+        sms[dev] = n < 148 ? n : 148;                                // (the merge kernel keeps the weights of at most 149 partials)
+    }
+    return sms[dev];
+}
 
-int launch_tree_attn(const TreeAttnArgs& a, void*, size_t, cudaStream_t st) {
-    if (a.B <= 0 || a.N <= 0) return GDN_OK;
-    tree_attn_kernel<<<(a.B * a.N * a.H + 3) / 4, 128, 0, st>>>(a);
+static void tree_shape(TreeAttnPlan& p, int N, int H, int KV) {
+    p.group = H / KV;
+    p.nodes = 128 / p.group < N ? 128 / p.group : N;
+    p.rows = p.nodes * p.group;
+    p.row_tiles = (N + p.nodes - 1) / p.nodes;
+    p.q_bufs = p.rows <= 64 ? 2 : 1;                                 // a second Q buffer hides the load between pairs where it fits
+    p.q_slab = (p.rows + 7) / 8 * 1024;
+}
+
+size_t tree_attn_workspace_bytes(int B, int N, int H, int KV) {
+    (void)B;
+    TreeAttnPlan p{};
+    tree_shape(p, N, H, KV);
+    const size_t G = 148;
+    return G * 16 + 2 * G * p.rows * (ATT_D + 2) * sizeof(float);
+}
+
+typedef CUresult (*TreeEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                 CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static bool tree_map(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims, const cuuint32_t* box) {
+    static TreeEncodeFn fn = nullptr;
+    if (!fn) {
+        cudaDriverEntryPointQueryResult qr;
+        void* f = nullptr;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &qr) != cudaSuccess || qr != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            return false;
+        }
+        fn = reinterpret_cast<TreeEncodeFn>(f);
+    }
+    cuuint64_t strides[3];
+    cuuint64_t s = 2;
+    for (int i = 0; i + 1 < rank; i++) { s *= dims[i]; strides[i] = s; }
+    const cuuint32_t es[4] = {1, 1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+static int gcd_of(int x, int y) { while (y) { const int r = x % y; x = y; y = r; } return x; }
+
+static int launch_pdl(const void* fn, dim3 grid, int threads, size_t smem, cudaStream_t st, void** args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    cudaLaunchKernelExC(&cfg, fn, args);
     return check_launch("tree_attn");
+}
+
+int launch_tree_attn(const TreeAttnArgs& all, void* workspace, size_t workspace_bytes, cudaStream_t st) {
+    (void)workspace_bytes;
+    static bool attr_set[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 0 && dev < 64 && !attr_set[dev]) {
+        if (cudaFuncSetAttribute(tree_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TA_SMEM) != cudaSuccess)
+            return check_launch("tree_attn smem attribute");
+        attr_set[dev] = true;
+    }
+    for (int b0 = 0; b0 < all.B; b0 += TA_MAX_B) {
+        TreeAttnPlan p{};
+        p.a = all;
+        TreeAttnArgs& a = p.a;
+        a.B = all.B - b0 < TA_MAX_B ? all.B - b0 : TA_MAX_B;
+        a.q += (size_t)b0 * a.N * a.H * ATT_D; a.out += (size_t)b0 * a.N * a.H * ATT_D;
+        a.k_new += (size_t)b0 * a.N * a.KV * ATT_D; a.v_new += (size_t)b0 * a.N * a.KV * ATT_D;
+        a.block_table += (size_t)b0 * a.max_pages; a.ctx_len += b0; a.parents += (size_t)b0 * a.N;
+        tree_shape(p, a.N, a.H, a.KV);
+        p.G = tree_sms();
+        p.info = static_cast<int*>(workspace);
+        p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + 148 * 16);
+        p.part = p.part_ml + 2 * 148 * (size_t)p.rows * 2;
+        p.k_box = gcd_of(a.page_size, TA_TK);
+        p.v_box = gcd_of(a.page_size, 32);
+        CUtensorMap tq, tk, tv, tkn, tvn;
+        const cuuint64_t dq[3] = {ATT_D, (cuuint64_t)a.H, (cuuint64_t)a.B * a.N}, dn[3] = {ATT_D, (cuuint64_t)a.KV, (cuuint64_t)a.B * a.N};
+        const cuuint64_t dp[4] = {ATT_D, (cuuint64_t)a.page_size, (cuuint64_t)a.KV, (cuuint64_t)a.n_pages};
+        const cuuint32_t bq[3] = {64, (cuuint32_t)p.group, (cuuint32_t)p.nodes}, bkn[3] = {64, 1, 64}, bvn[3] = {64, 1, 32};
+        const cuuint32_t bk[4] = {64, (cuuint32_t)p.k_box, 1, 1}, bv[4] = {64, (cuuint32_t)p.v_box, 1, 1};
+        if (!tree_map(&tq, a.q, 3, dq, bq) || !tree_map(&tk, a.k_pages, 4, dp, bk) || !tree_map(&tv, a.v_pages, 4, dp, bv) || !tree_map(&tkn, a.k_new, 3, dn, bkn) ||
+            !tree_map(&tvn, a.v_new, 3, dn, bvn)) {
+            set_error("gqa_tree_attn: tensor maps could not be made");
+            return GDN_E_UNSUPPORTED;
+        }
+        void* args[] = {&p, &tq, &tk, &tv, &tkn, &tvn};
+        int rc = launch_pdl((const void*)tree_attn_kernel, dim3(p.G), TA_THREADS, TA_SMEM, st, args);
+        if (rc) return rc;
+        void* margs[] = {&p};
+        rc = launch_pdl((const void*)tree_attn_merge_kernel, dim3(p.G, (p.rows + 31) / 32), TM_THREADS, 0, st, margs);
+        if (rc) return rc;
+    }
+    return GDN_OK;
 }
 
 }  // namespace gdn
