@@ -10,8 +10,8 @@
 // sequence occupies the whole GPU as well as many short ones; a pair that is cut leaves fp32 partials, which a second small kernel
 // joins (overlapping its launch with this kernel's end).  Every block derives the plan from ctx_len itself.
 //
-// Roles: warps 0-3 softmax (one thread per query row; warps without rows sleep), warp 4 issues the MMAs, warp 5 is the TMA producer,
-// warp 6 appends the nodes' rows to the cache.  Per tile
+// Roles: warps 0-3 softmax (one thread per query row; warps without rows sleep), warp 4 issues the MMAs, warps 5 and 6 are the TMA
+// producers of K and V, warp 7 appends the nodes' rows to the cache.  Per tile
 //     S [128 x 128]  = Q K^T      16 MMAs; K travels in slabs of 64 dims x 128 keys
 //     P              = 2^(S sc - m), written over S in tensor memory as bf16 hi + lo pairs (weights exact to 2^-17, as in the chained
 //                      and prefill kernels; hi alone would put an error of the size of the output's own rounding on every weight)
@@ -35,7 +35,7 @@ namespace gdn {
 
 using namespace sm100;
 
-constexpr int TA_THREADS = 224, TA_TK = 128;
+constexpr int TA_THREADS = 256, TA_TK = 128;
 constexpr int TA_MAX_B = 256;                                         // sequences per launch (the plan lives in shared memory)
 constexpr int TA_SLOT = 16384, TA_NK = 5, TA_NV = 5;                  // K slab: 128 keys x 64 dims; V chunk: 32 keys x 256 dims
 constexpr int TA_Q_BYTES = 65536;                                     // 128 rows, or two buffers of up to 64 rows
@@ -171,7 +171,11 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
         return false;
     };
     // the same for a whole warp: every lane gets the same answer, whatever a lane saw of an abort
-    auto warp_wait = [&](int b, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(b, parity)); };
+    auto warp_wait = [&](int b, uint32_t parity) -> bool {
+        int got = 0;
+        if (lane == 0) got = wait(b, parity);
+        return __shfl_sync(0xffffffffu, got, 0) != 0;
+    };
     // the part of the block's range that starts at tile x: it ends with the pair or with the range
     auto segment = [&](long long x) -> TreeSeg {
         int l = 0, r = a.B - 1;
@@ -192,97 +196,101 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
     // keys of tile t of a segment's pair (the last tile holds the nodes)
     auto limit_of = [&](const TreeSeg& s, int t) -> int { return t == s.tiles - 1 ? a.N : min(TA_TK, s.ctx - t * TA_TK); };
 
-    if (warp == 5) {
-        // ================= producer =================
+    if (warp == 5 || warp == 6) {
+        // ================= producers: warp 5 Q and K, warp 6 V =================
+        // Lane i works out page and row of box i of a tile (a tile has at most 32 boxes where the page size is a multiple of 4): done box
+        // by box the address arithmetic costs a warp more than the copies do (measured: 13 k cycles a tile against the 5.7 k that
+        // the memory needs).  Page numbers come in windows of 32 table entries, one per lane, the next window requested a window
+        // ahead: a plain load takes microseconds under the copies, and one per tile held the ring up (7.3 k cycles a tile).
+        const bool isk = warp == 5;
+        const int box = isk ? p.k_box : p.v_box, per_tile = TA_TK / box;
+        const int first_empty = isk ? AB_KEMPTY : AB_VEMPTY, first_full = isk ? AB_KFULL : AB_VFULL, ring = isk ? TA_NK : TA_NV;
+        const uint32_t base = isk ? sK : sV;
         uint64_t stream_policy;                                      // the cache is read once per row tile: first to leave L2 unless a second row tile follows
         if (p.row_tiles == 1) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(stream_policy));
         else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(stream_policy));
-        uint32_t nk = 0, nv = 0, nseg = 0;
+        uint32_t nr = 0, slot = 0, round = 0, nseg = 0;              // copies into the ring: their number, next slot, times around
         bool okp = true;
         for (long long x = lo; x < hi && okp; nseg++) {
             const TreeSeg s = segment(x);
             x += s.n;
-            const int qb = nseg % p.q_bufs;
-            if (nseg >= (uint32_t)p.q_bufs && !warp_wait(AB_QEMPTY + qb, nseg / p.q_bufs - 1)) { okp = false; break; }
-            if (lane == 0) {
-                mbar_expect_tx(bar(AB_QFULL + qb), p.rows * 512);
-                for (int j = 0; j < 4; j++)
-                    tma_load_3d(sQ + qb * (TA_Q_BYTES / 2) + j * p.q_slab, &tmQ, bar(AB_QFULL + qb), 64 * j, s.kvh * p.group, s.b * a.N + s.rt * p.nodes);
+            if (isk) {
+                const int qb = nseg % p.q_bufs;
+                if (nseg >= (uint32_t)p.q_bufs && !warp_wait(AB_QEMPTY + qb, nseg / p.q_bufs - 1)) { okp = false; break; }
+                if (lane == 0) {
+                    mbar_expect_tx(bar(AB_QFULL + qb), p.rows * 512);
+                    for (int j = 0; j < 4; j++)
+                        tma_load_3d(sQ + qb * (TA_Q_BYTES / 2) + j * p.q_slab, &tmQ, bar(AB_QFULL + qb), 64 * j, s.kvh * p.group, s.b * a.N + s.rt * p.nodes);
+                }
             }
-            // page numbers: two windows of 32 table entries, one entry per lane, the later one requested while the earlier is used
             const int* table = a.block_table + (size_t)s.b * a.max_pages;
-            const int pages = (int)((max(s.ctx, 0) + (long long)a.page_size - 1) / a.page_size);      // entries that hold context
-            auto entry = [&](int e) -> int {
-                if (e >= pages) return 0;
-                const int pg = table[e];
-                if (pg < 0 || pg >= a.n_pages) { atomicExch(a.status, 1); return 0; }      // reported; page 0 is read in its place
-                return pg;
+            const int entries = (int)(((long long)max(s.ctx, 0) + a.page_size - 1) / a.page_size);      // those that hold context
+            auto entry = [&](int e) -> int { return e < entries ? table[e] : 0; };
+            auto checked = [&](int pg) -> int {                      // a bad page number is reported, and page 0 read in its place
+                if (pg >= 0 && pg < a.n_pages) return pg;
+                atomicExch(a.status, 1);
+                return 0;
             };
-            int wk = (int)((long long)s.t0 * TA_TK / a.page_size), wv = wk;
-            int k_cur = entry(wk + lane), k_nxt = entry(wk + 32 + lane);
-            int v_cur = k_cur, v_nxt = k_nxt;
-            auto page_of = [&](int e, int& w, int& cur, int& nxt) -> int {
-                while (e >= w + 32) { w += 32; cur = nxt; nxt = entry(w + 32 + lane); }
-                return __shfl_sync(0xffffffffu, cur, e - w);
-            };
-            auto load_k = [&](int t) -> bool {
-                const int limit = limit_of(s, t);
-                const bool nodes = t == s.tiles - 1;
-                const int boxes = (limit + p.k_box - 1) / p.k_box;
-                for (int j = 0; j < 4; j++, nk++) {
-                    const int slot = nk % TA_NK;
-                    if (nk >= (uint32_t)TA_NK && !warp_wait(AB_KEMPTY + slot, nk / TA_NK - 1)) return false;
-                    if (lane == 0) {
-                        mbar_expect_tx(bar(AB_KFULL + slot), nodes ? 64 * 128 : boxes * p.k_box * 128);
-                        if (nodes) tma_load_3d(sK + slot * TA_SLOT, &tmKn, bar(AB_KFULL + slot), 64 * j, s.kvh, s.b * a.N);
-                    }
-                    if (nodes) continue;
-                    // (the windows only move forwards, so a slab walks the tile's boxes from a copy of them)
-                    int w = wk, cur = k_cur, nxt = k_nxt;
-                    for (int i = 0; i < boxes; i++) {
-                        const int key = t * TA_TK + i * p.k_box;
-                        const int page = page_of(key / a.page_size, w, cur, nxt);
-                        if (lane == 0)
-                            asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5, %6}], [%2], %7;"
-                                         ::"r"(sK + slot * TA_SLOT + i * p.k_box * 128), "l"(&tmK), "r"(bar(AB_KFULL + slot)), "r"(64 * j), "r"(key % a.page_size), "r"(s.kvh), "r"(page), "l"(stream_policy) : "memory");
-                    }
-                    if (j == 3) { wk = w; k_cur = cur; k_nxt = nxt; }
-                }
-                return true;
-            };
-            auto load_v = [&](int t) -> bool {
-                const int limit = limit_of(s, t);
-                const bool nodes = t == s.tiles - 1;
-                for (int c = 0; c < (limit + 31) / 32; c++, nv++) {
-                    const int slot = nv % TA_NV;
-                    if (nv >= (uint32_t)TA_NV && !warp_wait(AB_VEMPTY + slot, nv / TA_NV - 1)) return false;
-                    const int boxes = nodes ? 0 : (min(32, limit - 32 * c) + p.v_box - 1) / p.v_box;
-                    if (lane == 0) {
-                        mbar_expect_tx(bar(AB_VFULL + slot), nodes ? TA_SLOT : boxes * p.v_box * 512);
-                        if (nodes)
-                            for (int j = 0; j < 4; j++) tma_load_3d(sV + slot * TA_SLOT + j * 4096, &tmVn, bar(AB_VFULL + slot), 64 * j, s.kvh, s.b * a.N + 32 * c);
-                    }
-                    for (int i = 0; i < boxes; i++) {
-                        const int key = t * TA_TK + 32 * c + i * p.v_box;
-                        const int page = page_of(key / a.page_size, wv, v_cur, v_nxt);
-                        if (lane == 0)
-                            for (int j = 0; j < 4; j++)
-                                asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5, %6}], [%2], %7;"
-                                             ::"r"(sV + slot * TA_SLOT + j * 4096 + i * p.v_box * 128), "l"(&tmV), "r"(bar(AB_VFULL + slot)), "r"(64 * j), "r"(key % a.page_size), "r"(s.kvh), "r"(page), "l"(stream_policy) : "memory");
-                    }
-                }
-                return true;
-            };
-            okp = load_k(s.t0);
+            int w = (int)((long long)s.t0 * TA_TK / a.page_size);    // first entry of the current window
+            int cur = entry(w + lane), nxt = entry(w + 32 + lane);
             for (int t = s.t0; t < s.t0 + s.n && okp; t++) {
-                if (t + 1 < s.t0 + s.n) okp = load_k(t + 1);
-                if (okp) okp = load_v(t);
+                const int limit = limit_of(s, t);
+                const bool nodes = t == s.tiles - 1;
+                int page = 0, row = 0;                               // of this lane's box
+                if (!nodes && per_tile <= 32) {
+                    const int first = t * TA_TK / a.page_size;
+                    while (first >= w + 32) { w += 32; cur = nxt; nxt = entry(w + 32 + lane); }
+                    const int key = min(t * TA_TK + lane * box, s.ctx - 1), e = key / a.page_size - w;      // (boxes behind the context are not copied)
+                    row = key - (w + e) * a.page_size;
+                    const int p0 = __shfl_sync(0xffffffffu, cur, e & 31), p1 = __shfl_sync(0xffffffffu, nxt, e & 31);
+                    page = checked(e < 32 ? p0 : p1);
+                }
+                // K: four slabs of 64 dims, all boxes each; V: chunks of 32 keys, its boxes whole rows
+                const int steps = isk ? 4 : (limit + 31) / 32;
+                for (int j = 0; j < steps; j++) {
+                    if (round > 0 && !warp_wait(first_empty + slot, round - 1)) { okp = false; break; }
+                    const uint32_t full = bar(first_full + slot), dst = base + slot * TA_SLOT;
+                    const int i0 = isk ? 0 : j * (32 / box);         // the step's boxes [i0, i0 + cnt)
+                    const int cnt = nodes ? 0 : ((isk ? limit : min(32, limit - 32 * j)) + box - 1) / box;
+                    if (lane == 0) {
+                        mbar_expect_tx(full, nodes ? (isk ? 64 * 128 : TA_SLOT) : cnt * box * (isk ? 128 : 512));
+                        if (nodes && isk) tma_load_3d(dst, &tmKn, full, 64 * j, s.kvh, s.b * a.N);
+                        if (nodes && !isk)
+                            for (int k = 0; k < 4; k++) tma_load_3d(dst + k * 4096, &tmVn, full, 64 * k, s.kvh, s.b * a.N + 32 * j);
+                    }
+                    for (int i = 0; i < cnt; i++) {
+                        int pg, rw;
+                        if (per_tile <= 32) {
+                            pg = __shfl_sync(0xffffffffu, page, i0 + i);
+                            rw = __shfl_sync(0xffffffffu, row, i0 + i);
+                        } else {                                     // (page sizes that are not a multiple of 4: looked up in place)
+                            const int key = t * TA_TK + (i0 + i) * box, e = key / a.page_size;
+                            rw = key - e * a.page_size;
+                            pg = checked(table[e]);
+                        }
+                        if (lane == 0) {
+                            const uint32_t to = dst + i * box * 128;
+                            if (isk)
+                                asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5, %6, %7}], [%2], %8;"
+                                             ::"r"(to), "l"(&tmK), "r"(full), "r"(0), "r"(rw), "r"(j), "r"(s.kvh), "r"(pg), "l"(stream_policy) : "memory");
+                            else if (box == 32)                      // the four 64-dim blocks of 32 rows are the chunk's image
+                                asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5, %6, %7}], [%2], %8;"
+                                             ::"r"(to), "l"(&tmV), "r"(full), "r"(0), "r"(rw), "r"(0), "r"(s.kvh), "r"(pg), "l"(stream_policy) : "memory");
+                            else
+                                for (int k = 0; k < 4; k++)
+                                    asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5, %6, %7}], [%2], %8;"
+                                                 ::"r"(to + k * 4096), "l"(&tmV), "r"(full), "r"(0), "r"(rw), "r"(k), "r"(s.kvh), "r"(pg), "l"(stream_policy) : "memory");
+                        }
+                    }
+                    nr++;
+                    if (++slot == (uint32_t)ring) { slot = 0; round++; }
+                }
+                GDN_TSTAMP((int)(x - s.n - lo + t - s.t0) * 16 + (isk ? 8 : 9));
             }
         }
         if (!okp && lane == 0) {                                     // gave up: the copies in flight have to land before the block leaves
-            for (int i = 0; i < TA_NK; i++) if (nk > (uint32_t)i) mbar_wait(bar(AB_KFULL + i), ((nk - 1 - i) / TA_NK) & 1, 100000u);
-            for (int i = 0; i < TA_NV; i++) if (nv > (uint32_t)i) mbar_wait(bar(AB_VFULL + i), ((nv - 1 - i) / TA_NV) & 1, 100000u);
-            for (int i = 0; i < p.q_bufs; i++) if (nseg + 1 > (uint32_t)i) mbar_wait(bar(AB_QFULL + i), ((nseg - i) / p.q_bufs) & 1, 100000u);
+            for (int i = 0; i < ring; i++) if (nr > (uint32_t)i) mbar_wait(bar(first_full + i), ((nr - 1 - i) / ring) & 1, 100000u);
+            if (isk) for (int i = 0; i < p.q_bufs; i++) if (nseg + 1 > (uint32_t)i) mbar_wait(bar(AB_QFULL + i), ((nseg - i) / p.q_bufs) & 1, 100000u);
         }
     } else if (warp == 4) {
         // ================= MMA issuer =================
@@ -297,6 +305,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                 const uint32_t sp = tb + TAM_SP0 + (m & 1) * 128;
                 if (!wait(AB_PREADY + (m & 1), m >> 1)) return false;
                 if (first && ps > 0 && !wait(AB_OFREE, ps - 1)) return false;      // the epilogue before has read O
+                GDN_TSTAMP(m * 16 + 2);
                 bool fresh = first;
                 for (int c = 0; 32 * c < limit; c++, nv++) {
                     const int slot = nv % TA_NV;
@@ -315,6 +324,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                 }
                 mma_commit(bar(AB_PFREE + (m & 1)));
                 if (last) mma_commit(bar(AB_ODONE));
+                GDN_TSTAMP(m * 16 + 3);
                 return true;
             };
             int p_limit = 0;
@@ -330,6 +340,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                     // the buffer of tile n held P of tile n - 2, whose product was issued before: MMAs of one thread run in order
                     const uint32_t sp = tb + TAM_SP0 + (n & 1) * 128;
                     const uint32_t idesc = t == s.tiles - 1 ? I_QN : I_QK;
+                    GDN_TSTAMP(n * 16 + 0);
                     for (int j = 0; j < 4 && ok; j++, nk++) {
                         const int slot = nk % TA_NK;
                         if (!wait(AB_KFULL + slot, nk / TA_NK)) { ok = false; break; }
@@ -344,6 +355,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                     }
                     if (!ok) break;
                     mma_commit(bar(AB_SDONE + (n & 1)));
+                    GDN_TSTAMP(n * 16 + 1);
                     if (t == s.t0 + s.n - 1) mma_commit(bar(AB_QEMPTY + qb));
                     if (p_have) ok = issue_pv(n - 1, p_limit, p_first, p_last, p_seg);
                     p_have = true; p_limit = limit_of(s, t); p_first = t == s.t0; p_last = t == s.t0 + s.n - 1; p_seg = nseg;
@@ -352,7 +364,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
             if (ok && p_have) ok = issue_pv(n - 1, p_limit, p_first, p_last, p_seg);
             if (!ok) { mma_commit(bar(AB_DRAIN)); mbar_wait(bar(AB_DRAIN), 0, 100000u); }      // gave up: nothing may run on after the block
         }
-    } else if (warp == 6) {
+    } else if (warp == 7) {
         // ================= append: the nodes' rows into the cache, by the block that has a pair's first tile =================
         for (long long x = lo; x < hi;) {
             const TreeSeg s = segment(x);
@@ -402,6 +414,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                 const uint32_t sp = tl + TAM_SP0 + (n & 1) * 128;
                 if (!warp_wait(AB_SDONE + (n & 1), n >> 1)) { ok = false; break; }
                 tc_fence_after_sync();
+                if (warp == 0) GDN_TSTAMP(n * 16 + 4);
                 unsigned long long used = 0;                         // (nodes tile) nodes in use
                 if (nodes) {                                         // the ancestors of this row's node
                     unsigned long long l0, l1;
@@ -411,28 +424,30 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                     const unsigned long long x0 = shfl64(l0, node & 31), x1 = shfl64(l1, node & 31);
                     line = real ? (node < 32 ? x0 : x1) : 0;
                 }
-                float sv[128];
-                {
-                    uint32_t r0[32], r1[32], r2[32], r3[32];
-                    tmem_ld32(sp, r0); tmem_ld32(sp + 32, r1);
-                    if (!nodes) { tmem_ld32(sp + 64, r2); tmem_ld32(sp + 96, r3); }
+                // Two passes over the scores, 32 columns at a time in rolled loops: the code of a tile has to stay small (unrolled over the 128
+                // columns it drove the producers' and the issuer's code out of the instruction cache, and every step of theirs took
+                // hundreds of cycles).  Masked scores are replaced by -inf.
+                auto scores = [&](int g, float (&v)[32]) {
+                    uint32_t r[32];
+                    tmem_ld32(sp + 32 * g, r);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        sv[i] = __uint_as_float(r0[i]); sv[32 + i] = __uint_as_float(r1[i]);
-                        sv[64 + i] = nodes ? -INFINITY : __uint_as_float(r2[i]); sv[96 + i] = nodes ? -INFINITY : __uint_as_float(r3[i]);
+                    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+                    if (nodes || limit < 32 * g + 32) {
+                        const uint32_t see = nodes ? (uint32_t)(line >> (32 * g)) : (1u << (limit - 32 * g)) - 1u;
+#pragma unroll
+                        for (int i = 0; i < 32; i++) v[i] = (see >> i & 1) ? v[i] : -INFINITY;
                     }
-                }
-                if (nodes) {
-#pragma unroll
-                    for (int i = 0; i < 64; i++) sv[i] = (line >> i & 1) ? sv[i] : -INFINITY;
-                } else if (limit < TA_TK) {
-#pragma unroll
-                    for (int i = 0; i < 128; i++) sv[i] = i < limit ? sv[i] : -INFINITY;
-                }
+                };
                 float mt = -INFINITY;
+#pragma unroll 1
+                for (int g = 0; g < chunks; g++) {
+                    float v[32];
+                    scores(g, v);
 #pragma unroll
-                for (int i = 0; i < 128; i += 4) mt = fmaxf(mt, fmaxf(fmaxf(sv[i], sv[i + 1]), fmaxf(sv[i + 2], sv[i + 3])));
+                    for (int i = 0; i < 32; i += 4) mt = fmaxf(mt, fmaxf(fmaxf(v[i], v[i + 1]), fmaxf(v[i + 2], v[i + 3])));
+                }
+                if (warp == 0) GDN_TSTAMP(n * 16 + 5);
                 mt *= sc;                                            // (sc > 0: the maximum of the scaled scores)
                 // raise the reference only when it is far behind (or not set yet); O is rescaled then -- all lanes take part in the
                 // tensor-memory round trip, each with its own factor
@@ -460,15 +475,16 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                 // p = 2^(s sc - m) (a masked score gives 0) as bf16 hi + lo, written over the scores group by group: the 32 score
                 // columns of keys 32 g .. 32 g + 31 become 16 columns of hi pairs and 16 columns of lo pairs
                 const float nm = (m_run == -INFINITY) ? 0.f : -m_run;
-#pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    if (g >= chunks) continue;
+#pragma unroll 1
+                for (int g = 0; g < chunks; g++) {
+                    float v[32];
+                    scores(g, v);
                     uint32_t ph[16], pl[16];
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
                         float p0, p1;
-                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(fmaf(sv[32 * g + i], sc, nm)));
-                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(fmaf(sv[32 * g + i + 1], sc, nm)));
+                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p0) : "f"(fmaf(v[i], sc, nm)));
+                        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p1) : "f"(fmaf(v[i + 1], sc, nm)));
                         l_run += p0 + p1;
                         ph[i >> 1] = pack_bf16x2(p0, p1);
                         pl[i >> 1] = pack_bf16x2(p0 - __uint_as_float(ph[i >> 1] << 16), p1 - __uint_as_float(ph[i >> 1] & 0xffff0000u));
@@ -477,6 +493,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                     tmem_st16(sp + 32 * g + 16, pl);
                 }
                 tmem_wait_st();
+                if (warp == 0) GDN_TSTAMP(n * 16 + 6);
                 if (nodes || (limit & 15)) {
                     // value rows that nobody may see, and a node's non-finite values, are zeroed before the product reads them.  These warps
                     // do not wait for every phase of the V ring, and a parity cannot tell a phase from the one two before: once the
@@ -520,6 +537,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(AB_PREADY + (n & 1)));
+                if (warp == 0) GDN_TSTAMP(n * 16 + 7);
             }
             if (!ok) break;
             // ---- epilogue: O / l, or a partial (m, l, O) where the pair goes on in another block ----
@@ -687,7 +705,7 @@ size_t tree_attn_workspace_bytes(int B, int N, int H, int KV) {
 typedef CUresult (*TreeEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-static bool tree_map(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims, const cuuint32_t* box) {
+static bool tree_map(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
     static TreeEncodeFn fn = nullptr;
     if (!fn) {
         cudaDriverEntryPointQueryResult qr;
@@ -698,12 +716,9 @@ static bool tree_map(CUtensorMap* m, const void* base, int rank, const cuuint64_
         }
         fn = reinterpret_cast<TreeEncodeFn>(f);
     }
-    cuuint64_t strides[3];
-    cuuint64_t s = 2;
-    for (int i = 0; i + 1 < rank; i++) { s *= dims[i]; strides[i] = s; }
-    const cuuint32_t es[4] = {1, 1, 1, 1};
+    const cuuint32_t es[5] = {1, 1, 1, 1, 1};
     return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 static int gcd_of(int x, int y) { while (y) { const int r = x % y; x = y; y = r; } return x; }
@@ -745,12 +760,15 @@ int launch_tree_attn(const TreeAttnArgs& all, void* workspace, size_t workspace_
         p.k_box = gcd_of(a.page_size, TA_TK);
         p.v_box = gcd_of(a.page_size, 32);
         CUtensorMap tq, tk, tv, tkn, tvn;
+        // q, k_new, v_new: (dim, head, row); pages: (64 dims, row, 64-dim block, KV head, page), so that one copy can bring whole rows
+        const cuuint64_t row = ATT_D * 2, P = a.page_size;
         const cuuint64_t dq[3] = {ATT_D, (cuuint64_t)a.H, (cuuint64_t)a.B * a.N}, dn[3] = {ATT_D, (cuuint64_t)a.KV, (cuuint64_t)a.B * a.N};
-        const cuuint64_t dp[4] = {ATT_D, (cuuint64_t)a.page_size, (cuuint64_t)a.KV, (cuuint64_t)a.n_pages};
+        const cuuint64_t sq[2] = {row, row * a.H}, sn[2] = {row, row * a.KV};
+        const cuuint64_t dp[5] = {64, P, 4, (cuuint64_t)a.KV, (cuuint64_t)a.n_pages}, sp[4] = {row, 128, row * P, row * P * a.KV};
         const cuuint32_t bq[3] = {64, (cuuint32_t)p.group, (cuuint32_t)p.nodes}, bkn[3] = {64, 1, 64}, bvn[3] = {64, 1, 32};
-        const cuuint32_t bk[4] = {64, (cuuint32_t)p.k_box, 1, 1}, bv[4] = {64, (cuuint32_t)p.v_box, 1, 1};
-        if (!tree_map(&tq, a.q, 3, dq, bq) || !tree_map(&tk, a.k_pages, 4, dp, bk) || !tree_map(&tv, a.v_pages, 4, dp, bv) || !tree_map(&tkn, a.k_new, 3, dn, bkn) ||
-            !tree_map(&tvn, a.v_new, 3, dn, bvn)) {
+        const cuuint32_t bk[5] = {64, (cuuint32_t)p.k_box, 1, 1, 1}, bv[5] = {64, (cuuint32_t)p.v_box, p.v_box == 32 ? 4u : 1u, 1, 1};
+        if (!tree_map(&tq, a.q, 3, dq, sq, bq) || !tree_map(&tk, a.k_pages, 5, dp, sp, bk) || !tree_map(&tv, a.v_pages, 5, dp, sp, bv) ||
+            !tree_map(&tkn, a.k_new, 3, dn, sn, bkn) || !tree_map(&tvn, a.v_new, 3, dn, sn, bvn)) {
             set_error("gqa_tree_attn: tensor maps could not be made");
             return GDN_E_UNSUPPORTED;
         }
@@ -765,3 +783,9 @@ int launch_tree_attn(const TreeAttnArgs& all, void* workspace, size_t workspace_
 }
 
 }  // namespace gdn
+
+#ifdef GDN_TIMING
+extern "C" __attribute__((visibility("default"))) int gdn_timing_log_tree(long long* out_host, int n) {
+    return cudaMemcpyFromSymbol(out_host, gdn::g_tlog, sizeof(long long) * n) == cudaSuccess ? 0 : -5;
+}
+#endif
