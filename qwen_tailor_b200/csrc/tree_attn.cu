@@ -87,17 +87,30 @@ __device__ __forceinline__ unsigned long long shfl64(unsigned long long v, int s
     return (unsigned long long)__shfl_sync(0xffffffffu, (uint32_t)v, src) | (unsigned long long)__shfl_sync(0xffffffffu, (uint32_t)(v >> 32), src) << 32;
 }
 
+// tcgen05.mma with the accumulate flag in a register
+__device__ __forceinline__ void mma_ss_r(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .b64 da, db;\n\t.reg .pred p;\n\tmov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}"
+                 ::"r"(d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void mma_ts_r(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .b64 db;\n\t.reg .pred p;\n\tmov.b64 db, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}"
+                 ::"r"(d), "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc) : "memory");
+}
+
 __device__ __forceinline__ bool bf16_not_finite(uint32_t bits) { return (bits & 0x7f80u) == 0x7f80u; }
 
-// tile range [lo, hi) of block g when G blocks share N tiles
-__device__ __forceinline__ long long range_lo(int g, int G, long long N) { return (long long)g * N / G; }
+// first tile of block g when G blocks share N tiles: the first N % G blocks take one more (32-bit: a division costs a tenth of a 64-bit one)
+__device__ __forceinline__ int range_lo(int g, int G, int N) { const int q = N / G; return g * q + min(g, N - q * G); }
 
 __global__ void __launch_bounds__(TA_THREADS, 1)
 tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmKn, const __grid_constant__ CUtensorMap tmVn) {
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ uint64_t bars[AB_COUNT];
-    __shared__ long long s_cum[TA_MAX_B + 1];                        // tiles of all pairs of the sequences before
+    __shared__ int s_cum[TA_MAX_B + 1];                              // tiles of all pairs of the sequences before
+    __shared__ int s_ctx[TA_MAX_B];                                  // contexts, -1 = skipped
     __shared__ unsigned long long s_badv[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int s_abort;
@@ -108,6 +121,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");               // nothing an earlier kernel wrote is read before this
 
+    GDN_BSTAMP(0);
     // ---- plan ----
     const long long cap = (long long)a.max_pages * a.page_size;
     const int PP = a.KV * p.row_tiles;
@@ -123,18 +137,19 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
         return ctx;
     };
     if (warp == 0) {
-        long long run = 0;
+        int run = 0;
         for (int b0 = 0; b0 < a.B; b0 += 32) {
             const int b = b0 + lane;
-            int ctx = 0;
+            int x = 0;
             if (b < a.B) {
-                ctx = context(b);
-                if (ctx < 0) { if (blockIdx.x == 0) atomicExch(a.status, 1); ctx = 0; }
+                const int ctx = context(b);
+                if (ctx < 0 && blockIdx.x == 0) atomicExch(a.status, 1);
+                s_ctx[b] = ctx;
+                x = ((max(ctx, 0) + TA_TK - 1) / TA_TK + 1) * PP;
             }
-            long long x = b < a.B ? (long long)((ctx + TA_TK - 1) / TA_TK + 1) * PP : 0;
-            const long long own = x;
+            const int own = x;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) { const long long y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
+            for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(0xffffffffu, x, o); if (lane >= o) x += y; }
             if (b < a.B) s_cum[b] = run + x - own;
             run += __shfl_sync(0xffffffffu, x, 31);
         }
@@ -154,9 +169,10 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tb = tmem_slot;
-    const long long N_all = s_cum[a.B];
-    const int G = (int)min((long long)gridDim.x, N_all);
-    const long long lo = (int)blockIdx.x < G ? range_lo(blockIdx.x, G, N_all) : 0, hi = (int)blockIdx.x < G ? range_lo(blockIdx.x + 1, G, N_all) : 0;
+    GDN_BSTAMP(1);
+    const int N_all = s_cum[a.B];
+    const int G = min((int)gridDim.x, N_all);
+    const int lo = (int)blockIdx.x < G ? range_lo(blockIdx.x, G, N_all) : 0, hi = (int)blockIdx.x < G ? range_lo(blockIdx.x + 1, G, N_all) : 0;
 
     auto aborted = [&]() -> bool { return *(volatile int*)&s_abort != 0; };
     auto wait = [&](int b, uint32_t parity) -> bool {                // bounded; a failure tells the whole block to stop computing
@@ -177,19 +193,18 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
         return __shfl_sync(0xffffffffu, got, 0) != 0;
     };
     // the part of the block's range that starts at tile x: it ends with the pair or with the range
-    auto segment = [&](long long x) -> TreeSeg {
+    auto segment = [&](int x) -> TreeSeg {
         int l = 0, r = a.B - 1;
         while (l < r) { const int m = (l + r + 1) >> 1; if (s_cum[m] <= x) l = m; else r = m - 1; }
         TreeSeg s;
         s.b = l;
-        s.tiles = (int)((s_cum[l + 1] - s_cum[l]) / PP);
-        const long long off = x - s_cum[l];
-        const int pr = (int)(off / s.tiles);
-        s.t0 = (int)(off % s.tiles);
-        s.kvh = pr / p.row_tiles; s.rt = pr % p.row_tiles;
-        s.n = (int)min((long long)(s.tiles - s.t0), hi - x);
+        s.ctx = s_ctx[l];
+        s.tiles = (max(s.ctx, 0) + TA_TK - 1) / TA_TK + 1;
+        const int off = x - s_cum[l], pr = off / s.tiles;
+        s.t0 = off - pr * s.tiles;
+        s.kvh = pr / p.row_tiles; s.rt = pr - s.kvh * p.row_tiles;
+        s.n = min(s.tiles - s.t0, hi - x);
         s.more = x + s.n < hi;
-        s.ctx = context(l);
         return s;
     };
     const uint32_t sQ = sbase, sK = sbase + TA_Q_BYTES, sV = sK + TA_NK * TA_SLOT;
@@ -211,7 +226,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
         else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(stream_policy));
         uint32_t nr = 0, slot = 0, round = 0, nseg = 0;              // copies into the ring: their number, next slot, times around
         bool okp = true;
-        for (long long x = lo; x < hi && okp; nseg++) {
+        for (int x = lo; x < hi && okp; nseg++) {
             const TreeSeg s = segment(x);
             x += s.n;
             if (isk) {
@@ -224,14 +239,14 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                 }
             }
             const int* table = a.block_table + (size_t)s.b * a.max_pages;
-            const int entries = (int)(((long long)max(s.ctx, 0) + a.page_size - 1) / a.page_size);      // those that hold context
+            const int entries = s.ctx > 0 ? (s.ctx - 1) / a.page_size + 1 : 0;      // those that hold context
             auto entry = [&](int e) -> int { return e < entries ? table[e] : 0; };
             auto checked = [&](int pg) -> int {                      // a bad page number is reported, and page 0 read in its place
                 if (pg >= 0 && pg < a.n_pages) return pg;
                 atomicExch(a.status, 1);
                 return 0;
             };
-            int w = (int)((long long)s.t0 * TA_TK / a.page_size);    // first entry of the current window
+            int w = s.t0 * TA_TK / a.page_size;                      // first entry of the current window
             int cur = entry(w + lane), nxt = entry(w + 32 + lane);
             for (int t = s.t0; t < s.t0 + s.n && okp; t++) {
                 const int limit = limit_of(s, t);
@@ -298,7 +313,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
             constexpr uint32_t I_QK = idesc_bf16(128, 128, 0, 0), I_QN = idesc_bf16(128, 64, 0, 0);
             constexpr uint32_t I_PV = idesc_bf16(128, 256, 0, 1);    // B = V read N-major (dims contiguous)
             constexpr uint32_t HI = smem_desc_hi_sw128(1024);
-            uint32_t nk = 0, nv = 0, n = 0, nseg = 0;                // slabs, chunks, tiles and segments so far
+            uint32_t k_slot = 0, k_round = 0, v_slot = 0, v_round = 0, n = 0, nseg = 0;      // ring positions; tiles and segments so far
             bool ok = true;
             // the P V product of tile m with `limit` keys; first / last: of its segment (the ps-th)
             auto issue_pv = [&](uint32_t m, int limit, bool first, bool last, uint32_t ps) -> bool {
@@ -306,21 +321,20 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                 if (!wait(AB_PREADY + (m & 1), m >> 1)) return false;
                 if (first && ps > 0 && !wait(AB_OFREE, ps - 1)) return false;      // the epilogue before has read O
                 GDN_TSTAMP(m * 16 + 2);
-                bool fresh = first;
-                for (int c = 0; 32 * c < limit; c++, nv++) {
-                    const int slot = nv % TA_NV;
-                    if (!wait(AB_VFULL + slot, nv / TA_NV)) return false;
+                uint32_t acc = first ? 0 : 1;                        // the first product of a segment overwrites O
+                for (int c = 0; 32 * c < limit; c++) {
+                    if (!wait(AB_VFULL + v_slot, v_round)) return false;
                     tc_fence_after_sync();
-                    const uint32_t vlo = smem_desc_lo(sV + slot * TA_SLOT, 4096);
-                    const int steps = limit - 32 * c > 16 ? 2 : 1;
-                    for (int part = 0; part < 2; part++)             // hi, lo
-                        for (int ks = 0; ks < steps; ks++) {
-                            const uint32_t acol = sp + 32 * c + 16 * part + 8 * ks;
-                            if (fresh) mma_ts_w<false>(tb + TAM_O, acol, vlo + ks * 128, HI, I_PV);
-                            else mma_ts_w<true>(tb + TAM_O, acol, vlo + ks * 128, HI, I_PV);
-                            fresh = false;
-                        }
-                    mma_commit(bar(AB_VEMPTY + slot));
+                    const uint32_t vlo = smem_desc_lo(sV + v_slot * TA_SLOT, 4096), acol = sp + 32 * c;
+                    mma_ts_r(tb + TAM_O, acol, vlo, HI, I_PV, acc);  // hi and lo of keys 32 c .. 32 c + 15, then of the other 16
+                    mma_ts_w<true>(tb + TAM_O, acol + 16, vlo, HI, I_PV);
+                    if (limit - 32 * c > 16) {
+                        mma_ts_w<true>(tb + TAM_O, acol + 8, vlo + 128, HI, I_PV);
+                        mma_ts_w<true>(tb + TAM_O, acol + 24, vlo + 128, HI, I_PV);
+                    }
+                    acc = 1;
+                    mma_commit(bar(AB_VEMPTY + v_slot));
+                    if (++v_slot == TA_NV) { v_slot = 0; v_round++; }
                 }
                 mma_commit(bar(AB_PFREE + (m & 1)));
                 if (last) mma_commit(bar(AB_ODONE));
@@ -330,7 +344,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
             int p_limit = 0;
             bool p_have = false, p_first = false, p_last = false;
             uint32_t p_seg = 0;
-            for (long long x = lo; x < hi && ok; nseg++) {
+            for (int x = lo; x < hi && ok; nseg++) {
                 const TreeSeg s = segment(x);
                 x += s.n;
                 const int qb = nseg % p.q_bufs;
@@ -341,17 +355,15 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                     const uint32_t sp = tb + TAM_SP0 + (n & 1) * 128;
                     const uint32_t idesc = t == s.tiles - 1 ? I_QN : I_QK;
                     GDN_TSTAMP(n * 16 + 0);
-                    for (int j = 0; j < 4 && ok; j++, nk++) {
-                        const int slot = nk % TA_NK;
-                        if (!wait(AB_KFULL + slot, nk / TA_NK)) { ok = false; break; }
+                    for (int j = 0; j < 4; j++) {
+                        if (!wait(AB_KFULL + k_slot, k_round)) { ok = false; break; }
                         tc_fence_after_sync();
-                        const uint32_t klo = smem_desc_lo(sK + slot * TA_SLOT, 16);
+                        const uint32_t klo = smem_desc_lo(sK + k_slot * TA_SLOT, 16), ql = qlo + j * (p.q_slab >> 4);
+                        mma_ss_r(sp, ql, HI, klo, HI, idesc, j);     // (the first product of a tile overwrites S)
 #pragma unroll
-                        for (int kk = 0; kk < 4; kk++) {
-                            if (j == 0 && kk == 0) mma_ss_w<false>(sp, qlo + kk * 2, HI, klo + kk * 2, HI, idesc);
-                            else mma_ss_w<true>(sp, qlo + j * (p.q_slab >> 4) + kk * 2, HI, klo + kk * 2, HI, idesc);
-                        }
-                        mma_commit(bar(AB_KEMPTY + slot));
+                        for (int kk = 1; kk < 4; kk++) mma_ss_w<true>(sp, ql + kk * 2, HI, klo + kk * 2, HI, idesc);
+                        mma_commit(bar(AB_KEMPTY + k_slot));
+                        if (++k_slot == TA_NK) { k_slot = 0; k_round++; }
                     }
                     if (!ok) break;
                     mma_commit(bar(AB_SDONE + (n & 1)));
@@ -366,7 +378,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
         }
     } else if (warp == 7) {
         // ================= append: the nodes' rows into the cache, by the block that has a pair's first tile =================
-        for (long long x = lo; x < hi;) {
+        for (int x = lo; x < hi;) {
             const TreeSeg s = segment(x);
             x += s.n;
             if (s.t0 != 0 || s.rt != 0 || s.ctx < 0) continue;
@@ -394,7 +406,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
         const uint32_t tl = tb + ((uint32_t)(warp * 32) << 16);      // this warp's TMEM lanes
         uint32_t n = 0, nv = 0, nseg = 0, node_tiles = 0;
         bool ok = true;
-        for (long long x = lo; x < hi; nseg++) {
+        for (int x = lo; x < hi; nseg++) {
             const TreeSeg s = segment(x);
             x += s.n;
             const int node = s.rt * p.nodes + local;
@@ -540,9 +552,11 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                 if (warp == 0) GDN_TSTAMP(n * 16 + 7);
             }
             if (!ok) break;
+            GDN_BSTAMP(nseg == 0 ? 3 : 6);
             // ---- epilogue: O / l, or a partial (m, l, O) where the pair goes on in another block ----
             if (!warp_wait(AB_ODONE, nseg)) break;
             tc_fence_after_sync();
+            GDN_BSTAMP(nseg == 0 ? 4 : 7);
             const bool whole = s.n == s.tiles;
             const int slot = 2 * (int)blockIdx.x + (s.t0 == 0 ? 1 : 0);
             float* part = p.part + (size_t)slot * (64 * 4) * p.rows;
@@ -587,9 +601,10 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(AB_OFREE));
+            GDN_BSTAMP(nseg == 0 ? 5 : 8);
             if (tid == 0 && !s.more) {
                 // the pair that starts in this block and goes on in the next ones is joined by the merge kernel
-                const long long first = hi - s.n - s.t0;
+                const int first = hi - s.n - s.t0;
                 int parts = 0;
                 if (s.t0 == 0 && !whole) {
                     parts = 1;
@@ -604,72 +619,70 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
     tc_fence_before_sync();
     __syncthreads();
     if (warp == 4) tmem_dealloc(tb, 512);
+    GDN_BSTAMP(9);
 }
 
-// Joins the partials of the pair that starts in main block blockIdx.x and is cut: 32 rows per block (rows side by side in memory), eight
-// warps taking 32 columns each.
-constexpr int TM_THREADS = 256;
+// Joins the partials of the pair that starts in main block blockIdx.x and is cut: eight rows per block, a thread holds four columns of a row.
+// Bound: latency (a few hundred KiB out of L2), so all a block's (m, l) pairs are fetched at once and every thread has four partials in flight.
+constexpr int TM_THREADS = 512, TM_ROWS = 8;
 
 __global__ void __launch_bounds__(TM_THREADS) tree_attn_merge_kernel(const __grid_constant__ TreeAttnPlan p) {
-    __shared__ float s_w[149][32];
-    __shared__ __align__(16) __nv_bfloat16 s_out[32][ATT_D + 8];
-    __shared__ unsigned char s_live[32];
+    __shared__ float s_w[148][TM_ROWS], s_l[148][TM_ROWS];
+    __shared__ unsigned char s_live[TM_ROWS];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int g = blockIdx.x, parts = p.info[2 * g + 1];
+    GDN_BSTAMP(10);
     if (parts == 0) return;
     const TreeAttnArgs& a = p.a;
     const int pair = p.info[2 * g], rt = pair % p.row_tiles, kvh = pair / p.row_tiles % a.KV, b = pair / p.row_tiles / a.KV;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.y * 32 + lane;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = tid & (TM_ROWS - 1), row = blockIdx.y * TM_ROWS + r, cg = tid / TM_ROWS;
     const bool in = row < p.rows;
-    const int node = rt * p.nodes + row / p.group;
-    auto slot = [&](int k) -> int { return k == 0 ? 2 * g + 1 : 2 * (g + k); };
-    if (warp == 0) {
-        // the rows' common maximum, the partials' weights over the row's sum
-        float mx = -INFINITY, sum = 0.f;
-        for (int k = 0; k < parts; k++) if (in) mx = fmaxf(mx, p.part_ml[((size_t)slot(k) * p.rows + row) * 2]);
-        for (int k = 0; k < parts; k++) {
-            const float2 ml = in ? *reinterpret_cast<const float2*>(p.part_ml + ((size_t)slot(k) * p.rows + row) * 2) : make_float2(-INFINITY, 0.f);
-            const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mx);
-            sum = fmaf(w, ml.y, sum);
-            s_w[k][lane] = w;
-        }
-        const float inv = sum == 0.f ? 1.f : 1.f / sum;
-        for (int k = 0; k < parts; k++) s_w[k][lane] *= inv;
-    } else if (warp == 1) {
+    auto slot = [&](int k) -> size_t { return k == 0 ? 2 * g + 1 : 2 * (g + k); };
+    for (int k = cg; k < parts; k += TM_THREADS / TM_ROWS) {
+        const float2 ml = in ? *reinterpret_cast<const float2*>(p.part_ml + (slot(k) * p.rows + row) * 2) : make_float2(-INFINITY, 0.f);
+        s_w[k][r] = ml.x;
+        s_l[k][r] = ml.y;
+    }
+    if (warp == TM_ROWS) {                                           // which of the rows belong to nodes in use
         unsigned long long l0, l1;
         bool bad;
         const int* par = a.parents + (size_t)b * a.N;
         warp_lines(lane < a.N ? par[lane] : -2, lane + 32 < a.N ? par[lane + 32] : -2, l0, l1, bad);
+        const int node = rt * p.nodes + (blockIdx.y * TM_ROWS + (lane & (TM_ROWS - 1))) / p.group;
         const unsigned long long x0 = shfl64(l0, node & 31), x1 = shfl64(l1, node & 31);
-        s_live[lane] = in && node < a.N && (node < 32 ? x0 : x1) != 0;
+        if (lane < TM_ROWS) s_live[lane] = node < a.N && (node < 32 ? x0 : x1) != 0;
     }
     __syncthreads();
-    float4 acc[8];
+    if (warp < TM_ROWS) {                                            // the row's common maximum; weights over the row's sum
+        float mx = -INFINITY, sum = 0.f;
+        for (int k = lane; k < parts; k += 32) mx = fmaxf(mx, s_w[k][warp]);
 #pragma unroll
-    for (int i = 0; i < 8; i++) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (in) {
-#pragma unroll 2
-        for (int k = 0; k < parts; k++) {
-            const float w = s_w[k][lane];
-            const float4* src = reinterpret_cast<const float4*>(p.part) + ((size_t)slot(k) * 64 + warp * 8) * p.rows + row;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float4 o = __ldcg(src + (size_t)i * p.rows);
-                acc[i].x = fmaf(w, o.x, acc[i].x); acc[i].y = fmaf(w, o.y, acc[i].y); acc[i].z = fmaf(w, o.z, acc[i].z); acc[i].w = fmaf(w, o.w, acc[i].w);
-            }
+        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        for (int k = lane; k < parts; k += 32) {
+            const float m = s_w[k][warp], w = m == -INFINITY ? 0.f : exp2f(m - mx);
+            sum = fmaf(w, s_l[k][warp], sum);
+            s_w[k][warp] = w;
         }
+        sum = warp_sum(sum);
+        const float inv = sum == 0.f ? 1.f : 1.f / sum;
+        for (int k = lane; k < parts; k += 32) s_w[k][warp] *= inv;
     }
-    const bool live = s_live[lane];
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-        *reinterpret_cast<uint2*>(&s_out[lane][warp * 32 + 4 * i]) = live ? make_uint2(pack_bf16x2(acc[i].x, acc[i].y), pack_bf16x2(acc[i].z, acc[i].w)) : make_uint2(0, 0);
     __syncthreads();
-    for (int i = threadIdx.x; i < 32 * 32; i += TM_THREADS) {
-        const int r = i >> 5, gr = blockIdx.y * 32 + r, nd = rt * p.nodes + gr / p.group;
-        if (gr < p.rows && nd < a.N)
-            reinterpret_cast<uint4*>(a.out + (((size_t)b * a.N + nd) * a.H + kvh * p.group + gr % p.group) * ATT_D)[i & 31] = *reinterpret_cast<const uint4*>(&s_out[r][(i & 31) * 8]);
+    const int node = rt * p.nodes + row / p.group;
+    if (!in || node >= a.N) return;
+    const float4* part = reinterpret_cast<const float4*>(p.part) + (size_t)cg * p.rows + row;
+    const size_t step = (size_t)64 * p.rows;                         // float4s of a slot
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = 0; k < parts; k++) {
+        const float w = s_w[k][r];
+        const float4 o = __ldcg(part + slot(k) * step);
+        acc.x = fmaf(w, o.x, acc.x); acc.y = fmaf(w, o.y, acc.y); acc.z = fmaf(w, o.z, acc.z); acc.w = fmaf(w, o.w, acc.w);
     }
+    const uint2 v = s_live[r] ? make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w)) : make_uint2(0, 0);
+    *reinterpret_cast<uint2*>(a.out + (((size_t)b * a.N + node) * a.H + kvh * p.group + row % p.group) * ATT_D + 4 * cg) = v;
+    GDN_BSTAMP(11);
 }
 
 // ---- host side ----
@@ -680,7 +693,7 @@ static int tree_sms() {
     if (!sms[dev]) {
         int n = 0;
         if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) { cudaGetLastError(); n = 148; }
-        sms[dev] = n < 148 ? n : 148;                                // (the merge kernel keeps the weights of at most 149 partials)
+        sms[dev] = n < 148 ? n : 148;                                // (the merge kernel keeps the weights of at most 148 partials)
     }
     return sms[dev];
 }
@@ -776,7 +789,7 @@ int launch_tree_attn(const TreeAttnArgs& all, void* workspace, size_t workspace_
         int rc = launch_pdl((const void*)tree_attn_kernel, dim3(p.G), TA_THREADS, TA_SMEM, st, args);
         if (rc) return rc;
         void* margs[] = {&p};
-        rc = launch_pdl((const void*)tree_attn_merge_kernel, dim3(p.G, (p.rows + 31) / 32), TM_THREADS, 0, st, margs);
+        rc = launch_pdl((const void*)tree_attn_merge_kernel, dim3(p.G, (p.rows + TM_ROWS - 1) / TM_ROWS), TM_THREADS, 0, st, margs);
         if (rc) return rc;
     }
     return GDN_OK;
