@@ -104,6 +104,19 @@ __device__ __forceinline__ bool bf16_not_finite(uint32_t bits) { return (bits & 
 // first tile of block g when G blocks share N tiles: the first N % G blocks take one more (32-bit: a division costs a tenth of a 64-bit one)
 __device__ __forceinline__ int range_lo(int g, int G, int N) { const int q = N / G; return g * q + min(g, N - q * G); }
 
+// The rest of a bounded wait whose first poll failed; out of line, because a wait is needed in two dozen places and the code of the
+// roles' loops has to stay small (they run side by side out of one instruction cache).
+__device__ __noinline__ bool tree_wait_slow(uint32_t addr, uint32_t parity, volatile int* abort, int* status) {
+    for (uint32_t i = 0; i < 2000000u; i++) {
+        if (mbar_test_wait(addr, parity)) return true;
+        if ((i & 63u) == 63u && *abort) return false;
+        __nanosleep(20);
+    }
+    *abort = 1;
+    atomicExch(status, 2);
+    return false;
+}
+
 __global__ void __launch_bounds__(TA_THREADS, 1)
 tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmKn, const __grid_constant__ CUtensorMap tmVn) {
@@ -111,6 +124,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
     __shared__ uint64_t bars[AB_COUNT];
     __shared__ int s_cum[TA_MAX_B + 1];                              // tiles of all pairs of the sequences before
     __shared__ int s_ctx[TA_MAX_B];                                  // contexts, -1 = skipped
+    __shared__ int2 s_box[2][32];                                    // (page, row) of the boxes of a producer's tile
     __shared__ unsigned long long s_badv[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int s_abort;
@@ -175,21 +189,15 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
     const int lo = (int)blockIdx.x < G ? range_lo(blockIdx.x, G, N_all) : 0, hi = (int)blockIdx.x < G ? range_lo(blockIdx.x + 1, G, N_all) : 0;
 
     auto aborted = [&]() -> bool { return *(volatile int*)&s_abort != 0; };
-    auto wait = [&](int b, uint32_t parity) -> bool {                // bounded; a failure tells the whole block to stop computing
-        const uint32_t addr = bar(b);
-        for (uint32_t i = 0; i < 2000000u; i++) {
-            if (mbar_test_wait(addr, parity & 1u)) return true;
-            if ((i & 63u) == 63u && aborted()) return false;
-            __nanosleep(20);
-        }
-        atomicExch(&s_abort, 1);
-        atomicExch(a.status, 2);
-        return false;
+    // bounded; a failure tells the whole block to stop computing
+    auto wait = [&](int b, uint32_t parity) -> bool {
+        return mbar_test_wait(bar(b), parity & 1u) || tree_wait_slow(bar(b), parity & 1u, &s_abort, a.status);
     };
     // the same for a whole warp: every lane gets the same answer, whatever a lane saw of an abort
     auto warp_wait = [&](int b, uint32_t parity) -> bool {
+        if (__all_sync(0xffffffffu, mbar_test_wait(bar(b), parity & 1u))) return true;
         int got = 0;
-        if (lane == 0) got = wait(b, parity);
+        if (lane == 0) got = tree_wait_slow(bar(b), parity & 1u, &s_abort, a.status);
         return __shfl_sync(0xffffffffu, got, 0) != 0;
     };
     // the part of the block's range that starts at tile x: it ends with the pair or with the range
@@ -213,18 +221,18 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
 
     if (warp == 5 || warp == 6) {
         // ================= producers: warp 5 Q and K, warp 6 V =================
-        // Lane i works out page and row of box i of a tile (a tile has at most 32 boxes where the page size is a multiple of 4): done box
-        // by box the address arithmetic costs a warp more than the copies do (measured: 13 k cycles a tile against the 5.7 k that
-        // the memory needs).  Page numbers come in windows of 32 table entries, one per lane, the next window requested a window
-        // ahead: a plain load takes microseconds under the copies, and one per tile held the ring up (7.3 k cycles a tile).
+        // Lane i works out page and row of box i of a tile (a tile has at most 32 boxes where the page size is a multiple of 4); page
+        // numbers come in windows of 32 table entries, one per lane, the next window requested a window ahead, because a plain load
+        // takes microseconds under the copies.  Then lane j is the producer of the tile's j-th ring slot: it polls that slot and
+        // issues that slot's copies.  (One lane doing all of it, slot after slot, took 7 .. 13 k cycles a tile; the memory needs 5.7 k.)
         const bool isk = warp == 5;
-        const int box = isk ? p.k_box : p.v_box, per_tile = TA_TK / box;
+        const int box = isk ? p.k_box : p.v_box, per_tile = TA_TK / box, per_chunk = 32 / min(box, 32);
         const int first_empty = isk ? AB_KEMPTY : AB_VEMPTY, first_full = isk ? AB_KFULL : AB_VFULL, ring = isk ? TA_NK : TA_NV;
         const uint32_t base = isk ? sK : sV;
         uint64_t stream_policy;                                      // the cache is read once per row tile: first to leave L2 unless a second row tile follows
         if (p.row_tiles == 1) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(stream_policy));
         else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(stream_policy));
-        uint32_t nr = 0, slot = 0, round = 0, nseg = 0;              // copies into the ring: their number, next slot, times around
+        uint32_t nr = 0, nseg = 0;                                   // slots filled so far
         bool okp = true;
         for (int x = lo; x < hi && okp; nseg++) {
             const TreeSeg s = segment(x);
@@ -251,55 +259,55 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
             for (int t = s.t0; t < s.t0 + s.n && okp; t++) {
                 const int limit = limit_of(s, t);
                 const bool nodes = t == s.tiles - 1;
-                int page = 0, row = 0;                               // of this lane's box
                 if (!nodes && per_tile <= 32) {
                     const int first = t * TA_TK / a.page_size;
                     while (first >= w + 32) { w += 32; cur = nxt; nxt = entry(w + 32 + lane); }
                     const int key = min(t * TA_TK + lane * box, s.ctx - 1), e = key / a.page_size - w;      // (boxes behind the context are not copied)
-                    row = key - (w + e) * a.page_size;
                     const int p0 = __shfl_sync(0xffffffffu, cur, e & 31), p1 = __shfl_sync(0xffffffffu, nxt, e & 31);
-                    page = checked(e < 32 ? p0 : p1);
+                    s_box[warp - 5][lane] = make_int2(checked(e < 32 ? p0 : p1), key - (w + e) * a.page_size);
+                    __syncwarp();
                 }
                 // K: four slabs of 64 dims, all boxes each; V: chunks of 32 keys, its boxes whole rows
-                const int steps = isk ? 4 : (limit + 31) / 32;
-                for (int j = 0; j < steps; j++) {
-                    if (round > 0 && !warp_wait(first_empty + slot, round - 1)) { okp = false; break; }
-                    const uint32_t full = bar(first_full + slot), dst = base + slot * TA_SLOT;
-                    const int i0 = isk ? 0 : j * (32 / box);         // the step's boxes [i0, i0 + cnt)
-                    const int cnt = nodes ? 0 : ((isk ? limit : min(32, limit - 32 * j)) + box - 1) / box;
-                    if (lane == 0) {
-                        mbar_expect_tx(full, nodes ? (isk ? 64 * 128 : TA_SLOT) : cnt * box * (isk ? 128 : 512));
-                        if (nodes && isk) tma_load_3d(dst, &tmKn, full, 64 * j, s.kvh, s.b * a.N);
-                        if (nodes && !isk)
-                            for (int k = 0; k < 4; k++) tma_load_3d(dst + k * 4096, &tmVn, full, 64 * k, s.kvh, s.b * a.N + 32 * j);
-                    }
-                    for (int i = 0; i < cnt; i++) {
-                        int pg, rw;
-                        if (per_tile <= 32) {
-                            pg = __shfl_sync(0xffffffffu, page, i0 + i);
-                            rw = __shfl_sync(0xffffffffu, row, i0 + i);
-                        } else {                                     // (page sizes that are not a multiple of 4: looked up in place)
-                            const int key = t * TA_TK + (i0 + i) * box, e = key / a.page_size;
-                            rw = key - e * a.page_size;
-                            pg = checked(table[e]);
-                        }
-                        if (lane == 0) {
-                            const uint32_t to = dst + i * box * 128;
-                            if (isk)
-                                asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5, %6, %7}], [%2], %8;"
-                                             ::"r"(to), "l"(&tmK), "r"(full), "r"(0), "r"(rw), "r"(j), "r"(s.kvh), "r"(pg), "l"(stream_policy) : "memory");
-                            else if (box == 32)                      // the four 64-dim blocks of 32 rows are the chunk's image
-                                asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5, %6, %7}], [%2], %8;"
-                                             ::"r"(to), "l"(&tmV), "r"(full), "r"(0), "r"(rw), "r"(0), "r"(s.kvh), "r"(pg), "l"(stream_policy) : "memory");
-                            else
-                                for (int k = 0; k < 4; k++)
+                const int steps = isk ? 4 : (limit + 31) / 32, j = lane;
+                const uint32_t mine = nr + lane, slot = mine % ring, round = mine / ring;
+                const uint32_t full = bar(first_full + slot), empty = bar(first_empty + slot), dst = base + slot * TA_SLOT;
+                const int i0 = isk ? 0 : j * per_chunk;              // this lane's boxes [i0, i0 + cnt)
+                const int cnt = isk ? (limit + box - 1) / box : (min(32, limit - 32 * j) + box - 1) / box;
+                bool todo = lane < steps;
+                for (uint32_t polls = 0; __any_sync(0xffffffffu, todo); polls++) {
+                    if (todo && (round == 0 || mbar_test_wait(empty, (round - 1) & 1u))) {
+                        todo = false;
+                        if (nodes) {
+                            mbar_expect_tx(full, isk ? 64 * 128 : TA_SLOT);
+                            if (isk) tma_load_3d(dst, &tmKn, full, 64 * j, s.kvh, s.b * a.N);
+                            else for (int k = 0; k < 4; k++) tma_load_3d(dst + k * 4096, &tmVn, full, 64 * k, s.kvh, s.b * a.N + 32 * j);
+                        } else {
+                            mbar_expect_tx(full, cnt * box * (isk ? 128 : 512));
+                            for (int i = 0; i < cnt; i++) {
+                                int2 at;
+                                if (per_tile <= 32) at = s_box[warp - 5][i0 + i];
+                                else {                               // (page sizes that are not a multiple of 4: looked up in place)
+                                    const int key = t * TA_TK + (i0 + i) * box, e = key / a.page_size;
+                                    at = make_int2(checked(table[e]), key - e * a.page_size);
+                                }
+                                // V: the four 64-dim blocks of 32 rows are the chunk's image; of smaller boxes each block is a copy of its own
+                                const int copies = isk || box == 32 ? 1 : 4;
+                                for (int k = 0; k < copies; k++)
                                     asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5, %6, %7}], [%2], %8;"
-                                                 ::"r"(to + k * 4096), "l"(&tmV), "r"(full), "r"(0), "r"(rw), "r"(k), "r"(s.kvh), "r"(pg), "l"(stream_policy) : "memory");
+                                                 ::"r"(dst + i * box * 128 + k * 4096), "l"(isk ? &tmK : &tmV), "r"(full), "r"(0), "r"(at.y), "r"(isk ? j : k), "r"(s.kvh), "r"(at.x), "l"(stream_policy) : "memory");
+                            }
                         }
+                    } else if (todo) {
+                        __nanosleep(20);
                     }
-                    nr++;
-                    if (++slot == (uint32_t)ring) { slot = 0; round++; }
+                    if ((polls & 63u) == 63u && __any_sync(0xffffffffu, aborted() || polls > 2000000u)) { okp = false; break; }
                 }
+                if (!okp) {
+                    if (lane == 0 && !aborted()) { s_abort = 1; atomicExch(a.status, 2); }
+                    break;
+                }
+                nr += steps;
+                __syncwarp();                                        // (s_box is rewritten by the next tile)
                 GDN_TSTAMP((int)(x - s.n - lo + t - s.t0) * 16 + (isk ? 8 : 9));
             }
         }
