@@ -9,14 +9,14 @@ In-place writes are ordered against later readers by CUDA stream order.
 """
 from __future__ import annotations
 
-import ctypes
+from array import array
+from math import prod
 from typing import Sequence
 
-import numpy as np
 import torch
 
 from . import _lib
-from ._lib import check, on_device, ptr, require_same_device, stream_ptr
+from ._lib import check, on_device, ptr, raw_stream, require_same_device, stream_ptr
 from .config import Cfg
 from .gated_delta import _f32
 from .kernels import _rows
@@ -106,7 +106,7 @@ def attn_tree(q, k_new, v_new, k_pages, v_pages, block_table, ctx_len, parents, 
     ``compact_rows`` moves the accepted ones together afterwards).  Rows of unused nodes are not appended and their output is zero.
     One node per sequence (N = 1, parents = -1) is plain decode.  Returns o [B*N, H, 256] bf16 (``out``, if given).
     A malformed tree, context or page number is reported by ``_lib.device_status()``."""
-    require_same_device(q, k_new, v_new, k_pages, v_pages, block_table, ctx_len, parents, out)
+    dev = require_same_device(q, k_new, v_new, k_pages, v_pages, block_table, ctx_len, parents, out)
     for name, t in (("block_table", block_table), ("ctx_len", ctx_len), ("parents", parents)):
         if t.dtype != torch.int32 or not t.is_contiguous():
             raise ValueError(f"attn_tree: {name} must be contiguous int32")
@@ -129,10 +129,11 @@ def attn_tree(q, k_new, v_new, k_pages, v_pages, block_table, ctx_len, parents, 
     if B == 0:
         return out
     lib = _lib.load()
-    with on_device(q.device):
-        ws = torch.empty((lib.gqa_tree_attn_workspace_bytes(B, N, H, KV),), dtype=torch.uint8, device=q.device)
-        check(lib.gqa_tree_attn(ptr(q), ptr(k_new), ptr(v_new), ptr(k_pages), ptr(v_pages), ptr(block_table), ptr(ctx_len), ptr(parents), ptr(out),
-                                ptr(ws), ws.numel(), B, N, H, KV, page_size, block_table.shape[1], n_pages, stream_ptr(q.device)), "attn_tree")
+    with on_device(dev):
+        size = lib.gqa_tree_attn_workspace_bytes(B, N, H, KV)
+        ws = torch.empty((size,), dtype=torch.uint8, device=dev)
+        check(lib.gqa_tree_attn(q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), ctx_len.data_ptr(),
+                                parents.data_ptr(), out.data_ptr(), ws.data_ptr(), size, B, N, H, KV, page_size, block_table.shape[1], n_pages, raw_stream(dev)), "attn_tree")
     return out
 
 
@@ -171,27 +172,30 @@ def hrec(hist, Hn, slots, pos):
 def _pool_ptrs(who, pools, stacked):
     """The pools of ``pools`` (each a contiguous bf16 or fp32 tensor, all of one shape; stacked: each holds several along a leading
     layer dimension) as (first tensor, shape of one pool, device pointers)."""
-    pools = list(pools)
     if not pools:
         raise ValueError(f"{who}: no pools")
     first = pools[0]
     require_same_device(*pools)
-    ptrs = []
+    shape, dtype, ptrs = first.shape, first.dtype, array("Q")
+    if dtype not in (torch.bfloat16, torch.float32) or len(shape) < (3 if stacked else 2) or 0 in shape[1:]:
+        raise ValueError(f"{who}: pools must be non-empty bf16 or fp32 tensors, got {dtype} {tuple(shape)}")
+    step = prod(shape[1:]) * first.element_size()
     for t in pools:
-        if t.dtype not in (torch.bfloat16, torch.float32) or t.dtype != first.dtype or t.shape != first.shape or not t.is_contiguous():
-            raise ValueError(f"{who}: pools must be contiguous bf16 or fp32 tensors of one shape")
+        if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{who}: pools must be contiguous tensors of one shape and type")
+        p = t.data_ptr()
         if stacked:
-            step = t.stride(0) * t.element_size()
-            ptrs += [t.data_ptr() + i * step for i in range(t.shape[0])]
+            ptrs.extend(range(p, p + step * shape[0], step))
         else:
-            ptrs.append(t.data_ptr())
-    shape = first.shape[1:] if stacked else first.shape
-    if len(shape) < 2 or not all(shape):
-        raise ValueError(f"{who}: pools of shape {tuple(shape)}")
-    return first, tuple(shape), (ctypes.c_void_p * len(ptrs))(*ptrs), len(ptrs)
+            ptrs.append(p)
+    return first, shape[1:] if stacked else shape, ptrs
 
 
-def copy_entries(pools, dst: Sequence[int], src: Sequence[int], rows=None, stacked=False):
+def _address(a):
+    return a.buffer_info()[0]
+
+
+def copy_entries(pools: Sequence[torch.Tensor], dst: Sequence[int], src: Sequence[int], rows=None, stacked=False):
     """pool[dst[i]] = pool[src[i]] for every pool and i, in place, in one launch (no counterpart in the reference, which copies layer by
     layer with ``blit``): K/V pages, recurrent states or conv windows of all layers when a sequence is forked, checkpointed or moved.
 
@@ -199,34 +203,36 @@ def copy_entries(pools, dst: Sequence[int], src: Sequence[int], rows=None, stack
     dst, src: host integers.  One source may be copied to many entries; no dst may repeat or be a src (ValueError).
     rows (an int, or one per pair): only the first rows of every head of pages [n_entries, heads, page_size, dim] are copied.
     Every 160 pairs take one launch."""
-    first, shape, ptrs, n_pools = _pool_ptrs("copy_entries", pools, stacked)
-    d, s = np.ascontiguousarray(dst, dtype=np.int32), np.ascontiguousarray(src, dtype=np.int32)
-    if d.ndim != 1 or d.shape != s.shape:
-        raise ValueError(f"copy_entries: {d.shape} destinations for {s.shape} sources")
-    n = d.size
+    first, shape, ptrs = _pool_ptrs("copy_entries", pools, stacked)
+    d, s = array("i", dst), array("i", src)
+    n = len(d)
+    if n != len(s):
+        raise ValueError(f"copy_entries: {n} destinations for {len(s)} sources")
     if n == 0:
         return
-    if min(d.min(), s.min()) < 0 or max(d.max(), s.max()) >= shape[0]:
+    targets, sources = set(d), set(s)
+    if min(targets) < 0 or min(sources) < 0 or max(targets) >= shape[0] or max(sources) >= shape[0]:
         raise ValueError(f"copy_entries: an entry outside [0, {shape[0]})")
-    targets = set(d.tolist())
-    if len(targets) < n or not targets.isdisjoint(s.tolist()):
+    if len(targets) < n or not targets.isdisjoint(sources):
         raise ValueError("copy_entries: a destination is named twice, or is a source too")
-    item = first.element_size()
-    n_sub, sub_bytes, lens = 1, int(np.prod(shape[1:])) * item, None
+    item, lens = first.element_size(), None
+    n_sub, sub_bytes = 1, prod(shape[1:]) * item
     if rows is not None:
         if len(shape) != 4:
             raise ValueError(f"copy_entries: rows needs pools [n_entries, heads, page_size, dim], got entries of {tuple(shape[1:])}")
-        r = np.asarray(rows, dtype=np.int64)
-        if r.ndim > 1 or (r.ndim == 1 and r.size != n) or r.min() < 0 or r.max() > shape[2]:
+        r = array("q", [rows]) * n if isinstance(rows, int) else array("q", rows)
+        if len(r) != n or min(r) < 0 or max(r) > shape[2]:
             raise ValueError(f"copy_entries: rows must be one number or {n}, from 0 to {shape[2]}")
         n_sub, sub_bytes = shape[1], shape[2] * shape[3] * item
-        lens = np.ascontiguousarray(np.broadcast_to(r * (shape[3] * item), (n,)), dtype=np.int64)
-    with on_device(first.device):
-        check(_lib.load().gdn_entries_copy(ptrs, n_pools, shape[0], n_sub, sub_bytes, d.ctypes.data, s.ctypes.data, lens.ctypes.data if lens is not None else None, n,
-                                           stream_ptr(first.device)), "copy_entries")
+        row = shape[3] * item
+        lens = array("q", [rows * row]) * n if isinstance(rows, int) else array("q", [x * row for x in r])
+    dev = first.device
+    with on_device(dev):
+        check(_lib.load().gdn_entries_copy(_address(ptrs), len(ptrs), shape[0], n_sub, sub_bytes, _address(d), _address(s), _address(lens) if lens is not None else None, n,
+                                           raw_stream(dev)), "copy_entries")
 
 
-def compact_rows(pools, block_table, base, keep, n_keep, dst_table=None, stacked=False):
+def compact_rows(pools: Sequence[torch.Tensor], block_table, base, keep, n_keep, dst_table=None, stacked=False):
     """Row base[b] + keep[b, j] of sequence b moves to row base[b] + j for j < n_keep[b], in every pool and head, in one launch: the K/V
     rows of an accepted path move together behind the context (base = ctx_len, keep / n_keep from ``accept_tree``), or any subset of a
     sequence's rows to its front (base = 0).  No counterpart in the reference.
@@ -236,9 +242,9 @@ def compact_rows(pools, block_table, base, keep, n_keep, dst_table=None, stacked
     dst_table: the rows are written through this table instead (pages that the call does not read, or the same table): the
     source keeps its rows.  From the first keep entry that is out of order or range the rest of a sequence is left alone and
     ``_lib.device_status()`` reports it."""
-    first, shape, ptrs, n_pools = _pool_ptrs("compact_rows", pools, stacked)
+    first, shape, ptrs = _pool_ptrs("compact_rows", pools, stacked)
     dst_table = block_table if dst_table is None else dst_table
-    require_same_device(first, block_table, base, keep, n_keep, dst_table)
+    dev = require_same_device(first, block_table, base, keep, n_keep, dst_table)
     for name, t in (("block_table", block_table), ("dst_table", dst_table), ("base", base), ("keep", keep), ("n_keep", n_keep)):
         if t.dtype != torch.int32 or not t.is_contiguous():
             raise ValueError(f"compact_rows: {name} must be contiguous int32")
@@ -251,9 +257,9 @@ def compact_rows(pools, block_table, base, keep, n_keep, dst_table=None, stacked
     if block_table.shape[1] == 0:
         raise ValueError("compact_rows: an empty block table")
     n_pages, heads, page_size, dim = shape
-    with on_device(first.device):
-        check(_lib.load().gdn_rows_compact(ptrs, n_pools, n_pages, heads, page_size, dim * first.element_size(), ptr(block_table), ptr(dst_table),
-                                           block_table.shape[1], ptr(base), ptr(keep), ptr(n_keep), B, L, stream_ptr(first.device)), "compact_rows")
+    with on_device(dev):
+        check(_lib.load().gdn_rows_compact(_address(ptrs), len(ptrs), n_pages, heads, page_size, dim * first.element_size(), block_table.data_ptr(), dst_table.data_ptr(),
+                                           block_table.shape[1], base.data_ptr(), keep.data_ptr(), n_keep.data_ptr(), B, L, raw_stream(dev)), "compact_rows")
 
 
 class Pools:

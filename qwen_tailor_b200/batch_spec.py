@@ -10,13 +10,13 @@ Rollback after a verify is an index choice: the next round passes ``sel = n_new`
 """
 from __future__ import annotations
 
-import ctypes
+from array import array
 
 import torch
 
 from . import _lib
-from ._lib import check, on_device, ptr, require_same_device, stream_ptr
-from .batch import CD, DK, DV, HV, blit
+from ._lib import check, on_device, ptr, raw_stream, require_same_device, stream_ptr
+from .batch import CD, DK, DV, HV, PW, blit
 from .config import Cfg
 from .gated_delta import _f32
 from .kernels import _rows
@@ -55,17 +55,18 @@ def accept_tree(parents, toks, ids):
     parents int32 [B, N] as for ``attn_tree``, N <= 64; toks int32 [B, N] the nodes' tokens (those of roots are taken as confirmed); ids
     int32 [B, N] the target's token after every node.  Returns n_path int32 [B] and path int32 [B, N] (the path's nodes in order, then
     -1): what ``deltanet_commit`` and ``compact_rows`` take.  The round's next token is ids[b, path[b, n_path[b] - 1]]."""
-    require_same_device(parents, toks, ids)
+    dev = require_same_device(parents, toks, ids)
+    shape = parents.shape
     for t in (parents, toks, ids):
-        if t.dtype != torch.int32 or not t.is_contiguous() or t.dim() != 2 or t.shape != parents.shape:
+        if t.dtype != torch.int32 or not t.is_contiguous() or len(shape) != 2 or t.shape != shape:
             raise ValueError("accept_tree: parents, toks and ids must be contiguous int32 [B, N]")
-    B, N = parents.shape
+    B, N = shape
     if not 1 <= N <= 64:
         raise ValueError(f"accept_tree: 1 <= N <= 64 nodes, got {N}")
     path = torch.empty_like(parents)
-    n_path = torch.empty((B,), dtype=torch.int32, device=parents.device)
-    with on_device(parents.device):
-        check(_lib.load().gdn_tree_accept(ptr(parents), ptr(toks), ptr(ids), ptr(path), ptr(n_path), B, N, stream_ptr(parents.device)), "accept_tree")
+    n_path = torch.empty((B,), dtype=torch.int32, device=dev)
+    with on_device(dev):
+        check(_lib.load().gdn_tree_accept(parents.data_ptr(), toks.data_ptr(), ids.data_ptr(), path.data_ptr(), n_path.data_ptr(), B, N, raw_stream(dev)), "accept_tree")
     return n_path, path
 
 
@@ -78,7 +79,7 @@ def deltanet_tree(proj, conv_pool, conv_w, A_log, dt_bias, ssm_pool, slots, pos,
     ``attn_tree``, N <= 64; conv_pool, ssm_pool, slots, pos as for ``deltanet_b``.  Node i continues the conv window and the state that
     its parent leaves.  Returns y [B*N, 2048] bf16; rows of unused nodes are zero.  Conv, silu, norms and gates are computed in fp32
     and rounded nowhere before y; the chained kernels round to bf16 after each step, so the two agree to bf16 rounding."""
-    require_same_device(proj, conv_pool, conv_w, A_log, dt_bias, ssm_pool, slots, pos, parents, out)
+    dev = require_same_device(proj, conv_pool, conv_w, A_log, dt_bias, ssm_pool, slots, pos, parents, out)
     proj, stride = _rows(proj)
     if parents.dtype != torch.int32 or parents.dim() != 2 or not parents.is_contiguous():
         raise ValueError("deltanet_tree: parents must be contiguous int32 [B, N]")
@@ -88,13 +89,16 @@ def deltanet_tree(proj, conv_pool, conv_w, A_log, dt_bias, ssm_pool, slots, pos,
     if not 1 <= N <= 64 or proj.shape[0] != B * N or stride % 4:
         raise ValueError(f"deltanet_tree: 1 <= N <= 64 nodes and proj [B*N, 8224] with a row stride that is a multiple of 4 expected (B={B}, N={N}, proj {tuple(proj.shape)}, stride {stride})")
     if out is None:
-        out = torch.empty((B * N, HV * DV), dtype=torch.bfloat16, device=proj.device)
+        out = torch.empty((B * N, HV * DV), dtype=torch.bfloat16, device=dev)
     elif out.dtype != torch.bfloat16 or not out.is_contiguous() or tuple(out.shape) != (B * N, HV * DV):
         raise ValueError("deltanet_tree: out must be contiguous bf16 [B*N, 2048]")
-    cw = conv_w.to(torch.bfloat16).reshape(-1).contiguous()
-    with on_device(proj.device):
-        check(_lib.load().gdn_tree_verify(ptr(proj), stride, ptr(conv_pool), ptr(cw), ptr(_f32(A_log)), ptr(_f32(dt_bias)), ptr(ssm_pool), ptr(slots), ptr(pos),
-                                          ptr(parents), ssm_pool.shape[0], ptr(out), B, N, stream_ptr(proj.device)), "deltanet_tree")
+    cw = conv_w if conv_w.dtype == torch.bfloat16 and conv_w.is_contiguous() else conv_w.to(torch.bfloat16).contiguous()
+    if cw.numel() != CD * 4 or A_log.numel() != HV or dt_bias.numel() != HV:
+        raise ValueError(f"deltanet_tree: conv_w [6144*4], A_log [16] and dt_bias [16] expected, got {tuple(conv_w.shape)}, {tuple(A_log.shape)}, {tuple(dt_bias.shape)}")
+    A_log, dt_bias = _f32(A_log), _f32(dt_bias)
+    with on_device(dev):
+        check(_lib.load().gdn_tree_verify(proj.data_ptr(), stride, conv_pool.data_ptr(), cw.data_ptr(), A_log.data_ptr(), dt_bias.data_ptr(), ssm_pool.data_ptr(),
+                                          slots.data_ptr(), pos.data_ptr(), parents.data_ptr(), ssm_pool.shape[0], out.data_ptr(), B, N, raw_stream(dev)), "deltanet_tree")
     return out
 
 
@@ -110,12 +114,33 @@ def _check_index(who, B, **arrays):
             raise ValueError(f"{who}: {name} must be contiguous int32 [{B}]")
 
 
-def _layers(x):
-    """Device pointers of the layers of ``x``: a sequence of tensors, or one tensor with a leading layer dimension."""
+def _layers(who, name, x, L, ptrs, contiguous=True):
+    """Appends the device pointers of the layers of ``x`` -- a sequence of L tensors of one layout, or one tensor with a leading layer
+    dimension -- to ``ptrs``; returns a layer's (shape, strides, dtype, device)."""
     if isinstance(x, torch.Tensor):
-        step = x.stride(0) * x.element_size()
-        return [x.data_ptr() + i * step for i in range(x.shape[0])]
-    return [t.data_ptr() for t in x]
+        if x.dim() < 2 or x.shape[0] != L:
+            raise ValueError(f"{who}: {name} {tuple(x.shape)} for {L} layers")
+        shape, strides = x.shape[1:], x.stride()
+        step, p = strides[0] * x.element_size(), x.data_ptr()
+        if step:
+            ptrs.extend(range(p, p + step * L, step))
+        else:
+            ptrs.extend([p] * L)
+        strides, dtype, device = strides[1:], x.dtype, x.device
+        flat = x.is_contiguous() if contiguous else True
+    else:
+        if len(x) != L:
+            raise ValueError(f"{who}: {len(x)} {name} for {L} layers")
+        first = x[0]
+        shape, strides, dtype, device = first.shape, first.stride(), first.dtype, first.device
+        for t in x:
+            if t.shape != shape or t.stride() != strides or t.dtype != dtype or t.device != device:
+                raise ValueError(f"{who}: the layers of {name} must have one shape, type, layout and device")
+            ptrs.append(t.data_ptr())
+        flat = first.is_contiguous() if contiguous else True
+    if not flat:
+        raise ValueError(f"{who}: {name} must be contiguous")
+    return shape, strides, dtype, device
 
 
 def deltanet_commit(projs, conv_pools, conv_ws, A_logs, dt_biases, ssm_pools, slots, pos, path, n_path, dst_slots=None):
@@ -125,35 +150,36 @@ def deltanet_commit(projs, conv_pools, conv_ws, A_logs, dt_biases, ssm_pools, sl
     dt_biases fp32.  slots, pos int32 [B]; path int32 [B, E], n_path int32 [B] from ``accept_tree`` (E may be smaller than N if no path is
     longer).  The state after the path goes to slot dst_slots[b] (default: in place), the window to its buffer (pos + n_path) & 1.
     No destination may be another sequence's slot in the same call.  n_path = 0 leaves a slot as it is (or copies it to its destination)."""
-    args = [projs, conv_pools, conv_ws, A_logs, dt_biases, ssm_pools]
-    L = len(ssm_pools)
-    if L == 0 or any(len(x) != L for x in args):
-        raise ValueError(f"deltanet_commit: every argument needs one entry per layer, got {[len(x) for x in args]}")
-    firsts = [x[0] for x in args]
-    proj, stride = _rows(firsts[0])
+    who, L = "deltanet_commit", len(ssm_pools)
+    if L == 0:
+        raise ValueError(f"{who}: no layers")
+    ptrs = array("Q")
+    row, strides, dtype, _ = proj = _layers(who, "projs", projs, L, ptrs, contiguous=False)
+    conv, weights, a_log, dt_bias, ssm = (_layers(who, name, x, L, ptrs) for name, x in (("conv_pools", conv_pools), ("conv_ws", conv_ws), ("A_logs", A_logs),
+                                                                                           ("dt_biases", dt_biases), ("ssm_pools", ssm_pools)))
+    if dtype != torch.bfloat16 or len(row) != 2 or row[1] < PW or strides[1] != 1:
+        raise ValueError(f"{who}: proj must be bf16 [rows, >= 8224] with unit inner stride, got {tuple(row)} {dtype}")
+    n_slots = ssm[0][0]
+    if ssm[2] != torch.float32 or ssm[0][1:] != (HV, DV, DK) or conv[2] != torch.bfloat16 or conv[0] != (2 * n_slots, 3, CD):
+        raise ValueError(f"{who}: slot pools ssm fp32 [S, 16, 128, 128] and conv bf16 [2 S, 3, 6144] expected, got {tuple(ssm[0])} and {tuple(conv[0])}")
+    if weights[2] != torch.bfloat16 or weights[0].numel() != CD * 4 or any(x[2] != torch.float32 or x[0].numel() != HV for x in (a_log, dt_bias)):
+        raise ValueError(f"{who}: conv_ws bf16 [6144*4], A_logs and dt_biases fp32 [16] per layer expected")
     dst_slots = slots if dst_slots is None else dst_slots
-    require_same_device(*firsts, slots, pos, path, n_path, dst_slots)
-    _check_pools("deltanet_commit", firsts[1], firsts[5])
+    dev = require_same_device(slots, pos, path, n_path, dst_slots)
+    if any(x[3] != dev for x in (proj, conv, weights, a_log, dt_bias, ssm)):
+        raise ValueError(f"{who}: tensors on different devices in one call")
     if path.dtype != torch.int32 or path.dim() != 2 or not path.is_contiguous():
-        raise ValueError("deltanet_commit: path must be contiguous int32 [B, E]")
+        raise ValueError(f"{who}: path must be contiguous int32 [B, E]")
     B, E = path.shape
-    _check_index("deltanet_commit", B, slots=slots, pos=pos, n_path=n_path, dst_slots=dst_slots)
-    if firsts[2].dtype != torch.bfloat16 or firsts[2].numel() != CD * 4 or any(t.dtype != torch.float32 or t.numel() != HV for t in firsts[3:5]):
-        raise ValueError("deltanet_commit: conv_ws bf16 [6144*4], A_logs and dt_biases fp32 [16] per layer expected")
-    for x, first in zip(args, firsts):
-        if not (first.is_contiguous() or x is projs):
-            raise ValueError("deltanet_commit: weights and pools must be contiguous")
-        if not isinstance(x, torch.Tensor):
-            for t in x:
-                if t.shape != first.shape or t.dtype != first.dtype or t.stride() != first.stride() or t.device != first.device:
-                    raise ValueError("deltanet_commit: the layers' tensors must have one shape, type, layout and device")
-    N = proj.shape[0] // B if B else 1
-    if B and (N < 1 or proj.shape[0] != B * N):
-        raise ValueError(f"deltanet_commit: proj has {proj.shape[0]} rows for {B} sequences")
-    table = [(ctypes.c_void_p * L)(*_layers(x)) for x in args]
-    with on_device(proj.device):
-        check(_lib.load().gdn_tree_commit(table[0], stride, *table[1:], L, ptr(slots), ptr(dst_slots), ptr(pos), ptr(path), ptr(n_path), firsts[5].shape[0], B, N, E,
-                                          stream_ptr(proj.device)), "deltanet_commit")
+    _check_index(who, B, slots=slots, pos=pos, n_path=n_path, dst_slots=dst_slots)
+    N = row[0] // B if B else 1
+    if B and (N < 1 or row[0] != B * N):
+        raise ValueError(f"{who}: proj has {row[0]} rows for {B} sequences")
+    base = ptrs.buffer_info()[0]
+    at = [base + 8 * L * i for i in range(6)]
+    with on_device(dev):
+        check(_lib.load().gdn_tree_commit(at[0], strides[0], *at[1:], L, slots.data_ptr(), dst_slots.data_ptr(), pos.data_ptr(), path.data_ptr(), n_path.data_ptr(),
+                                          n_slots, B, N, E, raw_stream(dev)), who)
 
 
 class SpecPools:
