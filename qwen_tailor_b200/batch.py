@@ -11,6 +11,7 @@ from __future__ import annotations
 
 from array import array
 from math import prod
+from numbers import Integral
 from typing import Sequence
 
 import torch
@@ -220,12 +221,12 @@ def copy_entries(pools: Sequence[torch.Tensor], dst: Sequence[int], src: Sequenc
     if rows is not None:
         if len(shape) != 4:
             raise ValueError(f"copy_entries: rows needs pools [n_entries, heads, page_size, dim], got entries of {tuple(shape[1:])}")
-        r = array("q", [rows]) * n if isinstance(rows, int) else array("q", rows)
+        r = array("q", [rows] * n if isinstance(rows, Integral) else rows)
         if len(r) != n or min(r) < 0 or max(r) > shape[2]:
             raise ValueError(f"copy_entries: rows must be one number or {n}, from 0 to {shape[2]}")
         n_sub, sub_bytes = shape[1], shape[2] * shape[3] * item
         row = shape[3] * item
-        lens = array("q", [rows * row]) * n if isinstance(rows, int) else array("q", [x * row for x in r])
+        lens = array("q", [x * row for x in r])
     dev = first.device
     with on_device(dev):
         check(_lib.load().gdn_entries_copy(_address(ptrs), len(ptrs), shape[0], n_sub, sub_bytes, _address(d), _address(s), _address(lens) if lens is not None else None, n,

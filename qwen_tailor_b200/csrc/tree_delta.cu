@@ -12,12 +12,13 @@
 // Conv, silu, norm and gates stay in fp32 here, and nothing is rounded before y (bf16) or the state (fp32): the single-token and
 // chained kernels round to bf16 after each of these operations as the reference's graph does, so results agree with them to
 // bf16 rounding, not bit for bit.
+#include <cuda.h>
 #include "gdn_common.cuh"
 #include "launchers.cuh"
+#include "sm100_prims.cuh"
 
 namespace gdn {
 
-constexpr int TREE_MAX = 64;
 
 __device__ __forceinline__ float silu_f(float x) { return x / (1.f + expf(-x)); }
 __device__ __forceinline__ float log_decay_f(float A_log, float x) { return -expf(A_log) * (fmaxf(x, 0.f) + log1pf(expf(-fabsf(x)))); }
@@ -39,118 +40,360 @@ __device__ __forceinline__ unsigned long long tree_line(const int* par, int i, b
 }
 
 // ----------------------------------------------------------------------------------------------------------------------
-// verify: one block per (sequence, head)
+// verify: one block per (sequence, head), two blocks per SM.  NP = nodes padded to 16, 32 or 64.  Bound: HBM for the state (64 KiB a
+// head) in large batches, latency in small ones.
+//     [P1 | P2] = S0 [K; Q]^T     on the tensor cores, rows = value rows d: S0 in tensor memory, [K; Q] in shared memory
+//     G         = [K; Q] K^T      on the tensor cores
+// each operand as bf16 hi + lo and the three products that matter (what is dropped is 2^-16 of the factors; K and Q rounded to bf16
+// alone would put an error of the size of y's own rounding on every product).  The rest is fp32: thread d of four warps solves
+//     u_i = beta_i (v_i - e^G_i P1_i) - sum_j L_ij u_j
+// for its value row in blocks of 16 nodes, thread d of the other four follows with y_i = e^G_i P2_i + sum_j A_ij u_j.  L and A are
+// dense with zeros outside the ancestors; zeros do not stop NaN, so a head with a non-finite q, k, v or gate takes the sums over the
+// ancestors one by one instead.
+// Shared memory: [K; Q] hi and lo (1 KiB a node), later L and A; a region that receives the state (two halves of 32 KiB where
+// NP = 64, so that two blocks fit an SM) and then holds v and u.
 // ----------------------------------------------------------------------------------------------------------------------
-constexpr int TV_THREADS = 256;
+using namespace sm100;
 
-__global__ void __launch_bounds__(TV_THREADS) tree_verify_kernel(const TreeDeltaArgs a) {
-    extern __shared__ __align__(16) float sm[];
+constexpr int TV_THREADS = 256;
+constexpr float LOG2E = 1.4426950408889634f;
+template <int NP> struct TreeVerify {
+    static constexpr int HALVES = NP == 64 ? 2 : 1;                  // pieces the state arrives in
+    static constexpr int SLAB = 2 * NP * 128;                        // bytes of 64 dims of [K; Q]
+    static constexpr int KQ_BYTES = 4 * SLAB;                        // hi (two slabs), lo
+    static constexpr int ST_BYTES = 65536 / HALVES;
+    static constexpr int SMEM = KQ_BYTES + ST_BYTES;
+    static constexpr uint32_t TM_HI = 0, TM_LO = 64, TM_P = 128, TM_G = 0;       // G replaces S0 (products of one thread run in order)
+};
+
+__device__ __forceinline__ void split_bf16(float x, float y, uint32_t& hi, uint32_t& lo) {
+    hi = pack_bf16x2(x, y);
+    lo = pack_bf16x2(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
+}
+
+template <int NP>
+__global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDeltaArgs a, const __grid_constant__ CUtensorMap tmS) {
+    using C = TreeVerify<NP>;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    __shared__ uint64_t bars[2];                                     // state landed; products done
+    __shared__ unsigned long long s_line[NP];
+    __shared__ int s_par[NP], s_row[NP][4];                          // conv rows of a node: 0..2 the window, 3 + j node j
+    __shared__ float s_lg[NP], s_beta[NP], s_G[NP];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_odd, s_fail;                                    // a non-finite value in this head; a wait gave up
     const int N = a.N, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int b = blockIdx.x / HV, h = blockIdx.x % HV;
-    float *sq = sm, *sk = sq + N * DK, *su = sk + N * DK;            // q, k, v (then u) of the nodes
-    float *skk = su + N * DK, *sqk = skk + N * N;                    // M (k.k) beta, M (q.k)
-    __shared__ int s_par[TREE_MAX];
-    __shared__ unsigned long long s_line[TREE_MAX];
-    __shared__ float s_lg[TREE_MAX], s_beta[TREE_MAX], s_G[TREE_MAX];
+    const uint32_t sKQ = smem_addr(smem), sST = sKQ + C::KQ_BYTES;
+    const uint32_t b_state = smem_addr(&bars[0]), b_mma = smem_addr(&bars[1]);
+    if (sKQ & 1023u) { if (tid == 0) atomicExch(a.status, 4); return; }
     const int slot = a.slots[b], pos = a.pos[b];
     if (slot < 0 || slot >= a.n_slots || pos < 0) {                  // rows of a bad sequence: zeros
         if (tid == 0) atomicExch(a.status, 1);
         for (int i = tid; i < N * DV; i += TV_THREADS) a.y[((size_t)b * N + i / DV) * KD + h * DV + i % DV] = __float2bfloat16_rn(0.f);
         return;
     }
-    if (tid < N) s_par[tid] = a.parents[(size_t)b * N + tid];
-    __syncthreads();
+    auto load_state = [&](int half) {                                // two (or all four) boxes of 32 key columns
+        constexpr int BOXES = 4 / C::HALVES;
+        mbar_expect_tx(b_state, BOXES * 16384);
+        for (int k = 0; k < BOXES; k++) tma_load_2d(sST + k * 16384, &tmS, b_state, 32 * (half * BOXES + k), (slot * HV + h) * DV);
+    };
+    if (tid == 0) {
+        mbar_init(b_state, 1); mbar_init(b_mma, 1);
+        s_odd = s_fail = 0;
+        fence_barrier_init();
+        load_state(0);
+    }
+    if (warp == 7) { tmem_alloc(smem_addr(&s_tmem), 256); tmem_relinquish(); }
+    if (tid < NP) s_par[tid] = tid < N ? a.parents[(size_t)b * N + tid] : -2;
+    float lg = 0.f, beta = 0.f;
     if (tid < N) {
-        bool bad = false;
-        s_line[tid] = tree_line(s_par, tid, bad);
-        if (bad) atomicExch(a.status, 1);
         const __nv_bfloat16* row = a.proj + ((size_t)b * N + tid) * a.row_stride;
-        s_beta[tid] = sigmoid_f(ldbf(row + CD + KD + h));
-        s_lg[tid] = log_decay_f(a.A_log[h], ldbf(row + CD + KD + HV + h) + a.dt_bias[h]);
+        beta = sigmoid_f(ldbf(row + CD + KD + h));
+        lg = log_decay_f(a.A_log[h], ldbf(row + CD + KD + HV + h) + a.dt_bias[h]) * LOG2E;
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tb = s_tmem;
+    if (tid < NP) {
+        bool bad = false;
+        s_line[tid] = tid < N ? tree_line(s_par, tid, bad) : 0;
+        if (bad) atomicExch(a.status, 1);
+        s_lg[tid] = lg; s_beta[tid] = beta;
+        for (int t = 3, e = 3 + tid; t >= 0; t--) {
+            s_row[tid][t] = e;
+            e = e >= 3 ? (s_par[e - 3] >= 0 && s_par[e - 3] < e - 3 ? 3 + s_par[e - 3] : 2) : e - 1;
+        }
     }
     __syncthreads();
-    if (tid < N) {
+    if (tid < NP) {
         float g = 0.f;
         for (unsigned long long m = s_line[tid]; m; m &= m - 1) g += s_lg[__ffsll((long long)m) - 1];
         s_G[tid] = g;
+        if (s_line[tid] && !(isfinite(g) && isfinite(beta))) s_odd = 1;
     }
-    // conv over the path + silu + norms: one node per warp, four channels of q, k and v per lane
+    // ---- conv over the path, silu, norm: one node per warp, four channels per lane; v = false: q and k into the operand, true: v ----
     const __nv_bfloat16* window = a.conv_pool + ((size_t)slot * 2 + (pos & 1)) * 3 * CD;
-    for (int i = warp; i < N; i += TV_THREADS / 32) {
-        if (!s_line[i]) continue;
-        const __nv_bfloat16* row[4];
-        for (int t = 3, e = 3 + i; t >= 0; t--) {                    // rows: window 0..2, then nodes
-            row[t] = e >= 3 ? a.proj + ((size_t)b * N + e - 3) * a.row_stride : window + (size_t)e * CD;
-            e = e >= 3 ? (s_par[e - 3] >= 0 ? 3 + s_par[e - 3] : 2) : e - 1;
+    const __nv_bfloat16* rows = a.proj + (size_t)b * N * a.row_stride;
+    auto front = [&](int g, auto&& put) {
+        const int ch = g * KD + h * DK + 4 * lane;
+        float w[4][4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) unpack_bf16x4(*reinterpret_cast<const uint2*>(a.conv_w + (size_t)(ch + c) * 4), w[c]);
+#pragma unroll 2
+        for (int i = warp; i < NP; i += TV_THREADS / 32) {
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+            if (s_line[i]) {
+                uint2 raw[4];
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const int e = s_row[i][t];
+                    raw[t] = *reinterpret_cast<const uint2*>((e >= 3 ? rows + (size_t)(e - 3) * a.row_stride : window + (size_t)e * CD) + ch);
+                }
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    float r[4];
+                    unpack_bf16x4(raw[t], r);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) x[c] = fmaf(r[c], w[c][t], x[c]);
+                }
+#pragma unroll
+                for (int c = 0; c < 4; c++) x[c] = silu_f(x[c]);
+                const float ss = (x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3]);
+                if (!isfinite(ss)) s_odd = 1;
+                if (g < 2) {
+                    const float scale = rsqrtf(warp_sum(ss) + 1e-6f) * (g == 0 ? 0.08838834764831845f : 1.f);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) x[c] *= scale;
+                }
+            }
+            put(i, x);
         }
+    };
+    auto put_kq = [&](int row, const float (&x)[4]) {                // rows 0 .. NP - 1: K, then Q
+        uint2 hi, lo;
+        split_bf16(x[0], x[1], hi.x, lo.x);
+        split_bf16(x[2], x[3], hi.y, lo.y);
+        const uint32_t at = (lane >> 4) * C::SLAB + row * 128 + ((((lane >> 1) & 7) ^ (row & 7)) << 4) + (lane & 1) * 8;
+        *reinterpret_cast<uint2*>(smem + at) = hi;
+        *reinterpret_cast<uint2*>(smem + 2 * C::SLAB + at) = lo;
+    };
+    front(1, [&](int i, const float (&x)[4]) { put_kq(i, x); });
+    front(0, [&](int i, const float (&x)[4]) { put_kq(NP + i, x); });
+    fence_proxy_async_smem();
+    // ---- the state into tensor memory as hi + lo: lane = value row, warps 0-3 and 4-7 take every other box of 32 key columns ----
+    const uint32_t tl = tb + ((uint32_t)((warp & 3) * 32) << 16);
+    const int d = (warp & 3) * 32 + lane;
+#pragma unroll 1
+    for (int k = 0; k < 2; k++) {
+        const int box = 2 * k + (warp >> 2);
+        if ((k == 0 || C::HALVES == 2) && !mbar_wait(b_state, k)) { s_fail = 1; atomicExch(a.status, 2); }
+        const unsigned char* src = smem + C::KQ_BYTES + (C::HALVES == 2 ? box & 1 : box) * 16384 + d * 128;
+        uint32_t hi[16], lo[16];
 #pragma unroll
-        for (int g = 0; g < 3; g++) {
-            const int ch = g * KD + h * DK + 4 * lane;
-            float acc[4] = {0.f, 0.f, 0.f, 0.f}, w[4][4];
-#pragma unroll
-            for (int c = 0; c < 4; c++) unpack_bf16x4(*reinterpret_cast<const uint2*>(a.conv_w + (size_t)(ch + c) * 4), w[c]);
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) acc[c] = fmaf(ldbf(row[t] + ch + c), w[c][t], acc[c]);
-            float ss = 0.f;
-#pragma unroll
-            for (int c = 0; c < 4; c++) { acc[c] = silu_f(acc[c]); ss += acc[c] * acc[c]; }
-            float scale = 1.f;
-            if (g < 2) scale = rsqrtf(warp_sum(ss) + 1e-6f) * (g == 0 ? 0.08838834764831845f : 1.f);
-            float* dst = (g == 0 ? sq : g == 1 ? sk : su) + i * DK + 4 * lane;
-#pragma unroll
-            for (int c = 0; c < 4; c++) dst[c] = acc[c] * scale;
+        for (int c = 0; c < 8; c++) {
+            const float4 s = *reinterpret_cast<const float4*>(src + ((c ^ (d & 7)) << 4));
+            split_bf16(s.x, s.y, hi[2 * c], lo[2 * c]);
+            split_bf16(s.z, s.w, hi[2 * c + 1], lo[2 * c + 1]);
+        }
+        tmem_st16(tl + C::TM_HI + 16 * box, hi);
+        tmem_st16(tl + C::TM_LO + 16 * box, lo);
+        if (k == 0 && C::HALVES == 2) {
+            __syncthreads();                                         // the first half has been read
+            if (tid == 0) load_state(1);
         }
     }
+    tmem_wait_st();
+    tc_fence_before_sync();
     __syncthreads();
-    for (int p = tid; p < N * N; p += TV_THREADS) {
-        const int i = p / N, j = p % N;
-        float kk = 0.f, qk = 0.f;
-        if (s_line[i] >> j & 1) {
-            for (int c = 0; c < DK; c++) { kk = fmaf(sk[i * DK + c], sk[j * DK + c], kk); qk = fmaf(sq[i * DK + c], sk[j * DK + c], qk); }
-            const float M = expf(s_G[i] - s_G[j]);
-            kk *= M * s_beta[i]; qk *= M;
-        }
-        skk[p] = kk; sqk[p] = qk;
-    }
-    __syncthreads();
-    // two threads per value row, 64 key columns of S0 each
-    const int d = tid >> 1, half = tid & 1;
-    float S[DK / 2];
-    const float4* src = reinterpret_cast<const float4*>(a.ssm_pool + ((size_t)slot * HV + h) * DV * DK + d * DK + half * 64);
+    if (tid == 0) {
+        tc_fence_after_sync();
+        constexpr uint32_t HI = smem_desc_hi_sw128(1024);
+        constexpr uint32_t I_P = idesc_bf16(128, 2 * NP, 0, 0), I_G = idesc_bf16(128, NP, 0, 0);
+        const uint32_t kq = smem_desc_lo(sKQ, 16);
 #pragma unroll
-    for (int c = 0; c < 16; c++) *reinterpret_cast<float4*>(&S[4 * c]) = src[c];
-    for (int i = 0; i < N; i++) {
-        __nv_bfloat16* out = a.y + ((size_t)b * N + i) * KD + h * DV + d;
+        for (int ks = 0; ks < 8; ks++) {
+            const uint32_t bh = kq + (ks >> 2) * (C::SLAB >> 4) + (ks & 3) * 2, bl = bh + 2 * (C::SLAB >> 4);
+            if (ks == 0) mma_ts_w<false>(tb + C::TM_P, tb + C::TM_HI, bh, HI, I_P);
+            else mma_ts_w<true>(tb + C::TM_P, tb + C::TM_HI + 8 * ks, bh, HI, I_P);
+            mma_ts_w<true>(tb + C::TM_P, tb + C::TM_HI + 8 * ks, bl, HI, I_P);
+            mma_ts_w<true>(tb + C::TM_P, tb + C::TM_LO + 8 * ks, bh, HI, I_P);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 8; ks++) {
+            const uint32_t xh = kq + (ks >> 2) * (C::SLAB >> 4) + (ks & 3) * 2, xl = xh + 2 * (C::SLAB >> 4);
+            if (ks == 0) mma_ss_w<false>(tb + C::TM_G, xh, HI, xh, HI, I_G);
+            else mma_ss_w<true>(tb + C::TM_G, xh, HI, xh, HI, I_G);
+            mma_ss_w<true>(tb + C::TM_G, xh, HI, xl, HI, I_G);
+            mma_ss_w<true>(tb + C::TM_G, xl, HI, xh, HI, I_G);
+        }
+        mma_commit(b_mma);
+    }
+    float* su = reinterpret_cast<float*>(smem + C::KQ_BYTES);        // [NP][128]: v, then u
+    front(2, [&](int i, const float (&x)[4]) { *reinterpret_cast<float4*>(su + i * DV + 4 * lane) = make_float4(x[0], x[1], x[2], x[3]); });
+    if (!mbar_wait(b_mma, 0)) { s_fail = 1; atomicExch(a.status, 2); }
+    tc_fence_after_sync();
+    // ---- L[j][i] = beta_i M_ij (k_i . k_j) and A[j][i] = M_ij (q_i . k_j), j along rows, so that a thread reads them for four i at a time ----
+    float* sL = reinterpret_cast<float*>(smem);
+    float* sA = sL + NP * NP;
+    if (d < 2 * NP) {
+        const bool isq = d >= NP;
+        const int i = isq ? d - NP : d;
         const unsigned long long line = s_line[i];
-        if (!line) { if (half == 0) *out = __float2bfloat16_rn(0.f); continue; }
-        float p1 = 0.f, p2 = 0.f;
+        const float g = s_G[i], mul = isq ? 1.f : s_beta[i];
+        float* dst = isq ? sA : sL;
+        for (int j0 = (warp >> 2) * 16; j0 < NP; j0 += 32) {
+            uint32_t r[16];
+            tmem_ld16(tl + C::TM_G + j0, r);
+            tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < 64; c++) { p1 = fmaf(S[c], sk[i * DK + half * 64 + c], p1); p2 = fmaf(S[c], sq[i * DK + half * 64 + c], p2); }
-        p1 += __shfl_xor_sync(0xffffffffu, p1, 1);
-        p2 += __shfl_xor_sync(0xffffffffu, p2, 1);
-        const float grow = expf(s_G[i]);
-        float u = s_beta[i] * (su[i * DK + d] - grow * p1), y = grow * p2;
-        for (unsigned long long m = line & ~(1ull << i); m; m &= m - 1) {
-            const int j = __ffsll((long long)m) - 1;
-            u = fmaf(-skk[i * N + j], su[j * DK + d], u);
-            y = fmaf(sqk[i * N + j], su[j * DK + d], y);
+            for (int c = 0; c < 16; c++) {
+                const int j = j0 + c;
+                const bool on = (line >> j & 1) && (isq || j != i);
+                dst[j * NP + i] = on ? mul * exp2f(g - s_G[j]) * __uint_as_float(r[c]) : 0.f;
+            }
         }
-        y = fmaf(sqk[i * N + i], u, y);
-        __syncwarp();
-        if (half == 0) { su[i * DK + d] = u; *out = __float2bfloat16_rn(y); }      // column d belongs to these two threads
-        __syncwarp();
     }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const bool solver = warp < 4;
+    __nv_bfloat16* out = a.y + (size_t)b * N * KD + h * DV + d;
+    if (!s_odd) {
+#pragma unroll 1
+        for (int I = 0; I < NP / 16; I++) {
+            float x[16];
+            {
+                uint32_t r[16];
+                tmem_ld16(tl + C::TM_P + (solver ? 0 : NP) + 16 * I, r);
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 16; c++) {
+                    const int i = 16 * I + c;
+                    const float grow = exp2f(s_G[i]) * __uint_as_float(r[c]);
+                    x[c] = solver ? s_beta[i] * (su[i * DV + d] - grow) : grow;
+                    if (!s_line[i]) x[c] = 0.f;
+                }
+            }
+            const float* coef = (solver ? sL : sA) + 16 * I;
+            const float sign = solver ? -1.f : 1.f;
+            // the blocks before this one (y: this one too, once its u is there)
+#pragma unroll 1
+            for (int J = 0; J < I + (solver ? 0 : 1); J++) {
+                if (!solver && J == I) asm volatile("bar.sync %0, 256;" ::"r"(1 + I) : "memory");
+#pragma unroll
+                for (int c = 0; c < 16; c++) {
+                    const float u = sign * su[(16 * J + c) * DV + d];
+                    const float4* row = reinterpret_cast<const float4*>(coef + (16 * J + c) * NP);
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const float4 m = row[q];
+                        x[4 * q] = fmaf(m.x, u, x[4 * q]); x[4 * q + 1] = fmaf(m.y, u, x[4 * q + 1]);
+                        x[4 * q + 2] = fmaf(m.z, u, x[4 * q + 2]); x[4 * q + 3] = fmaf(m.w, u, x[4 * q + 3]);
+                    }
+                }
+            }
+            if (solver) {
+#pragma unroll
+                for (int c = 0; c < 15; c++) {
+                    const float4* row = reinterpret_cast<const float4*>(coef + (16 * I + c) * NP);
+#pragma unroll
+                    for (int q = (c + 1) / 4; q < 4; q++) {          // (entries up to c are zero)
+                        const float4 m = row[q];
+                        if (4 * q > c) x[4 * q] = fmaf(-m.x, x[c], x[4 * q]);
+                        if (4 * q + 1 > c) x[4 * q + 1] = fmaf(-m.y, x[c], x[4 * q + 1]);
+                        if (4 * q + 2 > c) x[4 * q + 2] = fmaf(-m.z, x[c], x[4 * q + 2]);
+                        if (4 * q + 3 > c) x[4 * q + 3] = fmaf(-m.w, x[c], x[4 * q + 3]);
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < 16; c++) su[(16 * I + c) * DV + d] = x[c];
+                __threadfence_block();
+                asm volatile("bar.arrive %0, 256;" ::"r"(1 + I) : "memory");
+            } else {
+#pragma unroll
+                for (int c = 0; c < 16; c++)
+                    if (16 * I + c < N) out[(size_t)(16 * I + c) * KD] = __float2bfloat16_rn(x[c]);
+            }
+        }
+    } else if (solver) {
+        // a non-finite value somewhere: only what lies on a node's own path enters its sums
+        for (int i0 = 0; i0 < NP; i0 += 16) {
+            uint32_t r1[16], r2[16];
+            tmem_ld16(tl + C::TM_P + i0, r1);
+            tmem_ld16(tl + C::TM_P + NP + i0, r2);
+            tmem_wait_ld();
+            for (int c = 0; c < 16 && i0 + c < N; c++) {
+                const int i = i0 + c;
+                float p1 = 0.f, p2 = 0.f;
+#pragma unroll
+                for (int k = 0; k < 16; k++) if (k == c) { p1 = __uint_as_float(r1[k]); p2 = __uint_as_float(r2[k]); }
+                const unsigned long long line = s_line[i];
+                const float grow = exp2f(s_G[i]);
+                float u = s_beta[i] * (su[i * DV + d] - grow * p1), y = grow * p2;
+                for (unsigned long long m = line & ~(1ull << i); m; m &= m - 1) {
+                    const int j = __ffsll((long long)m) - 1;
+                    u = fmaf(-sL[j * NP + i], su[j * DV + d], u);
+                    y = fmaf(sA[j * NP + i], su[j * DV + d], y);
+                }
+                y = fmaf(sA[i * NP + i], u, y);
+                su[i * DV + d] = u;                                  // (column d is this thread's)
+                out[(size_t)i * KD] = __float2bfloat16_rn(line ? y : 0.f);
+            }
+        }
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (s_fail && tid == 0) { mbar_wait(b_state, C::HALVES - 1, 100000u); mbar_wait(b_mma, 0, 100000u); }      // copies and products in flight end first
+    __syncthreads();
+    if (warp == 7) tmem_dealloc(tb, 256);
+}
+
+typedef CUresult (*StateEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// the pool as rows of 128 fp32 key columns; box = 32 columns x the 128 value rows of a head
+static bool state_map(CUtensorMap* m, const float* pool, int n_slots) {
+    static StateEncodeFn fn = nullptr;
+    if (!fn) {
+        cudaDriverEntryPointQueryResult qr;
+        void* f = nullptr;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &qr) != cudaSuccess || qr != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            return false;
+        }
+        fn = reinterpret_cast<StateEncodeFn>(f);
+    }
+    const cuuint64_t dims[2] = {DK, (cuuint64_t)n_slots * HV * DV}, strides[1] = {DK * 4};
+    const cuuint32_t box[2] = {32, DV}, es[2] = {1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<float*>(pool), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int NP>
+static int run_tree_verify(const TreeDeltaArgs& a, const CUtensorMap& tm, cudaStream_t st) {
+    static bool attr_set[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 0 && dev < 64 && !attr_set[dev]) {
+        if (cudaFuncSetAttribute(tree_verify_kernel<NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, TreeVerify<NP>::SMEM) != cudaSuccess)
+            return check_launch("tree_verify smem attribute");
+        attr_set[dev] = true;
+    }
+    tree_verify_kernel<NP><<<a.B * HV, TV_THREADS, TreeVerify<NP>::SMEM, st>>>(a, tm);
+    return check_launch("tree_verify");
 }
 
 int launch_tree_verify(const TreeDeltaArgs& a, cudaStream_t st) {
     if (a.B <= 0 || a.N <= 0) return GDN_OK;
-    const int smem = (3 * a.N * DK + 2 * a.N * a.N) * 4;
-    if (cudaFuncSetAttribute(tree_verify_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (3 * TREE_MAX * DK + 2 * TREE_MAX * TREE_MAX) * 4) != cudaSuccess)
-        return check_launch("tree_verify smem attribute");
-    tree_verify_kernel<<<a.B * HV, TV_THREADS, smem, st>>>(a);
-    return check_launch("tree_verify");
+    CUtensorMap tm;
+    if (!state_map(&tm, a.ssm_pool, a.n_slots)) {
+        set_error("gdn_tree_verify: the state's tensor map could not be made");
+        return GDN_E_UNSUPPORTED;
+    }
+    if (a.N <= 16) return run_tree_verify<16>(a, tm, st);
+    if (a.N <= 32) return run_tree_verify<32>(a, tm, st);
+    return run_tree_verify<64>(a, tm, st);
 }
 
 // ----------------------------------------------------------------------------------------------------------------------
