@@ -13,6 +13,7 @@
 // chained kernels round to bf16 after each of these operations as the reference's graph does, so results agree with them to
 // bf16 rounding, not bit for bit.
 #include <cuda.h>
+#include <type_traits>
 #include "gdn_common.cuh"
 #include "launchers.cuh"
 #include "sm100_prims.cuh"
@@ -71,13 +72,22 @@ __device__ __forceinline__ void split_bf16(float x, float y, uint32_t& hi, uint3
     lo = pack_bf16x2(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
 }
 
+// two fp32 fused multiply-adds in one instruction (sm_100): x += a * b on both halves
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float x, float y) { f32x2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y)); return r; }
+__device__ __forceinline__ float2 unpack2(f32x2 v) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v)); return r; }
+__device__ __forceinline__ void fma2(f32x2& x, f32x2 a, f32x2 b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(x) : "l"(a), "l"(b)); }
+// the fast approximations of exp and of the division are good to a few fp32 ulp, far below y's rounding to bf16
+__device__ __forceinline__ float silu_fast(float x) { return __fdividef(x, 1.f + __expf(-x)); }
+
 template <int NP>
 __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDeltaArgs a, const __grid_constant__ CUtensorMap tmS) {
     using C = TreeVerify<NP>;
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ uint64_t bars[2];                                     // state landed; products done
     __shared__ unsigned long long s_line[NP];
-    __shared__ int s_par[NP], s_row[NP][4];                          // conv rows of a node: 0..2 the window, 3 + j node j
+    __shared__ int s_par[NP];
+    __shared__ __align__(16) const __nv_bfloat16* s_row[NP][4];      // conv rows of a node: t-3 .. t along its path
     __shared__ float s_lg[NP], s_beta[NP], s_G[NP];
     __shared__ uint32_t s_tmem;
     __shared__ int s_odd, s_fail;                                    // a non-finite value in this head; a wait gave up
@@ -86,6 +96,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
     const uint32_t sKQ = smem_addr(smem), sST = sKQ + C::KQ_BYTES;
     const uint32_t b_state = smem_addr(&bars[0]), b_mma = smem_addr(&bars[1]);
     if (sKQ & 1023u) { if (tid == 0) atomicExch(a.status, 4); return; }
+    GDN_BSTAMP(0);
     const int slot = a.slots[b], pos = a.pos[b];
     if (slot < 0 || slot >= a.n_slots || pos < 0) {                  // rows of a bad sequence: zeros
         if (tid == 0) atomicExch(a.status, 1);
@@ -120,8 +131,9 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
         s_line[tid] = tid < N ? tree_line(s_par, tid, bad) : 0;
         if (bad) atomicExch(a.status, 1);
         s_lg[tid] = lg; s_beta[tid] = beta;
-        for (int t = 3, e = 3 + tid; t >= 0; t--) {
-            s_row[tid][t] = e;
+        const __nv_bfloat16* window = a.conv_pool + ((size_t)slot * 2 + (pos & 1)) * 3 * CD;
+        for (int t = 3, e = 3 + tid; t >= 0; t--) {                  // e: 0..2 the window, 3 + j node j
+            s_row[tid][t] = e >= 3 ? a.proj + ((size_t)b * N + e - 3) * a.row_stride : window + (size_t)e * CD;
             e = e >= 3 ? (s_par[e - 3] >= 0 && s_par[e - 3] < e - 3 ? 3 + s_par[e - 3] : 2) : e - 1;
         }
     }
@@ -132,42 +144,63 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
         s_G[tid] = g;
         if (s_line[tid] && !(isfinite(g) && isfinite(beta))) s_odd = 1;
     }
-    // ---- conv over the path, silu, norm: one node per warp, four channels per lane; v = false: q and k into the operand, true: v ----
-    const __nv_bfloat16* window = a.conv_pool + ((size_t)slot * 2 + (pos & 1)) * 3 * CD;
-    const __nv_bfloat16* rows = a.proj + (size_t)b * N * a.row_stride;
-    auto front = [&](int g, auto&& put) {
-        const int ch = g * KD + h * DK + 4 * lane;
-        float w[4][4];
+    GDN_BSTAMP(1);
+    // ---- conv over the path, silu, norm: a node per warp, four channels per lane, two nodes' loads in flight; GROUPS = 2: q and k,
+    //      1: v ----
+    auto front = [&](auto first_group, auto groups, auto&& put) {
+        constexpr int G0 = decltype(first_group)::value, GROUPS = decltype(groups)::value;
+        const int ch = h * DK + 4 * lane;
+        f32x2 w[GROUPS][4][2];                                       // taps of channels 0, 1 and of 2, 3
 #pragma unroll
-        for (int c = 0; c < 4; c++) unpack_bf16x4(*reinterpret_cast<const uint2*>(a.conv_w + (size_t)(ch + c) * 4), w[c]);
-#pragma unroll 2
-        for (int i = warp; i < NP; i += TV_THREADS / 32) {
-            float x[4] = {0.f, 0.f, 0.f, 0.f};
-            if (s_line[i]) {
-                uint2 raw[4];
+        for (int g = 0; g < GROUPS; g++) {
+            float f[4][4];
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const int e = s_row[i][t];
-                    raw[t] = *reinterpret_cast<const uint2*>((e >= 3 ? rows + (size_t)(e - 3) * a.row_stride : window + (size_t)e * CD) + ch);
-                }
+            for (int c = 0; c < 4; c++) unpack_bf16x4(*reinterpret_cast<const uint2*>(a.conv_w + (size_t)((G0 + g) * KD + ch + c) * 4), f[c]);
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    float r[4];
-                    unpack_bf16x4(raw[t], r);
+            for (int k = 0; k < 4; k++) { w[g][k][0] = pack2(f[0][k], f[1][k]); w[g][k][1] = pack2(f[2][k], f[3][k]); }
+        }
+#pragma unroll 1
+        for (int i0 = warp; i0 < NP; i0 += 16) {
+            uint2 raw[2][GROUPS][4];
 #pragma unroll
-                    for (int c = 0; c < 4; c++) x[c] = fmaf(r[c], w[c][t], x[c]);
-                }
+            for (int n = 0; n < 2; n++) {
+                const int i = i0 + 8 * n;
+                if (s_line[i])
 #pragma unroll
-                for (int c = 0; c < 4; c++) x[c] = silu_f(x[c]);
-                const float ss = (x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3]);
-                if (!isfinite(ss)) s_odd = 1;
-                if (g < 2) {
-                    const float scale = rsqrtf(warp_sum(ss) + 1e-6f) * (g == 0 ? 0.08838834764831845f : 1.f);
+                    for (int k = 0; k < 4; k++) {
+                        const __nv_bfloat16* row = s_row[i][k] + ch;
 #pragma unroll
-                    for (int c = 0; c < 4; c++) x[c] *= scale;
+                        for (int g = 0; g < GROUPS; g++) raw[n][g][k] = *reinterpret_cast<const uint2*>(row + (G0 + g) * KD);
+                    }
+            }
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                const int i = i0 + 8 * n;
+                const bool on = s_line[i] != 0;
+#pragma unroll
+                for (int g = 0; g < GROUPS; g++) {
+                    float x[4] = {0.f, 0.f, 0.f, 0.f};
+                    if (on) {
+                        f32x2 s0 = 0, s1 = 0;
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const uint2 r = raw[n][g][k];
+                            fma2(s0, pack2(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u)), w[g][k][0]);
+                            fma2(s1, pack2(__uint_as_float(r.y << 16), __uint_as_float(r.y & 0xffff0000u)), w[g][k][1]);
+                        }
+                        const float2 a0 = unpack2(s0), a1 = unpack2(s1);
+                        x[0] = silu_fast(a0.x); x[1] = silu_fast(a0.y); x[2] = silu_fast(a1.x); x[3] = silu_fast(a1.y);
+                        float ss = (x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3]);
+                        if (!(ss < INFINITY)) s_odd = 1;
+                        if (G0 + g < 2) {
+                            const float scale = rsqrtf(warp_sum(ss) + 1e-6f) * (G0 + g == 0 ? 0.08838834764831845f : 1.f);
+#pragma unroll
+                            for (int c = 0; c < 4; c++) x[c] *= scale;
+                        }
+                    }
+                    put(g, i, x);
                 }
             }
-            put(i, x);
         }
     };
     auto put_kq = [&](int row, const float (&x)[4]) {                // rows 0 .. NP - 1: K, then Q
@@ -178,8 +211,8 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
         *reinterpret_cast<uint2*>(smem + at) = hi;
         *reinterpret_cast<uint2*>(smem + 2 * C::SLAB + at) = lo;
     };
-    front(1, [&](int i, const float (&x)[4]) { put_kq(i, x); });
-    front(0, [&](int i, const float (&x)[4]) { put_kq(NP + i, x); });
+    front(std::integral_constant<int, 0>(), std::integral_constant<int, 2>(), [&](int g, int i, const float (&x)[4]) { put_kq((g == 0 ? NP : 0) + i, x); });
+    GDN_BSTAMP(2);
     fence_proxy_async_smem();
     // ---- the state into tensor memory as hi + lo: lane = value row, warps 0-3 and 4-7 take every other box of 32 key columns ----
     const uint32_t tl = tb + ((uint32_t)((warp & 3) * 32) << 16);
@@ -206,7 +239,8 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
     tmem_wait_st();
     tc_fence_before_sync();
     __syncthreads();
-    if (tid == 0) {
+    GDN_BSTAMP(3);
+    if (tid == TV_THREADS - 32) {
         tc_fence_after_sync();
         constexpr uint32_t HI = smem_desc_hi_sw128(1024);
         constexpr uint32_t I_P = idesc_bf16(128, 2 * NP, 0, 0), I_G = idesc_bf16(128, NP, 0, 0);
@@ -229,10 +263,13 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
         }
         mma_commit(b_mma);
     }
+    GDN_BSTAMP(4);
     float* su = reinterpret_cast<float*>(smem + C::KQ_BYTES);        // [NP][128]: v, then u
-    front(2, [&](int i, const float (&x)[4]) { *reinterpret_cast<float4*>(su + i * DV + 4 * lane) = make_float4(x[0], x[1], x[2], x[3]); });
+    front(std::integral_constant<int, 2>(), std::integral_constant<int, 1>(), [&](int, int i, const float (&x)[4]) { *reinterpret_cast<float4*>(su + i * DV + 4 * lane) = make_float4(x[0], x[1], x[2], x[3]); });
+    GDN_BSTAMP(5);
     if (!mbar_wait(b_mma, 0)) { s_fail = 1; atomicExch(a.status, 2); }
     tc_fence_after_sync();
+    GDN_BSTAMP(6);
     // ---- L[j][i] = beta_i M_ij (k_i . k_j) and A[j][i] = M_ij (q_i . k_j), j along rows, so that a thread reads them for four i at a time ----
     float* sL = reinterpret_cast<float*>(smem);
     float* sA = sL + NP * NP;
@@ -257,63 +294,79 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
+    GDN_BSTAMP(7);
     const bool solver = warp < 4;
     __nv_bfloat16* out = a.y + (size_t)b * N * KD + h * DV + d;
     if (!s_odd) {
 #pragma unroll 1
         for (int I = 0; I < NP / 16; I++) {
-            float x[16];
+            f32x2 x[8];                                              // nodes 16 I + 2 k, + 1
+            unsigned long long rel = 0;                              // who is on the path of one of them
             {
                 uint32_t r[16];
                 tmem_ld16(tl + C::TM_P + (solver ? 0 : NP) + 16 * I, r);
                 tmem_wait_ld();
+                float f[16];
 #pragma unroll
                 for (int c = 0; c < 16; c++) {
                     const int i = 16 * I + c;
+                    const unsigned long long line = s_line[i];
+                    rel |= line;
                     const float grow = exp2f(s_G[i]) * __uint_as_float(r[c]);
-                    x[c] = solver ? s_beta[i] * (su[i * DV + d] - grow) : grow;
-                    if (!s_line[i]) x[c] = 0.f;
+                    f[c] = line ? (solver ? s_beta[i] * (su[i * DV + d] - grow) : grow) : 0.f;
                 }
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[k] = pack2(f[2 * k], f[2 * k + 1]);
             }
             const float* coef = (solver ? sL : sA) + 16 * I;
             const float sign = solver ? -1.f : 1.f;
-            // the blocks before this one (y: this one too, once its u is there)
-#pragma unroll 1
-            for (int J = 0; J < I + (solver ? 0 : 1); J++) {
-                if (!solver && J == I) asm volatile("bar.sync %0, 256;" ::"r"(1 + I) : "memory");
+            auto add = [&](int j, float u) {                         // x += coef[j] u
+                const ulonglong2* row = reinterpret_cast<const ulonglong2*>(coef + j * NP);
+                const f32x2 uu = pack2(u, u);
 #pragma unroll
-                for (int c = 0; c < 16; c++) {
-                    const float u = sign * su[(16 * J + c) * DV + d];
-                    const float4* row = reinterpret_cast<const float4*>(coef + (16 * J + c) * NP);
-#pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        const float4 m = row[q];
-                        x[4 * q] = fmaf(m.x, u, x[4 * q]); x[4 * q + 1] = fmaf(m.y, u, x[4 * q + 1]);
-                        x[4 * q + 2] = fmaf(m.z, u, x[4 * q + 2]); x[4 * q + 3] = fmaf(m.w, u, x[4 * q + 3]);
-                    }
+                for (int q = 0; q < 4; q++) {
+                    const ulonglong2 m = row[q];
+                    fma2(x[2 * q], m.x, uu);
+                    fma2(x[2 * q + 1], m.y, uu);
                 }
+            };
+            // nodes of earlier blocks, only those that are an ancestor of one of these: two at a time (the odd one out once more, with 0)
+            for (unsigned long long m = rel & ((1ull << 16 * I) - 1); m;) {
+                const int j = __ffsll((long long)m) - 1;
+                m &= m - 1;
+                const int j2 = m ? __ffsll((long long)m) - 1 : j;
+                const float u = sign * su[j * DV + d], u2 = m ? sign * su[j2 * DV + d] : 0.f;
+                m &= m - 1;
+                add(j, u);
+                add(j2, u2);
             }
             if (solver) {
 #pragma unroll
-                for (int c = 0; c < 15; c++) {
-                    const float4* row = reinterpret_cast<const float4*>(coef + (16 * I + c) * NP);
+                for (int c = 0; c < 16; c++) {                       // (entries up to c are zero)
+                    const float2 p = unpack2(x[c / 2]);
+                    const float u = c & 1 ? p.y : p.x;
+                    su[(16 * I + c) * DV + d] = u;
+                    const f32x2 uu = pack2(-u, -u);
+                    const ulonglong2* row = reinterpret_cast<const ulonglong2*>(coef + (16 * I + c) * NP);
 #pragma unroll
-                    for (int q = (c + 1) / 4; q < 4; q++) {          // (entries up to c are zero)
-                        const float4 m = row[q];
-                        if (4 * q > c) x[4 * q] = fmaf(-m.x, x[c], x[4 * q]);
-                        if (4 * q + 1 > c) x[4 * q + 1] = fmaf(-m.y, x[c], x[4 * q + 1]);
-                        if (4 * q + 2 > c) x[4 * q + 2] = fmaf(-m.z, x[c], x[4 * q + 2]);
-                        if (4 * q + 3 > c) x[4 * q + 3] = fmaf(-m.w, x[c], x[4 * q + 3]);
+                    for (int q = c / 4; q < 4; q++) {
+                        const ulonglong2 m = row[q];
+                        if (4 * q + 1 > c) fma2(x[2 * q], m.x, uu);
+                        if (4 * q + 3 > c) fma2(x[2 * q + 1], m.y, uu);
                     }
                 }
-#pragma unroll
-                for (int c = 0; c < 16; c++) su[(16 * I + c) * DV + d] = x[c];
                 __threadfence_block();
                 asm volatile("bar.arrive %0, 256;" ::"r"(1 + I) : "memory");
             } else {
+                asm volatile("bar.sync %0, 256;" ::"r"(1 + I) : "memory");
+#pragma unroll 4
+                for (int c = 0; c < 16; c++) add(16 * I + c, su[(16 * I + c) * DV + d]);
 #pragma unroll
-                for (int c = 0; c < 16; c++)
-                    if (16 * I + c < N) out[(size_t)(16 * I + c) * KD] = __float2bfloat16_rn(x[c]);
+                for (int k = 0; k < 8; k++) {
+                    const float2 v = unpack2(x[k]);
+                    if (16 * I + 2 * k < N) out[(size_t)(16 * I + 2 * k) * KD] = __float2bfloat16_rn(v.x);
+                    if (16 * I + 2 * k + 1 < N) out[(size_t)(16 * I + 2 * k + 1) * KD] = __float2bfloat16_rn(v.y);
+                }
             }
         }
     } else if (solver) {
@@ -342,8 +395,10 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
             }
         }
     }
+    GDN_BSTAMP(8);
     tc_fence_before_sync();
     __syncthreads();
+    GDN_BSTAMP(9);
     if (s_fail && tid == 0) { mbar_wait(b_state, C::HALVES - 1, 100000u); mbar_wait(b_mma, 0, 100000u); }      // copies and products in flight end first
     __syncthreads();
     if (warp == 7) tmem_dealloc(tb, 256);
@@ -554,3 +609,9 @@ int launch_tree_commit(const TreeCommitArgs& a, int n_layers, cudaStream_t st) {
 }
 
 }  // namespace gdn
+
+#ifdef GDN_TIMING
+extern "C" __attribute__((visibility("default"))) int gdn_timing_log_delta(long long* out_host, int n) {
+    return cudaMemcpyFromSymbol(out_host, gdn::g_tlog, sizeof(long long) * n) == cudaSuccess ? 0 : -5;
+}
+#endif
