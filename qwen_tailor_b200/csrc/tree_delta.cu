@@ -63,7 +63,7 @@ template <int NP> struct TreeVerify {
     static constexpr int SLAB = 2 * NP * 128;                        // bytes of 64 dims of [K; Q]
     static constexpr int KQ_BYTES = 4 * SLAB;                        // hi (two slabs), lo
     static constexpr int ST_BYTES = 65536 / HALVES;
-    static constexpr int SMEM = KQ_BYTES + ST_BYTES;
+    static constexpr int SMEM = KQ_BYTES + ST_BYTES + DV * 4;        // + a row of zeros behind the last u
     static constexpr uint32_t TM_HI = 0, TM_LO = 64, TM_P = 128, TM_G = 0;       // G replaces S0 (products of one thread run in order)
 };
 
@@ -88,7 +88,10 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
     __shared__ unsigned long long s_line[NP];
     __shared__ int s_par[NP];
     __shared__ __align__(16) const __nv_bfloat16* s_row[NP][4];      // conv rows of a node: t-3 .. t along its path
-    __shared__ float s_lg[NP], s_beta[NP], s_G[NP];
+    __shared__ float s_lg[NP], s_beta[NP];
+    __shared__ __align__(16) float s_G[NP], s_grow[NP], s_bgrow[NP];  // G (log2), e^G, beta e^G
+    __shared__ __align__(4) unsigned char s_list[NP / 16][NP];       // per block of 16 nodes: their ancestors in earlier blocks,
+    __shared__ int s_cnt[NP / 16];                                   // in fours (filled up with NP, the row of zeros)
     __shared__ uint32_t s_tmem;
     __shared__ int s_odd, s_fail;                                    // a non-finite value in this head; a wait gave up
     const int N = a.N, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -133,7 +136,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
         s_lg[tid] = lg; s_beta[tid] = beta;
         const __nv_bfloat16* window = a.conv_pool + ((size_t)slot * 2 + (pos & 1)) * 3 * CD;
         for (int t = 3, e = 3 + tid; t >= 0; t--) {                  // e: 0..2 the window, 3 + j node j
-            s_row[tid][t] = e >= 3 ? a.proj + ((size_t)b * N + e - 3) * a.row_stride : window + (size_t)e * CD;
+            s_row[tid][t] = tid >= N ? window : e >= 3 ? a.proj + ((size_t)b * N + e - 3) * a.row_stride : window + (size_t)e * CD;
             e = e >= 3 ? (s_par[e - 3] >= 0 && s_par[e - 3] < e - 3 ? 3 + s_par[e - 3] : 2) : e - 1;
         }
     }
@@ -142,9 +145,25 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
         float g = 0.f;
         for (unsigned long long m = s_line[tid]; m; m &= m - 1) g += s_lg[__ffsll((long long)m) - 1];
         s_G[tid] = g;
+        s_grow[tid] = s_line[tid] ? exp2f(g) : 0.f;
+        s_bgrow[tid] = s_line[tid] ? beta * exp2f(g) : 0.f;
         if (s_line[tid] && !(isfinite(g) && isfinite(beta))) s_odd = 1;
     }
     GDN_BSTAMP(1);
+    if (warp >= 8 - NP / 16) {                                       // the lists, one block of nodes per warp
+        const int I = warp - (8 - NP / 16);
+        unsigned long long rel = 0;
+        for (int i = 0; i < 16; i++) rel |= s_line[16 * I + i];
+        rel &= (1ull << (16 * I)) - 1;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int j = lane + 32 * k;
+            if (j < NP && (rel >> j & 1)) s_list[I][__popcll(rel & ((1ull << j) - 1))] = (unsigned char)j;
+        }
+        const int cnt = __popcll(rel);
+        if (lane < 3 && cnt + lane < NP) s_list[I][cnt + lane] = NP;
+        if (lane == 0) s_cnt[I] = cnt;
+    }
     // ---- conv over the path, silu, norm: a node per warp, four channels per lane, two nodes' loads in flight; GROUPS = 2: q and k,
     //      1: v ----
     auto front = [&](auto first_group, auto groups, auto&& put) {
@@ -163,44 +182,57 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
         for (int i0 = warp; i0 < NP; i0 += 16) {
             uint2 raw[2][GROUPS][4];
 #pragma unroll
-            for (int n = 0; n < 2; n++) {
-                const int i = i0 + 8 * n;
-                if (s_line[i])
+            for (int n = 0; n < 2; n++)
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const __nv_bfloat16* row = s_row[i][k] + ch;
+                for (int k = 0; k < 4; k++) {
+                    const __nv_bfloat16* row = s_row[i0 + 8 * n][k] + ch;
 #pragma unroll
-                        for (int g = 0; g < GROUPS; g++) raw[n][g][k] = *reinterpret_cast<const uint2*>(row + (G0 + g) * KD);
-                    }
-            }
+                    for (int g = 0; g < GROUPS; g++) raw[n][g][k] = *reinterpret_cast<const uint2*>(row + (G0 + g) * KD);
+                }
+            float x[2][GROUPS][4], ss[2 * GROUPS];
 #pragma unroll
             for (int n = 0; n < 2; n++) {
-                const int i = i0 + 8 * n;
-                const bool on = s_line[i] != 0;
+                const bool on = s_line[i0 + 8 * n] != 0;
 #pragma unroll
                 for (int g = 0; g < GROUPS; g++) {
-                    float x[4] = {0.f, 0.f, 0.f, 0.f};
-                    if (on) {
-                        f32x2 s0 = 0, s1 = 0;
+                    f32x2 s0 = 0, s1 = 0;
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const uint2 r = raw[n][g][k];
-                            fma2(s0, pack2(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u)), w[g][k][0]);
-                            fma2(s1, pack2(__uint_as_float(r.y << 16), __uint_as_float(r.y & 0xffff0000u)), w[g][k][1]);
-                        }
-                        const float2 a0 = unpack2(s0), a1 = unpack2(s1);
-                        x[0] = silu_fast(a0.x); x[1] = silu_fast(a0.y); x[2] = silu_fast(a1.x); x[3] = silu_fast(a1.y);
-                        float ss = (x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3]);
-                        if (!(ss < INFINITY)) s_odd = 1;
-                        if (G0 + g < 2) {
-                            const float scale = rsqrtf(warp_sum(ss) + 1e-6f) * (G0 + g == 0 ? 0.08838834764831845f : 1.f);
-#pragma unroll
-                            for (int c = 0; c < 4; c++) x[c] *= scale;
-                        }
+                    for (int k = 0; k < 4; k++) {
+                        const uint2 r = raw[n][g][k];
+                        fma2(s0, pack2(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u)), w[g][k][0]);
+                        fma2(s1, pack2(__uint_as_float(r.y << 16), __uint_as_float(r.y & 0xffff0000u)), w[g][k][1]);
                     }
-                    put(g, i, x);
+                    const float2 a0 = unpack2(s0), a1 = unpack2(s1);
+                    float (&y)[4] = x[n][g];
+                    y[0] = on ? silu_fast(a0.x) : 0.f; y[1] = on ? silu_fast(a0.y) : 0.f;
+                    y[2] = on ? silu_fast(a1.x) : 0.f; y[3] = on ? silu_fast(a1.y) : 0.f;
+                    ss[n * GROUPS + g] = (y[0] * y[0] + y[1] * y[1]) + (y[2] * y[2] + y[3] * y[3]);
+                    if (!(ss[n * GROUPS + g] < INFINITY)) s_odd = 1;
                 }
             }
+            if (G0 == 0) {
+                // the four sums over the warp in seven shuffles: each quarter of the lanes ends up with one of them
+                const bool up = lane & 16, odd = lane & 8;
+                const float t0 = (up ? ss[1] : ss[0]) + __shfl_xor_sync(0xffffffffu, up ? ss[0] : ss[1], 16);
+                const float t1 = (up ? ss[2 * GROUPS - 1] : ss[2 * GROUPS - 2]) + __shfl_xor_sync(0xffffffffu, up ? ss[2 * GROUPS - 2] : ss[2 * GROUPS - 1], 16);
+                float q = (odd ? t1 : t0) + __shfl_xor_sync(0xffffffffu, odd ? t0 : t1, 8);
+                q += __shfl_xor_sync(0xffffffffu, q, 4);
+                q += __shfl_xor_sync(0xffffffffu, q, 2);
+                q += __shfl_xor_sync(0xffffffffu, q, 1);
+                const float r = rsqrtf(q + 1e-6f);                   // lanes 0-7: node 0 q, 16-23: node 0 k, 8-15: node 1 q, 24-31: node 1 k
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int g = 0; g < GROUPS; g++) {
+                        const float scale = __shfl_sync(0xffffffffu, r, 16 * g + 8 * n) * (g == 0 ? 0.08838834764831845f : 1.f);
+#pragma unroll
+                        for (int c = 0; c < 4; c++) x[n][g][c] *= scale;
+                    }
+            }
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int g = 0; g < GROUPS; g++) put(g, i0 + 8 * n, x[n][g]);
         }
     };
     auto put_kq = [&](int row, const float (&x)[4]) {                // rows 0 .. NP - 1: K, then Q
@@ -265,7 +297,11 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
     }
     GDN_BSTAMP(4);
     float* su = reinterpret_cast<float*>(smem + C::KQ_BYTES);        // [NP][128]: v, then u
-    front(std::integral_constant<int, 2>(), std::integral_constant<int, 1>(), [&](int, int i, const float (&x)[4]) { *reinterpret_cast<float4*>(su + i * DV + 4 * lane) = make_float4(x[0], x[1], x[2], x[3]); });
+    front(std::integral_constant<int, 2>(), std::integral_constant<int, 1>(), [&](int, int i, const float (&x)[4]) {
+        const float m = s_line[i] ? s_beta[i] : 0.f;
+        *reinterpret_cast<float4*>(su + i * DV + 4 * lane) = s_line[i] ? make_float4(m * x[0], m * x[1], m * x[2], m * x[3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+    });
+    if (tid < DV) su[NP * DV + tid] = 0.f;
     GDN_BSTAMP(5);
     if (!mbar_wait(b_mma, 0)) { s_fail = 1; atomicExch(a.status, 2); }
     tc_fence_after_sync();
@@ -276,18 +312,19 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
     if (d < 2 * NP) {
         const bool isq = d >= NP;
         const int i = isq ? d - NP : d;
-        const unsigned long long line = s_line[i];
+        const unsigned long long line = isq ? s_line[i] : s_line[i] & ~(1ull << i);
         const float g = s_G[i], mul = isq ? 1.f : s_beta[i];
-        float* dst = isq ? sA : sL;
+        float* dst = (isq ? sA : sL) + i;
         for (int j0 = (warp >> 2) * 16; j0 < NP; j0 += 32) {
             uint32_t r[16];
             tmem_ld16(tl + C::TM_G + j0, r);
             tmem_wait_ld();
+            const uint32_t on = (uint32_t)(line >> j0);
 #pragma unroll
             for (int c = 0; c < 16; c++) {
-                const int j = j0 + c;
-                const bool on = (line >> j & 1) && (isq || j != i);
-                dst[j * NP + i] = on ? mul * exp2f(g - s_G[j]) * __uint_as_float(r[c]) : 0.f;
+                float e;
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g - s_G[j0 + c]));
+                dst[(j0 + c) * NP] = on >> c & 1 ? mul * e * __uint_as_float(r[c]) : 0.f;
             }
         }
     }
@@ -301,27 +338,28 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
 #pragma unroll 1
         for (int I = 0; I < NP / 16; I++) {
             f32x2 x[8];                                              // nodes 16 I + 2 k, + 1
-            unsigned long long rel = 0;                              // who is on the path of one of them
             {
                 uint32_t r[16];
                 tmem_ld16(tl + C::TM_P + (solver ? 0 : NP) + 16 * I, r);
                 tmem_wait_ld();
+                const float4* grow = reinterpret_cast<const float4*>((solver ? s_bgrow : s_grow) + 16 * I);
                 float f[16];
 #pragma unroll
-                for (int c = 0; c < 16; c++) {
-                    const int i = 16 * I + c;
-                    const unsigned long long line = s_line[i];
-                    rel |= line;
-                    const float grow = exp2f(s_G[i]) * __uint_as_float(r[c]);
-                    f[c] = line ? (solver ? s_beta[i] * (su[i * DV + d] - grow) : grow) : 0.f;
+                for (int q = 0; q < 4; q++) {
+                    const float4 m = grow[q];
+                    f[4 * q] = m.x * __uint_as_float(r[4 * q]); f[4 * q + 1] = m.y * __uint_as_float(r[4 * q + 1]);
+                    f[4 * q + 2] = m.z * __uint_as_float(r[4 * q + 2]); f[4 * q + 3] = m.w * __uint_as_float(r[4 * q + 3]);
                 }
+                if (solver)
+#pragma unroll
+                    for (int c = 0; c < 16; c++) f[c] = su[(16 * I + c) * DV + d] - f[c];
 #pragma unroll
                 for (int k = 0; k < 8; k++) x[k] = pack2(f[2 * k], f[2 * k + 1]);
             }
             const float* coef = (solver ? sL : sA) + 16 * I;
             const float sign = solver ? -1.f : 1.f;
             auto add = [&](int j, float u) {                         // x += coef[j] u
-                const ulonglong2* row = reinterpret_cast<const ulonglong2*>(coef + j * NP);
+                const ulonglong2* row = reinterpret_cast<const ulonglong2*>(coef + (j & (NP - 1)) * NP);      // (NP, with u = 0: any row)
                 const f32x2 uu = pack2(u, u);
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
@@ -330,15 +368,14 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
                     fma2(x[2 * q + 1], m.y, uu);
                 }
             };
-            // nodes of earlier blocks, only those that are an ancestor of one of these: two at a time (the odd one out once more, with 0)
-            for (unsigned long long m = rel & ((1ull << 16 * I) - 1); m;) {
-                const int j = __ffsll((long long)m) - 1;
-                m &= m - 1;
-                const int j2 = m ? __ffsll((long long)m) - 1 : j;
-                const float u = sign * su[j * DV + d], u2 = m ? sign * su[j2 * DV + d] : 0.f;
-                m &= m - 1;
-                add(j, u);
-                add(j2, u2);
+            // nodes of earlier blocks, only those that are an ancestor of one of these, four at a time
+            for (int k = 0; k < s_cnt[I]; k += 4) {
+                const uint32_t js = *reinterpret_cast<const uint32_t*>(&s_list[I][k]);
+                float u[4];
+#pragma unroll
+                for (int q = 0; q < 4; q++) u[q] = sign * su[(js >> 8 * q & 255) * DV + d];
+#pragma unroll
+                for (int q = 0; q < 4; q++) add(js >> 8 * q & 255, u[q]);
             }
             if (solver) {
 #pragma unroll
@@ -359,8 +396,18 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
                 asm volatile("bar.arrive %0, 256;" ::"r"(1 + I) : "memory");
             } else {
                 asm volatile("bar.sync %0, 256;" ::"r"(1 + I) : "memory");
-#pragma unroll 4
-                for (int c = 0; c < 16; c++) add(16 * I + c, su[(16 * I + c) * DV + d]);
+#pragma unroll
+                for (int c = 0; c < 16; c++) {                       // (entries before c are zero)
+                    const float u = su[(16 * I + c) * DV + d];
+                    const f32x2 uu = pack2(u, u);
+                    const ulonglong2* row = reinterpret_cast<const ulonglong2*>(coef + (16 * I + c) * NP);
+#pragma unroll
+                    for (int q = c / 4; q < 4; q++) {
+                        const ulonglong2 m = row[q];
+                        fma2(x[2 * q], m.x, uu);
+                        fma2(x[2 * q + 1], m.y, uu);
+                    }
+                }
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
                     const float2 v = unpack2(x[k]);
@@ -383,7 +430,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
                 for (int k = 0; k < 16; k++) if (k == c) { p1 = __uint_as_float(r1[k]); p2 = __uint_as_float(r2[k]); }
                 const unsigned long long line = s_line[i];
                 const float grow = exp2f(s_G[i]);
-                float u = s_beta[i] * (su[i * DV + d] - grow * p1), y = grow * p2;
+                float u = su[i * DV + d] - s_beta[i] * grow * p1, y = grow * p2;
                 for (unsigned long long m = line & ~(1ull << i); m; m &= m - 1) {
                     const int j = __ffsll((long long)m) - 1;
                     u = fmaf(-sL[j * NP + i], su[j * DV + d], u);
