@@ -100,6 +100,11 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
     const uint32_t b_state = smem_addr(&bars[0]), b_mma = smem_addr(&bars[1]);
     if (sKQ & 1023u) { if (tid == 0) atomicExch(a.status, 4); return; }
     GDN_BSTAMP(0);
+    // every row of the tree is first touched in the conv, a few rows at a time: asked for now, they come out of L2 then
+    for (int k = tid; k < N * 6; k += TV_THREADS) {
+        const __nv_bfloat16* line = a.proj + ((size_t)b * N + k / 6) * a.row_stride + (k % 6 >> 1) * KD + h * DK + (k & 1) * 64;
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
+    }
     const int slot = a.slots[b], pos = a.pos[b];
     if (slot < 0 || slot >= a.n_slots || pos < 0) {                  // rows of a bad sequence: zeros
         if (tid == 0) atomicExch(a.status, 1);
