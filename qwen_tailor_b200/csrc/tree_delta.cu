@@ -21,7 +21,6 @@
 namespace gdn {
 
 
-__device__ __forceinline__ float silu_f(float x) { return x / (1.f + expf(-x)); }
 __device__ __forceinline__ float log_decay_f(float A_log, float x) { return -expf(A_log) * (fmaxf(x, 0.f) + log1pf(expf(-fabsf(x)))); }
 __device__ __forceinline__ float sigmoid_f(float x) { return 1.f / (1.f + expf(-x)); }
 
@@ -548,108 +547,148 @@ int launch_tree_accept(const int* parents, const int* toks, const int* ids, int*
 }
 
 // ----------------------------------------------------------------------------------------------------------------------
-// commit: one block per (layer, sequence, head).  Bound: HBM, the state once in and once out (2 MiB per layer and sequence).  The
-// state lies in registers -- a row on 8 lanes of 4 float4 each, so that a quarter warp reads 128 contiguous bytes -- and is requested
-// before the conv / norm / gate work of the path's tokens, which hides behind its latency.
+// commit: one block per (layer, sequence, head), two per SM.  Bound: HBM, the state once in and once out (2 MiB per layer and
+// sequence), and behind it the issue slots (about 10 k instructions a head and four tokens).  The state lies in registers, a row on 8
+// lanes of 4 float4 each, so that a quarter warp reads 128 contiguous bytes.  Two levels of loads, each all at once, because a load
+// costs microseconds while the states stream: first the indices, the path and the weights, then everything they point to; the
+// conv / norm / gate work of the path's tokens runs while the state arrives.  24 sequences x 18 layers: 253 us (3.8 TB/s); measured
+// and not kept: half heads on four blocks per SM (305), 512 threads a head (309), the next states prefetched into L2 (268), persistent
+// blocks with a bulk-copy ring, preparing warps and eight tokens at a time (225 .. 380 by variant, 25 against 16 us for one sequence).
 // ----------------------------------------------------------------------------------------------------------------------
-constexpr int CM_THREADS = 256, CM_STEPS = 16;                      // tokens of the path prepared at a time
+constexpr int CM_THREADS = 256, CM_STEPS = 16;                       // tokens of the path prepared at a time
+constexpr int CM_PATH = 64, CM_AHEAD = 8;                            // path entries kept in shared memory; raw rows in flight
+
+// silu to a few fp32 ulp: expf's own error and an approximate division
+__device__ __forceinline__ float silu_ulp(float x) { return __fdividef(x, 1.f + expf(-x)); }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) { f32x2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 
 __global__ void __launch_bounds__(CM_THREADS, 2) tree_commit_kernel(const __grid_constant__ TreeCommitArgs a) {
-    __shared__ float s_k[CM_STEPS][DK], s_v[CM_STEPS][DV], s_g[CM_STEPS], s_beta[CM_STEPS], s_red[CM_STEPS][4];
-    __shared__ int s_bad;
+    __shared__ __align__(16) float s_k[CM_STEPS][DK];
+    __shared__ float s_v[CM_STEPS][DV], s_g[CM_STEPS], s_beta[CM_STEPS], s_red[CM_STEPS][4];
+    __shared__ int s_path[CM_PATH];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int layer = blockIdx.y, b = blockIdx.x / HV, h = blockIdx.x % HV;
-    const int slot = a.slots[b], dst = a.dst_slots[b], pos = a.pos[b], n = a.n_path[b];
+    const int h = blockIdx.x % HV, b = blockIdx.x / HV, layer = blockIdx.y;
+    const bool isv = tid >= 128;                                     // threads 0-127: channel of k (and the window of q's), the others: of v
+    const int c = tid & 127, ch = (isv ? 2 : 1) * KD + h * DK + c, chq = h * DK + c;
     const int* path = a.path + (size_t)b * a.E;
-    if (tid == 0) s_bad = 0;
-    __syncthreads();
-    if (slot < 0 || slot >= a.n_slots || dst < 0 || dst >= a.n_slots || pos < 0 || n < 0 || n > a.E) { if (tid == 0) atomicExch(a.status, 1); return; }
-    for (int j = tid; j < n; j += CM_THREADS)
-        if (path[j] < 0 || path[j] >= a.N) s_bad = 1;
-    __syncthreads();
-    if (s_bad) { if (tid == 0) atomicExch(a.status, 1); return; }
-    if (n == 0 && slot == dst) return;
-    // ---- the state ----
-    const size_t head = (size_t)h * DV * DK;
-    const int row = warp * 16 + (lane >> 3), col = (lane & 7) * 4;   // rows row + 4 i, columns col + 32 m
-    float4 S[4][4];
-    {
-        const float* src = a.ssm_pool[layer] + (size_t)slot * STATE_ELEMS + head;
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int m = 0; m < 4; m++) S[i][m] = __ldcs(reinterpret_cast<const float4*>(src + (row + 4 * i) * DK + col + 32 * m));
-    }
-    // ---- the conv window: thread t < 128 owns channel t of q and of k, the others channel t - 128 of v ----
-    const int c = tid & 127;
-    const bool isv = tid >= 128;
-    const __nv_bfloat16* proj = a.proj[layer] + (size_t)b * a.N * a.row_stride;
+    const int first = tid < CM_PATH && tid < a.E ? path[tid] : 0;
+    const int slot = a.slots[b], dst = a.dst_slots[b], pos = a.pos[b], n = a.n_path[b];
+    const uint2 taps = *reinterpret_cast<const uint2*>(a.conv_w[layer] + (size_t)ch * 4);
+    const float A_log = a.A_log[layer][h], dt_bias = a.dt_bias[layer][h];
+    bool bad = slot < 0 || slot >= a.n_slots || dst < 0 || dst >= a.n_slots || pos < 0 || n < 0 || n > a.E;
+    if (!bad && n == 0 && slot == dst) return;
+    if (tid < CM_PATH) s_path[tid] = first;
+    bad = bad || (tid < n && tid < CM_PATH && (first < 0 || first >= a.N));
+    if (!bad)
+        for (int j = CM_PATH + tid; j < n; j += CM_THREADS) bad = bad || path[j] < 0 || path[j] >= a.N;
+    if (__syncthreads_or(bad)) { if (tid == 0) atomicExch(a.status, 1); return; }
+    auto node = [&](int j) -> int { return j < CM_PATH ? s_path[j] : path[j]; };
+    const __nv_bfloat16* rows = a.proj[layer] + (size_t)b * a.N * a.row_stride;
     const __nv_bfloat16* win = a.conv_pool[layer] + ((size_t)slot * 2 + (pos & 1)) * 3 * CD;
-    __nv_bfloat16* wout = a.conv_pool[layer] + ((size_t)dst * 2 + (((unsigned)pos + (unsigned)n) & 1)) * 3 * CD;
-    const int ch = (isv ? 2 : 1) * KD + h * DK + c, chq = h * DK + c;
-    float w[4];
-    unpack_bf16x4(*reinterpret_cast<const uint2*>(a.conv_w[layer] + (size_t)ch * 4), w);
-    // raw row r of the sequence: r = 0..2 the window, 3 + j the path's tokens
-    auto raw = [&](int r, int chan) -> __nv_bfloat16 { return r < 3 ? win[(size_t)r * CD + chan] : proj[(size_t)path[r - 3] * a.row_stride + chan]; };
-    __nv_bfloat16 x0 = raw(0, ch), x1 = raw(1, ch), x2 = raw(2, ch);
-    __nv_bfloat16 q0, q1, q2;
+    // raw row r of the sequence: 0..2 the window, 3 + j the path's tokens
+    auto raw = [&](int r, int chan) -> __nv_bfloat16 { return r < 3 ? win[(size_t)r * CD + chan] : rows[(size_t)node(r - 3) * a.row_stride + chan]; };
+    __nv_bfloat16 x0 = win[ch], x1 = win[CD + ch], x2 = win[2 * CD + ch], q0, q1, q2;
     if (!isv) { q0 = raw(n, chq); q1 = raw(n + 1, chq); q2 = raw(n + 2, chq); }
-    for (int j0 = 0; j0 < n; j0 += CM_STEPS) {
-        const int cnt = min(CM_STEPS, n - j0);
-        __syncthreads();                                             // the steps before have read the shared rows
-        if (tid < cnt) {
-            const __nv_bfloat16* r = proj + (size_t)path[j0 + tid] * a.row_stride;
-            s_beta[tid] = sigmoid_f(ldbf(r + CD + KD + h));
-            s_g[tid] = expf(log_decay_f(a.A_log[layer][h], ldbf(r + CD + KD + HV + h) + a.dt_bias[layer][h]));
-        }
-        for (int j = 0; j < cnt; j++) {
-            const __nv_bfloat16 x3 = raw(3 + j0 + j, ch);
-            float v = fmaf(__bfloat162float(x3), w[3], fmaf(__bfloat162float(x2), w[2], fmaf(__bfloat162float(x1), w[1], __bfloat162float(x0) * w[0])));
-            v = silu_f(v);
-            x0 = x1; x1 = x2; x2 = x3;
-            if (isv) s_v[j][c] = v;
-            else {
-                s_k[j][c] = v;
-                const float ss = warp_sum(v * v);
-                if (lane == 0) s_red[j][warp] = ss;
-            }
-        }
-        __syncthreads();
-        if (!isv)
-            for (int j = 0; j < cnt; j++) s_k[j][c] *= rsqrtf(s_red[j][0] + s_red[j][1] + s_red[j][2] + s_red[j][3] + 1e-6f);
-        __syncthreads();
-        for (int j = 0; j < cnt; j++) {
-            const float g = s_g[j], beta = s_beta[j];
-            float4 k[4];
+    __nv_bfloat16 x[CM_AHEAD];                                       // the next raw rows
+    auto fetch = [&](int j0) {
 #pragma unroll
-            for (int m = 0; m < 4; m++) k[m] = *reinterpret_cast<const float4*>(&s_k[j][col + 32 * m]);
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float p = 0.f;
-#pragma unroll
-                for (int m = 0; m < 4; m++) {
-                    float4& s = S[i][m];
-                    s.x *= g; s.y *= g; s.z *= g; s.w *= g;
-                    p = fmaf(s.x, k[m].x, fmaf(s.y, k[m].y, fmaf(s.z, k[m].z, fmaf(s.w, k[m].w, p))));
-                }
-                p += __shfl_xor_sync(0xffffffffu, p, 1);
-                p += __shfl_xor_sync(0xffffffffu, p, 2);
-                p += __shfl_xor_sync(0xffffffffu, p, 4);
-                const float d = (s_v[j][row + 4 * i] - p) * beta;
-#pragma unroll
-                for (int m = 0; m < 4; m++) {
-                    float4& s = S[i][m];
-                    s.x = fmaf(d, k[m].x, s.x); s.y = fmaf(d, k[m].y, s.y); s.z = fmaf(d, k[m].z, s.z); s.w = fmaf(d, k[m].w, s.w);
-                }
-            }
-        }
-    }
-    float* out = a.ssm_pool[layer] + (size_t)dst * STATE_ELEMS + head;
+        for (int q = 0; q < CM_AHEAD; q++)
+            if (j0 + q < n) x[q] = rows[(size_t)node(j0 + q) * a.row_stride + ch];
+    };
+    fetch(0);
+    __nv_bfloat16 raw_a, raw_b;
+    auto fetch_gates = [&](int j) {
+        const __nv_bfloat16* r = rows + (size_t)node(j) * a.row_stride + CD + KD + h;
+        raw_b = r[0]; raw_a = r[HV];
+    };
+    if (tid < min(n, CM_STEPS)) fetch_gates(tid);
+    // ---- the state ----
+    const int row = warp * 16 + (lane >> 3), col = (lane & 7) * 4;   // rows row + 4 i, columns col + 32 m
+    const size_t at = (size_t)h * DV * DK + (size_t)row * DK + col;
+    const float* src = a.ssm_pool[layer] + (size_t)slot * STATE_ELEMS + at;
+    ulonglong2 S[4][4];
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int m = 0; m < 4; m++) __stcs(reinterpret_cast<float4*>(out + (row + 4 * i) * DK + col + 32 * m), S[i][m]);
+        for (int m = 0; m < 4; m++) {
+            const float4 v = __ldcs(reinterpret_cast<const float4*>(src + 4 * i * DK + 32 * m));
+            S[i][m] = make_ulonglong2(pack2(v.x, v.y), pack2(v.z, v.w));
+        }
+    float w[4];
+    unpack_bf16x4(taps, w);
+    for (int j0 = 0; j0 < n; j0 += CM_STEPS) {
+        const int cnt = min(CM_STEPS, n - j0);
+        if (j0) {
+            __syncthreads();                                         // the steps before have read the shared rows
+            if (tid < cnt) fetch_gates(j0 + tid);
+        }
+        if (tid < cnt) {
+            s_beta[tid] = sigmoid_f(__bfloat162float(raw_b));
+            s_g[tid] = expf(log_decay_f(A_log, __bfloat162float(raw_a) + dt_bias));
+        }
+        for (int j1 = 0; j1 < cnt; j1 += CM_AHEAD) {
+            if (j0 + j1) fetch(j0 + j1);
+#pragma unroll
+            for (int q = 0; q < CM_AHEAD; q++) {
+                if (j1 + q >= cnt) break;
+                const float f = fmaf(__bfloat162float(x[q]), w[3], fmaf(__bfloat162float(x2), w[2], fmaf(__bfloat162float(x1), w[1], __bfloat162float(x0) * w[0])));
+                const float v = silu_ulp(f);
+                x0 = x1; x1 = x2; x2 = x[q];
+                if (isv) s_v[j1 + q][c] = v;
+                else {
+                    s_k[j1 + q][c] = v;
+                    const float ss = warp_sum(v * v);
+                    if (lane == 0) s_red[j1 + q][warp] = ss;
+                }
+            }
+        }
+        __syncthreads();
+        for (int j = 0; j < cnt; j++) {
+            // k is used as it left the conv; its length enters the two places where k does
+            const float r = rsqrtf((s_red[j][0] + s_red[j][1]) + (s_red[j][2] + s_red[j][3]) + 1e-6f);
+            const float g = s_g[j], beta = s_beta[j];
+            const f32x2 gg = pack2(g, g);
+            ulonglong2 k[4];
+#pragma unroll
+            for (int m = 0; m < 4; m++) k[m] = *reinterpret_cast<const ulonglong2*>(&s_k[j][col + 32 * m]);
+            float p[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                f32x2 p0 = 0, p1 = 0;
+#pragma unroll
+                for (int m = 0; m < 4; m++) {
+                    S[i][m].x = mul2(S[i][m].x, gg); S[i][m].y = mul2(S[i][m].y, gg);
+                    fma2(p0, S[i][m].x, k[m].x); fma2(p1, S[i][m].y, k[m].y);
+                }
+                const float2 a0 = unpack2(p0), a1 = unpack2(p1);
+                p[i] = (a0.x + a0.y) + (a1.x + a1.y);
+            }
+            // the four rows' sums over their eight lanes: two exchanges leave lane l with row l & 3's, one more completes it
+            const bool o1 = lane & 1, o2 = lane & 2;
+            const float t0 = (o1 ? p[1] : p[0]) + __shfl_xor_sync(0xffffffffu, o1 ? p[0] : p[1], 1);
+            const float t1 = (o1 ? p[3] : p[2]) + __shfl_xor_sync(0xffffffffu, o1 ? p[2] : p[3], 1);
+            float s = (o2 ? t1 : t0) + __shfl_xor_sync(0xffffffffu, o2 ? t0 : t1, 2);
+            s += __shfl_xor_sync(0xffffffffu, s, 4);
+            const float u = (s_v[j][row + 4 * (lane & 3)] - s * r) * beta * r;      // of row `row + 4 (lane & 3)`
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float ui = __shfl_sync(0xffffffffu, u, (lane & 24) + i);
+                const f32x2 uu = pack2(ui, ui);
+#pragma unroll
+                for (int m = 0; m < 4; m++) { fma2(S[i][m].x, uu, k[m].x); fma2(S[i][m].y, uu, k[m].y); }
+            }
+        }
+    }
+    float* out = a.ssm_pool[layer] + (size_t)dst * STATE_ELEMS + at;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+            const float2 lo = unpack2(S[i][m].x), hi = unpack2(S[i][m].y);
+            __stcs(reinterpret_cast<float4*>(out + 4 * i * DK + 32 * m), make_float4(lo.x, lo.y, hi.x, hi.y));
+        }
     // a window buffer that is read and written in one call (n even): every channel has been read by the thread that writes it
+    __nv_bfloat16* wout = a.conv_pool[layer] + ((size_t)dst * 2 + (((unsigned)pos + (unsigned)n) & 1)) * 3 * CD;
     wout[ch] = x0; wout[CD + ch] = x1; wout[2 * CD + ch] = x2;
     if (!isv) { wout[chq] = q0; wout[CD + chq] = q1; wout[2 * CD + chq] = q2; }
 }
