@@ -41,6 +41,7 @@ constexpr int TA_SLOT = 16384, TA_NK = 5, TA_NV = 5;                  // K slab:
 constexpr int TA_Q_BYTES = 65536;                                     // 128 rows, or two buffers of up to 64 rows
 constexpr int TA_SMEM = TA_Q_BYTES + (TA_NK + TA_NV) * TA_SLOT;
 constexpr uint32_t TAM_O = 0, TAM_SP0 = 256;
+constexpr int TA_TAIL = 1;                                            // plan weight of a pair's epilogue, in tiles (about 3 us against 2.7)
 constexpr float TA_RAISE = 8.f;                                       // log2 units
 enum {
     AB_QFULL = 0, AB_QEMPTY = 2, AB_KFULL = 4, AB_KEMPTY = AB_KFULL + TA_NK, AB_VFULL = AB_KEMPTY + TA_NK, AB_VEMPTY = AB_VFULL + TA_NV,
@@ -58,10 +59,10 @@ struct TreeAttnPlan {
     int k_box, v_box;            // keys per copy
 };
 
-struct TreeSeg { int b, kvh, rt, t0, n, tiles, ctx; bool more; };     // tiles [t0, t0 + n) of a pair with `tiles` of them; more: the block's range goes on
+struct TreeSeg { int b, kvh, rt, t0, n, span, tiles, ctx; };          // tiles [t0, t0 + n) of a pair with `tiles` of them; span: of the plan
 
 // {i, ancestors} of nodes lane and lane + 32 of one tree, as bit masks (0 = unused); par0 / par1: their parents (-2 beyond N)
-__device__ __forceinline__ void warp_lines(int par0, int par1, unsigned long long& l0, unsigned long long& l1, bool& bad) {
+__device__ __noinline__ void warp_lines(int par0, int par1, unsigned long long& l0, unsigned long long& l1, bool& bad) {
     const int lane = threadIdx.x & 31;
     const bool late0 = par0 >= lane, late1 = par1 >= lane + 32;      // a parent that does not precede its child
     if (late0) par0 = -2;
@@ -70,6 +71,7 @@ __device__ __forceinline__ void warp_lines(int par0, int par1, unsigned long lon
     int at0 = par0 < -1 ? -2 : par0, at1 = par1 < -1 ? -2 : par1;    // >= 0: still walking, -1: reached the root, -2: unused
     l0 = 1ull << lane; l1 = 1ull << (lane + 32);
     const bool in0 = par0 >= -1, in1 = par1 >= -1;
+#pragma unroll 1
     while (__any_sync(0xffffffffu, at0 >= 0 || at1 >= 0)) {
         if (at0 >= 0) l0 |= 1ull << at0;
         if (at1 >= 0) l1 |= 1ull << at1;
@@ -145,6 +147,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
         if (ctx < 0 || ctx > cap) return -1;
         if ((long long)ctx + a.N > cap) {                            // (rare: only then do the tree's unused nodes matter)
             int last = a.N - 1;
+#pragma unroll 1
             while (last >= 0 && a.parents[(size_t)b * a.N + last] < -1) last--;
             if ((long long)ctx + last >= cap) return -1;
         }
@@ -152,6 +155,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
     };
     if (warp == 0) {
         int run = 0;
+#pragma unroll 1
         for (int b0 = 0; b0 < a.B; b0 += 32) {
             const int b = b0 + lane;
             int x = 0;
@@ -159,7 +163,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                 const int ctx = context(b);
                 if (ctx < 0 && blockIdx.x == 0) atomicExch(a.status, 1);
                 s_ctx[b] = ctx;
-                x = ((max(ctx, 0) + TA_TK - 1) / TA_TK + 1) * PP;
+                x = ((max(ctx, 0) + TA_TK - 1) / TA_TK + 1 + TA_TAIL) * PP;
             }
             const int own = x;
 #pragma unroll
@@ -203,22 +207,24 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
     // the part of the block's range that starts at tile x: it ends with the pair or with the range
     auto segment = [&](int x) -> TreeSeg {
         int l = 0, r = a.B - 1;
+#pragma unroll 1
         while (l < r) { const int m = (l + r + 1) >> 1; if (s_cum[m] <= x) l = m; else r = m - 1; }
         TreeSeg s;
         s.b = l;
         s.ctx = s_ctx[l];
         s.tiles = (max(s.ctx, 0) + TA_TK - 1) / TA_TK + 1;
-        const int off = x - s_cum[l], pr = off / s.tiles;
-        s.t0 = off - pr * s.tiles;
+        const int off = x - s_cum[l], len = s.tiles + TA_TAIL, pr = off / len;
+        s.t0 = off - pr * len;
         s.kvh = pr / p.row_tiles; s.rt = pr - s.kvh * p.row_tiles;
-        s.n = min(s.tiles - s.t0, hi - x);
-        s.more = x + s.n < hi;
+        s.span = min(len - s.t0, hi - x);
+        s.n = min(s.tiles - s.t0, s.span);                           // (0 or less where the range starts in a pair's tail)
         return s;
     };
     const uint32_t sQ = sbase, sK = sbase + TA_Q_BYTES, sV = sK + TA_NK * TA_SLOT;
     // keys of tile t of a segment's pair (the last tile holds the nodes)
     auto limit_of = [&](const TreeSeg& s, int t) -> int { return t == s.tiles - 1 ? a.N : min(TA_TK, s.ctx - t * TA_TK); };
 
+    if (tid == 0) *reinterpret_cast<int2*>(p.info + 2 * blockIdx.x) = make_int2(0, 0);      // (no pair to join, as far as is known)
     if (warp == 5 || warp == 6) {
         // ================= producers: warp 5 Q and K, warp 6 V =================
         // Lane i works out page and row of box i of a tile (a tile has at most 32 boxes where the page size is a multiple of 4); page
@@ -234,9 +240,11 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
         else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(stream_policy));
         uint32_t nr = 0, nseg = 0;                                   // slots filled so far
         bool okp = true;
-        for (int x = lo; x < hi && okp; nseg++) {
+#pragma unroll 1
+        for (int x = lo; x < hi && okp;) {
             const TreeSeg s = segment(x);
-            x += s.n;
+            x += s.span;
+            if (s.n <= 0) continue;
             if (isk) {
                 const int qb = nseg % p.q_bufs;
                 if (nseg >= (uint32_t)p.q_bufs && !warp_wait(AB_QEMPTY + qb, nseg / p.q_bufs - 1)) { okp = false; break; }
@@ -256,11 +264,13 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
             };
             int w = s.t0 * TA_TK / a.page_size;                      // first entry of the current window
             int cur = entry(w + lane), nxt = entry(w + 32 + lane);
+#pragma unroll 1
             for (int t = s.t0; t < s.t0 + s.n && okp; t++) {
                 const int limit = limit_of(s, t);
                 const bool nodes = t == s.tiles - 1;
                 if (!nodes && per_tile <= 32) {
                     const int first = t * TA_TK / a.page_size;
+#pragma unroll 1
                     while (first >= w + 32) { w += 32; cur = nxt; nxt = entry(w + 32 + lane); }
                     const int key = min(t * TA_TK + lane * box, s.ctx - 1), e = key / a.page_size - w;      // (boxes behind the context are not copied)
                     const int p0 = __shfl_sync(0xffffffffu, cur, e & 31), p1 = __shfl_sync(0xffffffffu, nxt, e & 31);
@@ -274,6 +284,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                 const int i0 = isk ? 0 : j * per_chunk;              // this lane's boxes [i0, i0 + cnt)
                 const int cnt = isk ? (limit + box - 1) / box : (min(32, limit - 32 * j) + box - 1) / box;
                 bool todo = lane < steps;
+#pragma unroll 1
                 for (uint32_t polls = 0; __any_sync(0xffffffffu, todo); polls++) {
                     if (todo && (round == 0 || mbar_test_wait(empty, (round - 1) & 1u))) {
                         todo = false;
@@ -283,6 +294,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                             else for (int k = 0; k < 4; k++) tma_load_3d(dst + k * 4096, &tmVn, full, 64 * k, s.kvh, s.b * a.N + 32 * j);
                         } else {
                             mbar_expect_tx(full, cnt * box * (isk ? 128 : 512));
+#pragma unroll 1
                             for (int i = 0; i < cnt; i++) {
                                 int2 at;
                                 if (per_tile <= 32) at = s_box[warp - 5][i0 + i];
@@ -292,6 +304,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                                 }
                                 // V: the four 64-dim blocks of 32 rows are the chunk's image; of smaller boxes each block is a copy of its own
                                 const int copies = isk || box == 32 ? 1 : 4;
+#pragma unroll 1
                                 for (int k = 0; k < copies; k++)
                                     asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5, %6, %7}], [%2], %8;"
                                                  ::"r"(dst + i * box * 128 + k * 4096), "l"(isk ? &tmK : &tmV), "r"(full), "r"(0), "r"(at.y), "r"(isk ? j : k), "r"(s.kvh), "r"(at.x), "l"(stream_policy) : "memory");
@@ -308,8 +321,8 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                 }
                 nr += steps;
                 __syncwarp();                                        // (s_box is rewritten by the next tile)
-                GDN_TSTAMP((int)(x - s.n - lo + t - s.t0) * 16 + (isk ? 8 : 9));
             }
+            nseg++;
         }
         if (!okp && lane == 0) {                                     // gave up: the copies in flight have to land before the block leaves
             for (int i = 0; i < ring; i++) if (nr > (uint32_t)i) mbar_wait(bar(first_full + i), ((nr - 1 - i) / ring) & 1, 100000u);
@@ -330,6 +343,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                 if (first && ps > 0 && !wait(AB_OFREE, ps - 1)) return false;      // the epilogue before has read O
                 GDN_TSTAMP(m * 16 + 2);
                 uint32_t acc = first ? 0 : 1;                        // the first product of a segment overwrites O
+#pragma unroll 2
                 for (int c = 0; 32 * c < limit; c++) {
                     if (!wait(AB_VFULL + v_slot, v_round)) return false;
                     tc_fence_after_sync();
@@ -352,17 +366,21 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
             int p_limit = 0;
             bool p_have = false, p_first = false, p_last = false;
             uint32_t p_seg = 0;
-            for (int x = lo; x < hi && ok; nseg++) {
+#pragma unroll 1
+            for (int x = lo; x < hi && ok;) {
                 const TreeSeg s = segment(x);
-                x += s.n;
+                x += s.span;
+                if (s.n <= 0) continue;
                 const int qb = nseg % p.q_bufs;
                 if (!wait(AB_QFULL + qb, nseg / p.q_bufs)) { ok = false; break; }
                 const uint32_t qlo = smem_desc_lo(sQ + qb * (TA_Q_BYTES / 2), 16);
-                for (int t = s.t0; t < s.t0 + s.n && ok; t++, n++) {
+#pragma unroll 1
+            for (int t = s.t0; t < s.t0 + s.n && ok; t++, n++) {
                     // the buffer of tile n held P of tile n - 2, whose product was issued before: MMAs of one thread run in order
                     const uint32_t sp = tb + TAM_SP0 + (n & 1) * 128;
                     const uint32_t idesc = t == s.tiles - 1 ? I_QN : I_QK;
                     GDN_TSTAMP(n * 16 + 0);
+#pragma unroll
                     for (int j = 0; j < 4; j++) {
                         if (!wait(AB_KFULL + k_slot, k_round)) { ok = false; break; }
                         tc_fence_after_sync();
@@ -380,15 +398,17 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                     if (p_have) ok = issue_pv(n - 1, p_limit, p_first, p_last, p_seg);
                     p_have = true; p_limit = limit_of(s, t); p_first = t == s.t0; p_last = t == s.t0 + s.n - 1; p_seg = nseg;
                 }
+                nseg++;
             }
             if (ok && p_have) ok = issue_pv(n - 1, p_limit, p_first, p_last, p_seg);
             if (!ok) { mma_commit(bar(AB_DRAIN)); mbar_wait(bar(AB_DRAIN), 0, 100000u); }      // gave up: nothing may run on after the block
         }
     } else if (warp == 7) {
         // ================= append: the nodes' rows into the cache, by the block that has a pair's first tile =================
+#pragma unroll 1
         for (int x = lo; x < hi;) {
             const TreeSeg s = segment(x);
-            x += s.n;
+            x += s.span;
             if (s.t0 != 0 || s.rt != 0 || s.ctx < 0) continue;
             const int* par = a.parents + (size_t)s.b * a.N;
             unsigned long long l0, l1;
@@ -397,6 +417,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
             if (bad) atomicExch(a.status, 1);
             const unsigned long long used = __ballot_sync(0xffffffffu, l0 != 0) | (unsigned long long)__ballot_sync(0xffffffffu, l1 != 0) << 32;
             const int* table = a.block_table + (size_t)s.b * a.max_pages;
+#pragma unroll 1
             for (int i = 0; i < a.N; i++) {
                 if (!(used >> i & 1)) continue;
                 const int at = s.ctx + i;
@@ -414,9 +435,11 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
         const uint32_t tl = tb + ((uint32_t)(warp * 32) << 16);      // this warp's TMEM lanes
         uint32_t n = 0, nv = 0, nseg = 0, node_tiles = 0;
         bool ok = true;
-        for (int x = lo; x < hi; nseg++) {
+#pragma unroll 1
+        for (int x = lo; x < hi;) {
             const TreeSeg s = segment(x);
-            x += s.n;
+            x += s.span;
+            if (s.n <= 0) continue;
             const int node = s.rt * p.nodes + local;
             const bool real = row < p.rows && node < a.N;
             const bool has_nodes = s.t0 + s.n == s.tiles;
@@ -428,6 +451,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
             }
             unsigned long long line = 0, badv = 0;
             float m_run = -INFINITY, l_run = 0.f;
+#pragma unroll 1
             for (int t = s.t0; t < s.t0 + s.n && ok; t++, n++) {
                 const int limit = limit_of(s, t), chunks = (limit + 31) / 32;
                 const bool nodes = t == s.tiles - 1;
@@ -521,10 +545,12 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                     if (n > 0 && !warp_wait(AB_PFREE + ((n - 1) & 1), (n - 1) >> 1)) { ok = false; break; }
                     unsigned long long seen_bad = 0;
                     // (nodes: all rows of its chunks; the last context tile: the rows behind the context, up to the next multiple of 16 keys)
+#pragma unroll 1
                     for (int c = nodes ? 0 : chunks - 1; c < chunks && ok; c++) {
                         const int slot = (nv + c) % TA_NV;
                         if (!warp_wait(AB_VFULL + slot, (nv + c) / TA_NV)) { ok = false; break; }
                         const int r0 = nodes ? 0 : limit & 31, r1 = nodes ? 32 : (r0 + 15) & ~15;
+#pragma unroll 1
                         for (int i = row; i < (r1 - r0) * 32; i += n_warps * 32) {
                             const int r = r0 + (i >> 5), k = 32 * c + r, ch = i & 31;
                             uint4* at = reinterpret_cast<uint4*>(smem + TA_Q_BYTES + TA_NK * TA_SLOT + slot * TA_SLOT + (ch >> 3) * 4096 + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
@@ -577,6 +603,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                 tmem_ld32(tl + TAM_O + c0, u);
                 tmem_wait_ld();
                 if (add) {
+#pragma unroll 1
                     for (unsigned long long r = add; r; r &= r - 1) {
                         const __nv_bfloat16* v = a.v_new + (((size_t)s.b * a.N + (__ffsll((long long)r) - 1)) * a.KV + s.kvh) * ATT_D + c0;
 #pragma unroll
@@ -610,20 +637,17 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(AB_OFREE));
             GDN_BSTAMP(nseg == 0 ? 5 : 8);
-            if (tid == 0 && !s.more) {
+            if (tid == 0 && s.t0 == 0 && !whole) {
                 // the pair that starts in this block and goes on in the next ones is joined by the merge kernel
-                const int first = hi - s.n - s.t0;
-                int parts = 0;
-                if (s.t0 == 0 && !whole) {
-                    parts = 1;
-                    while (range_lo(blockIdx.x + parts, G, N_all) < first + s.tiles) parts++;
-                }
-                p.info[2 * blockIdx.x] = (s.b * a.KV + s.kvh) * p.row_tiles + s.rt;
-                p.info[2 * blockIdx.x + 1] = parts;
+                int parts = 1;
+#pragma unroll 1
+                while (range_lo(blockIdx.x + parts, G, N_all) < hi - s.n + s.tiles) parts++;
+                *reinterpret_cast<int2*>(p.info + 2 * blockIdx.x) = make_int2((s.b * a.KV + s.kvh) * p.row_tiles + s.rt, parts);
             }
+            nseg++;
         }
     }
-    if (tid == 0 && (lo >= hi || aborted())) p.info[2 * blockIdx.x + 1] = 0;
+    if (tid == 0 && aborted()) p.info[2 * blockIdx.x + 1] = 0;
     tc_fence_before_sync();
     __syncthreads();
     if (warp == 4) tmem_dealloc(tb, 512);
@@ -631,27 +655,36 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
 }
 
 // Joins the partials of the pair that starts in main block blockIdx.x and is cut: eight rows per block, a thread holds four columns of a row.
-// Bound: latency (a few hundred KiB out of L2), so all a block's (m, l) pairs are fetched at once and every thread has four partials in flight.
-constexpr int TM_THREADS = 512, TM_ROWS = 8;
+// Bound: latency (a few hundred KiB out of L2), so all a block needs is requested at once, six partials a thread.
+constexpr int TM_THREADS = 512, TM_ROWS = 8, TM_AHEAD = 6;
 
 __global__ void __launch_bounds__(TM_THREADS) tree_attn_merge_kernel(const __grid_constant__ TreeAttnPlan p) {
     __shared__ float s_w[148][TM_ROWS], s_l[148][TM_ROWS];
     __shared__ unsigned char s_live[TM_ROWS];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int g = blockIdx.x, parts = p.info[2 * g + 1];
+    const int g = blockIdx.x;
+    const int2 info = *reinterpret_cast<const int2*>(p.info + 2 * g);
+    const int pair = info.x, parts = info.y;
     GDN_BSTAMP(10);
     if (parts == 0) return;
     const TreeAttnArgs& a = p.a;
-    const int pair = p.info[2 * g], rt = pair % p.row_tiles, kvh = pair / p.row_tiles % a.KV, b = pair / p.row_tiles / a.KV;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = tid & (TM_ROWS - 1), row = blockIdx.y * TM_ROWS + r, cg = tid / TM_ROWS;
     const bool in = row < p.rows;
     auto slot = [&](int k) -> size_t { return k == 0 ? 2 * g + 1 : 2 * (g + k); };
+    // (requested at once: the rows' (m, l), the first partials and the tree; a dependent round trip to L2 costs most of a microsecond)
+    const float4* part = reinterpret_cast<const float4*>(p.part) + (size_t)cg * p.rows + row;
+    const size_t step = (size_t)64 * p.rows;                         // float4s of a slot
+    float4 o[TM_AHEAD];
+#pragma unroll
+    for (int k = 0; k < TM_AHEAD; k++)
+        if (in && k < parts) o[k] = __ldcg(part + slot(k) * step);
     for (int k = cg; k < parts; k += TM_THREADS / TM_ROWS) {
-        const float2 ml = in ? *reinterpret_cast<const float2*>(p.part_ml + (slot(k) * p.rows + row) * 2) : make_float2(-INFINITY, 0.f);
+        const float2 ml = in ? __ldcg(reinterpret_cast<const float2*>(p.part_ml + (slot(k) * p.rows + row) * 2)) : make_float2(-INFINITY, 0.f);
         s_w[k][r] = ml.x;
         s_l[k][r] = ml.y;
     }
+    const int rt = pair % p.row_tiles, kvh = pair / p.row_tiles % a.KV, b = pair / p.row_tiles / a.KV;
     if (warp == TM_ROWS) {                                           // which of the rows belong to nodes in use
         unsigned long long l0, l1;
         bool bad;
@@ -679,15 +712,15 @@ __global__ void __launch_bounds__(TM_THREADS) tree_attn_merge_kernel(const __gri
     __syncthreads();
     const int node = rt * p.nodes + row / p.group;
     if (!in || node >= a.N) return;
-    const float4* part = reinterpret_cast<const float4*>(p.part) + (size_t)cg * p.rows + row;
-    const size_t step = (size_t)64 * p.rows;                         // float4s of a slot
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float w, float4 x) {
+        acc.x = fmaf(w, x.x, acc.x); acc.y = fmaf(w, x.y, acc.y); acc.z = fmaf(w, x.z, acc.z); acc.w = fmaf(w, x.w, acc.w);
+    };
+#pragma unroll
+    for (int k = 0; k < TM_AHEAD; k++)
+        if (k < parts) add(s_w[k][r], o[k]);
 #pragma unroll 4
-    for (int k = 0; k < parts; k++) {
-        const float w = s_w[k][r];
-        const float4 o = __ldcg(part + slot(k) * step);
-        acc.x = fmaf(w, o.x, acc.x); acc.y = fmaf(w, o.y, acc.y); acc.z = fmaf(w, o.z, acc.z); acc.w = fmaf(w, o.w, acc.w);
-    }
+    for (int k = TM_AHEAD; k < parts; k++) add(s_w[k][r], __ldcg(part + slot(k) * step));
     const uint2 v = s_live[r] ? make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w)) : make_uint2(0, 0);
     *reinterpret_cast<uint2*>(a.out + (((size_t)b * a.N + node) * a.H + kvh * p.group + row % p.group) * ATT_D + 4 * cg) = v;
     GDN_BSTAMP(11);
