@@ -104,7 +104,17 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
         const __nv_bfloat16* line = a.proj + ((size_t)b * N + k / 6) * a.row_stride + (k % 6 >> 1) * KD + h * DK + (k & 1) * 64;
         asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
     }
+    // everything that only needs the block's own numbers, in one round of loads
     const int slot = a.slots[b], pos = a.pos[b];
+    const int par = tid < N ? a.parents[(size_t)b * N + tid] : -2;
+    float lg = 0.f, beta = 0.f;
+    if (tid < N) {
+        const __nv_bfloat16* row = a.proj + ((size_t)b * N + tid) * a.row_stride;
+        const __nv_bfloat16 rb = row[CD + KD + h], ra = row[CD + KD + HV + h];
+        const float A_log = a.A_log[h], dt_bias = a.dt_bias[h];
+        beta = sigmoid_f(__bfloat162float(rb));
+        lg = log_decay_f(A_log, __bfloat162float(ra) + dt_bias) * LOG2E;
+    }
     if (slot < 0 || slot >= a.n_slots || pos < 0) {                  // rows of a bad sequence: zeros
         if (tid == 0) atomicExch(a.status, 1);
         for (int i = tid; i < N * DV; i += TV_THREADS) a.y[((size_t)b * N + i / DV) * KD + h * DV + i % DV] = __float2bfloat16_rn(0.f);
@@ -122,37 +132,32 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
         load_state(0);
     }
     if (warp == 7) { tmem_alloc(smem_addr(&s_tmem), 256); tmem_relinquish(); }
-    if (tid < NP) s_par[tid] = tid < N ? a.parents[(size_t)b * N + tid] : -2;
-    float lg = 0.f, beta = 0.f;
-    if (tid < N) {
-        const __nv_bfloat16* row = a.proj + ((size_t)b * N + tid) * a.row_stride;
-        beta = sigmoid_f(ldbf(row + CD + KD + h));
-        lg = log_decay_f(a.A_log[h], ldbf(row + CD + KD + HV + h) + a.dt_bias[h]) * LOG2E;
-    }
+    if (tid < NP) { s_par[tid] = par; s_lg[tid] = lg; }
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tb = s_tmem;
     if (tid < NP) {
         bool bad = false;
-        s_line[tid] = tid < N ? tree_line(s_par, tid, bad) : 0;
+        const unsigned long long line = tid < N ? tree_line(s_par, tid, bad) : 0;
         if (bad) atomicExch(a.status, 1);
-        s_lg[tid] = lg; s_beta[tid] = beta;
+        float g = 0.f;
+        for (unsigned long long m = line; m; m &= m - 1) g += s_lg[__ffsll((long long)m) - 1];
+        s_line[tid] = line;
+        s_beta[tid] = beta;
+        s_G[tid] = g;
+        s_grow[tid] = line ? exp2f(g) : 0.f;
+        s_bgrow[tid] = line ? beta * exp2f(g) : 0.f;
+        if (line && !(isfinite(g) && isfinite(beta))) s_odd = 1;
+    } else if (tid < 2 * NP) {                                       // (two threads a node: the one above and this one)
+        const int i = tid - NP;
         const __nv_bfloat16* window = a.conv_pool + ((size_t)slot * 2 + (pos & 1)) * 3 * CD;
-        for (int t = 3, e = 3 + tid; t >= 0; t--) {                  // e: 0..2 the window, 3 + j node j
-            s_row[tid][t] = tid >= N ? window : e >= 3 ? a.proj + ((size_t)b * N + e - 3) * a.row_stride : window + (size_t)e * CD;
+        for (int t = 3, e = 3 + i; t >= 0; t--) {                    // e: 0..2 the window, 3 + j node j
+            s_row[i][t] = i >= N ? window : e >= 3 ? a.proj + ((size_t)b * N + e - 3) * a.row_stride : window + (size_t)e * CD;
             e = e >= 3 ? (s_par[e - 3] >= 0 && s_par[e - 3] < e - 3 ? 3 + s_par[e - 3] : 2) : e - 1;
         }
     }
     __syncthreads();
-    if (tid < NP) {
-        float g = 0.f;
-        for (unsigned long long m = s_line[tid]; m; m &= m - 1) g += s_lg[__ffsll((long long)m) - 1];
-        s_G[tid] = g;
-        s_grow[tid] = s_line[tid] ? exp2f(g) : 0.f;
-        s_bgrow[tid] = s_line[tid] ? beta * exp2f(g) : 0.f;
-        if (s_line[tid] && !(isfinite(g) && isfinite(beta))) s_odd = 1;
-    }
     GDN_BSTAMP(1);
     if (warp >= 8 - NP / 16) {                                       // the lists, one block of nodes per warp
         const int I = warp - (8 - NP / 16);
@@ -182,9 +187,8 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
 #pragma unroll
             for (int k = 0; k < 4; k++) { w[g][k][0] = pack2(f[0][k], f[1][k]); w[g][k][1] = pack2(f[2][k], f[3][k]); }
         }
-#pragma unroll 1
-        for (int i0 = warp; i0 < NP; i0 += 16) {
-            uint2 raw[2][GROUPS][4];
+        uint2 raw[2][GROUPS][4];
+        auto fetch = [&](int i0) {
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll
@@ -193,20 +197,31 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
 #pragma unroll
                     for (int g = 0; g < GROUPS; g++) raw[n][g][k] = *reinterpret_cast<const uint2*>(row + (G0 + g) * KD);
                 }
+        };
+        fetch(warp);
+#pragma unroll 1
+        for (int i0 = warp; i0 < NP; i0 += 16) {
+            f32x2 sum[2][GROUPS][2];
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int g = 0; g < GROUPS; g++) {
+                    sum[n][g][0] = sum[n][g][1] = 0;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint2 r = raw[n][g][k];
+                        fma2(sum[n][g][0], pack2(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u)), w[g][k][0]);
+                        fma2(sum[n][g][1], pack2(__uint_as_float(r.y << 16), __uint_as_float(r.y & 0xffff0000u)), w[g][k][1]);
+                    }
+                }
+            if (i0 + 16 < NP) fetch(i0 + 16);                        // (arrive during what follows)
             float x[2][GROUPS][4], ss[2 * GROUPS];
 #pragma unroll
             for (int n = 0; n < 2; n++) {
                 const bool on = s_line[i0 + 8 * n] != 0;
 #pragma unroll
                 for (int g = 0; g < GROUPS; g++) {
-                    f32x2 s0 = 0, s1 = 0;
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint2 r = raw[n][g][k];
-                        fma2(s0, pack2(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u)), w[g][k][0]);
-                        fma2(s1, pack2(__uint_as_float(r.y << 16), __uint_as_float(r.y & 0xffff0000u)), w[g][k][1]);
-                    }
-                    const float2 a0 = unpack2(s0), a1 = unpack2(s1);
+                    const float2 a0 = unpack2(sum[n][g][0]), a1 = unpack2(sum[n][g][1]);
                     float (&y)[4] = x[n][g];
                     y[0] = on ? silu_fast(a0.x) : 0.f; y[1] = on ? silu_fast(a0.y) : 0.f;
                     y[2] = on ? silu_fast(a1.x) : 0.f; y[3] = on ? silu_fast(a1.y) : 0.f;
