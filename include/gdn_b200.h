@@ -252,6 +252,7 @@ GDN_API int gdn_hrec(void* hist, const void* rows, const int* slots, const int* 
  * ancestors; its k / v row is appended at position ctx_len[b] + i (rows of unused nodes are not written; their out rows are zero).
  *   q, out bf16 [B*N, H, 256];  k_new, v_new bf16 [B*N, KV, 256];  H % KV == 0, H / KV <= 16
  *   k_pages, v_pages bf16 [n_pages, KV, page_size, 256];  block_table int32 [B, max_pages];  ctx_len int32 [B]
+ *   max_pages * page_size < 2^31 - 4096, and the tiles of 128 keys of at most 256 sequences times KV times row tiles below 2^31 (GDN_E_UNSUPPORTED)
  *   workspace: at least gqa_tree_attn_workspace_bytes(B, N, H, KV) bytes, 16-byte aligned, contents need no initialisation, not shared by
  *   calls that overlap on the GPU
  *   A sequence whose ctx_len is negative, or whose last used node does not fit max_pages * page_size, is skipped (out rows zero,
@@ -275,8 +276,9 @@ GDN_API int gdn_tree_accept(const int* parents, const int* toks, const int* ids,
 
 /* Advances recurrent state and conv window of n_layers layers along a path through each sequence's tree: state and window of slot
  * slots[b] (window buffer pos[b] & 1) after the tokens path[b][0 .. n_path[b]-1] go to slot dst_slots[b] (window buffer
- * (pos[b] + n_path[b]) & 1); dst_slots may equal slots.  A sequence with a bad index or path entry is skipped (status 1).  No
- * dst_slots[b] may be a slot that another sequence of the call reads or writes with n_path > 0 (the result would depend on the order).
+ * (pos[b] + n_path[b]) & 1); dst_slots may equal slots.  A sequence with a bad index or path entry is skipped (status 1), and
+ * so are sequences of which one writes a slot that another reads or writes (the result would depend on the order), the pools' last slot
+ * excepted: padding goes there, and its content is unspecified.  n_path[b] = 0 with dst_slots[b] = slots[b] touches nothing.
  *   The `_host` arrays hold one device pointer per layer: proj bf16 [B*N, row_stride], conv_pool, conv_w, A_log, dt_bias, ssm_pool as for
  *   gdn_deltanet_b.   path int32 [B, E]: nodes of the tree, 0 <= path < N */
 GDN_API int gdn_tree_commit(const void* const* proj_host, long long row_stride, void* const* conv_pool_host, const void* const* conv_w_host,

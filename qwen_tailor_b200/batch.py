@@ -132,7 +132,7 @@ def attn_tree(q, k_new, v_new, k_pages, v_pages, block_table, ctx_len, parents, 
     lib = _lib.load()
     with on_device(dev):
         size = lib.gqa_tree_attn_workspace_bytes(B, N, H, KV)
-        ws = torch.empty((size,), dtype=torch.uint8, device=dev)
+        ws = q.new_empty((size,), dtype=torch.uint8)
         check(lib.gqa_tree_attn(q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), ctx_len.data_ptr(),
                                 parents.data_ptr(), out.data_ptr(), ws.data_ptr(), size, B, N, H, KV, page_size, block_table.shape[1], n_pages, raw_stream(dev)), "attn_tree")
     return out
@@ -257,6 +257,8 @@ def compact_rows(pools: Sequence[torch.Tensor], block_table, base, keep, n_keep,
                          f"keep {tuple(keep.shape)}, n_keep {tuple(n_keep.shape)}")
     if block_table.shape[1] == 0:
         raise ValueError("compact_rows: an empty block table")
+    if len(set(ptrs)) < len(ptrs):
+        raise ValueError("compact_rows: a pool is named twice (its rows would move twice)")
     n_pages, heads, page_size, dim = shape
     with on_device(dev):
         check(_lib.load().gdn_rows_compact(_address(ptrs), len(ptrs), n_pages, heads, page_size, dim * first.element_size(), block_table.data_ptr(), dst_table.data_ptr(),

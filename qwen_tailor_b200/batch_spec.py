@@ -64,7 +64,7 @@ def accept_tree(parents, toks, ids):
     if not 1 <= N <= 64:
         raise ValueError(f"accept_tree: 1 <= N <= 64 nodes, got {N}")
     path = torch.empty_like(parents)
-    n_path = torch.empty((B,), dtype=torch.int32, device=dev)
+    n_path = parents.new_empty((B,))
     with on_device(dev):
         check(_lib.load().gdn_tree_accept(parents.data_ptr(), toks.data_ptr(), ids.data_ptr(), path.data_ptr(), n_path.data_ptr(), B, N, raw_stream(dev)), "accept_tree")
     return n_path, path
@@ -89,7 +89,7 @@ def deltanet_tree(proj, conv_pool, conv_w, A_log, dt_bias, ssm_pool, slots, pos,
     if not 1 <= N <= 64 or proj.shape[0] != B * N or stride % 4:
         raise ValueError(f"deltanet_tree: 1 <= N <= 64 nodes and proj [B*N, 8224] with a row stride that is a multiple of 4 expected (B={B}, N={N}, proj {tuple(proj.shape)}, stride {stride})")
     if out is None:
-        out = torch.empty((B * N, HV * DV), dtype=torch.bfloat16, device=dev)
+        out = ssm_pool.new_empty((B * N, HV * DV), dtype=torch.bfloat16)
     elif out.dtype != torch.bfloat16 or not out.is_contiguous() or tuple(out.shape) != (B * N, HV * DV):
         raise ValueError("deltanet_tree: out must be contiguous bf16 [B*N, 2048]")
     cw = conv_w if conv_w.dtype == torch.bfloat16 and conv_w.is_contiguous() else conv_w.to(torch.bfloat16).contiguous()
@@ -149,7 +149,9 @@ def deltanet_commit(projs, conv_pools, conv_ws, A_logs, dt_biases, ssm_pools, sl
     projs [B*N, 8224] bf16 (what ``deltanet_tree`` was called with), conv_pools / ssm_pools (slot pools), conv_ws bf16, A_logs and
     dt_biases fp32.  slots, pos int32 [B]; path int32 [B, E], n_path int32 [B] from ``accept_tree`` (E may be smaller than N if no path is
     longer).  The state after the path goes to slot dst_slots[b] (default: in place), the window to its buffer (pos + n_path) & 1.
-    No destination may be another sequence's slot in the same call.  n_path = 0 leaves a slot as it is (or copies it to its destination)."""
+    n_path = 0 leaves a slot as it is (or copies it to its destination).  A sequence with a bad index is skipped, and so are sequences of
+    which one writes a slot that another reads or writes; ``_lib.device_status()`` reports it.  The pools' last slot is exempt: it takes the
+    padding of a batch, and what it holds afterwards is unspecified."""
     who, L = "deltanet_commit", len(ssm_pools)
     if L == 0:
         raise ValueError(f"{who}: no layers")
@@ -175,6 +177,8 @@ def deltanet_commit(projs, conv_pools, conv_ws, A_logs, dt_biases, ssm_pools, sl
     N = row[0] // B if B else 1
     if B and (N < 1 or row[0] != B * N):
         raise ValueError(f"{who}: proj has {row[0]} rows for {B} sequences")
+    if L > 1 and len(set(ptrs[5 * L:])) < L:
+        raise ValueError(f"{who}: one ssm pool for two layers")
     base = ptrs.buffer_info()[0]
     at = [base + 8 * L * i for i in range(6)]
     with on_device(dev):

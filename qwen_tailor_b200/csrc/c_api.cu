@@ -364,6 +364,10 @@ int gqa_tree_attn(const void* q, const void* k_new, const void* v_new, void* k_p
     if (rc) return rc;
     REQUIRE(H > 0 && KV > 0 && H % KV == 0 && H / KV <= 16, GDN_E_SHAPE, "gqa_tree_attn: H=%d KV=%d (H a multiple of KV, at most 16 query heads on one)", H, KV);
     REQUIRE(page_size > 0 && max_pages > 0 && n_pages > 0, GDN_E_SHAPE, "gqa_tree_attn: page_size=%d max_pages=%d n_pages=%d", page_size, max_pages, n_pages);
+    // positions and the plan's tile numbers are 32-bit
+    const long long cap = (long long)max_pages * page_size, most = tree_attn_plan_tiles(B, N, H, KV, cap);
+    REQUIRE(cap <= 0x7fffffffll - 4096 && most <= 0x7fffffffll, GDN_E_UNSUPPORTED, "gqa_tree_attn: block_table of %d x %d rows is too long for %d sequences (%lld tiles)",
+            max_pages, page_size, B, most);
     if (B == 0) return GDN_OK;
     REQUIRE(q && k_new && v_new && k_pages && v_pages && block_table && ctx_len && out && workspace, GDN_E_NULL, "gqa_tree_attn: null pointer");
     REQUIRE(aligned16(q) && aligned16(k_new) && aligned16(v_new) && aligned16(k_pages) && aligned16(v_pages) && aligned16(out) && aligned16(workspace),
@@ -449,15 +453,13 @@ int gdn_rows_compact(void* const* pools_host, int n_pools, int n_pages, int head
     REQUIRE((long long)B * heads < (1ll << 31), GDN_E_SHAPE, "gdn_rows_compact: B=%d heads=%d", B, heads);
     if (n_pools == 0 || B == 0 || L == 0) return GDN_OK;
     REQUIRE(pools_host && block_table && dst_table && base && keep && n_keep, GDN_E_NULL, "gdn_rows_compact: null pointer");
+    for (int p = 0; p < n_pools; p++) REQUIRE(pools_host[p] && (uintptr_t)pools_host[p] % 2 == 0, GDN_E_NULL, "gdn_rows_compact: null or odd pool %d", p);
     int* status = status_ptr();
     REQUIRE(status, GDN_E_LAUNCH, "gdn_rows_compact: no CUDA device");
     for (int p0 = 0; p0 < n_pools; p0 += RC_MAX_POOLS) {
         RowsArgs a{};
         const int cnt = n_pools - p0 < RC_MAX_POOLS ? n_pools - p0 : RC_MAX_POOLS;
-        for (int p = 0; p < cnt; p++) {
-            REQUIRE(pools_host[p0 + p] && (uintptr_t)pools_host[p0 + p] % 2 == 0, GDN_E_NULL, "gdn_rows_compact: null or odd pool %d", p0 + p);
-            a.pool[p] = pools_host[p0 + p];
-        }
+        for (int p = 0; p < cnt; p++) a.pool[p] = pools_host[p0 + p];
         a.table = block_table; a.dst_table = dst_table; a.base = base; a.keep = keep; a.n_keep = n_keep; a.status = status;
         a.row_bytes = row_bytes; a.B = B; a.L = L; a.heads = heads; a.page_size = page_size; a.max_pages = max_pages; a.n_pages = n_pages;
         const int rc = launch_rows_compact(a, cnt, static_cast<cudaStream_t>(stream));

@@ -183,6 +183,7 @@ struct TreeAttnArgs {
     int B, N, H, KV, page_size, max_pages, n_pages;
 };
 size_t tree_attn_workspace_bytes(int B, int N, int H, int KV);
+long long tree_attn_plan_tiles(int B, int N, int H, int KV, long long cap);
 int launch_tree_attn(const TreeAttnArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t st);
 
 }  // namespace gdn

@@ -756,6 +756,13 @@ size_t tree_attn_workspace_bytes(int B, int N, int H, int KV) {
     return G * 16 + 2 * G * p.rows * (ATT_D + 2) * sizeof(float);
 }
 
+// tiles of the longest plan a launch can meet, for contexts up to `cap` rows
+long long tree_attn_plan_tiles(int B, int N, int H, int KV, long long cap) {
+    TreeAttnPlan p{};
+    tree_shape(p, N, H, KV);
+    return (long long)(B < TA_MAX_B ? B : TA_MAX_B) * KV * p.row_tiles * ((cap + TA_TK - 1) / TA_TK + 1 + TA_TAIL);
+}
+
 typedef CUresult (*TreeEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 

@@ -50,13 +50,16 @@ __device__ __forceinline__ unsigned long long tree_line(const int* par, int i, b
 // for its value row in blocks of 16 nodes, thread d of the other four follows with y_i = e^G_i P2_i + sum_j A_ij u_j.  L and A are
 // dense with zeros outside the ancestors; zeros do not stop NaN, so a head with a non-finite q, k, v or gate takes the sums over the
 // ancestors one by one instead.
+// M_ij is 2 to the difference of two sums G, which can be far larger than their difference (a path through tokens that wipe the state out).
+// G is summed in 64 bits and split into hi = fp32(G) and lo; with u'_i = 2^-lo_i u_i in place of u the solve needs 2^(hi_i - hi_j) only, and
+// lo enters factors of single nodes: beta_i 2^-lo_i on v, 2^lo_i on A's row.
 // Shared memory: [K; Q] hi and lo (1 KiB a node), later L and A; a region that receives the state (two halves of 32 KiB where
 // NP = 64, so that two blocks fit an SM) and then holds v and u.
 // ----------------------------------------------------------------------------------------------------------------------
 using namespace sm100;
 
 constexpr int TV_THREADS = 256;
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOG2E = 1.4426950408889634f, TV_WIPED = -160.f;      // 2^-160 is below the smallest fp32 number
 template <int NP> struct TreeVerify {
     static constexpr int HALVES = NP == 64 ? 2 : 1;                  // pieces the state arrives in
     static constexpr int SLAB = 2 * NP * 128;                        // bytes of 64 dims of [K; Q]
@@ -88,7 +91,8 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
     __shared__ int s_par[NP];
     __shared__ __align__(16) const __nv_bfloat16* s_row[NP][4];      // conv rows of a node: t-3 .. t along its path
     __shared__ float s_lg[NP], s_beta[NP];
-    __shared__ __align__(16) float s_G[NP], s_grow[NP], s_bgrow[NP];  // G (log2), e^G, beta e^G
+    __shared__ __align__(16) float s_G[NP], s_grow[NP], s_bgrow[NP];  // G (log2), rounded to fp32; e^G; beta 2^(G rounded)
+    __shared__ float s_up[NP], s_bdown[NP];                          // with lo = what the rounding of G dropped: 2^lo; beta 2^-lo
     __shared__ __align__(4) unsigned char s_list[NP / 16][NP];       // per block of 16 nodes: their ancestors in earlier blocks,
     __shared__ int s_cnt[NP / 16];                                   // in fours (filled up with NP, the row of zeros)
     __shared__ uint32_t s_tmem;
@@ -114,6 +118,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
         const float A_log = a.A_log[h], dt_bias = a.dt_bias[h];
         beta = sigmoid_f(__bfloat162float(rb));
         lg = log_decay_f(A_log, __bfloat162float(ra) + dt_bias) * LOG2E;
+        if (lg < TV_WIPED) lg = TV_WIPED;                            // (the decay is zero in fp32 either way; sums stay in range; NaN passes)
     }
     if (slot < 0 || slot >= a.n_slots || pos < 0) {                  // rows of a bad sequence: zeros
         if (tid == 0) atomicExch(a.status, 1);
@@ -141,13 +146,17 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
         bool bad = false;
         const unsigned long long line = tid < N ? tree_line(s_par, tid, bad) : 0;
         if (bad) atomicExch(a.status, 1);
-        float g = 0.f;
-        for (unsigned long long m = line; m; m &= m - 1) g += s_lg[__ffsll((long long)m) - 1];
+        double sum = 0.;
+        for (unsigned long long m = line; m; m &= m - 1) sum += s_lg[__ffsll((long long)m) - 1];
+        const float g = (float)sum;
         s_line[tid] = line;
         s_beta[tid] = beta;
+        const float lo = (float)(sum - g), up = exp2f(lo), e = exp2f(g);
         s_G[tid] = g;
-        s_grow[tid] = line ? exp2f(g) : 0.f;
-        s_bgrow[tid] = line ? beta * exp2f(g) : 0.f;
+        s_up[tid] = up;
+        s_bdown[tid] = line ? __fdividef(beta, up) : 0.f;
+        s_grow[tid] = line ? e * up : 0.f;
+        s_bgrow[tid] = line ? beta * e : 0.f;
         if (line && !(isfinite(g) && isfinite(beta))) s_odd = 1;
     } else if (tid < 2 * NP) {                                       // (two threads a node: the one above and this one)
         const int i = tid - NP;
@@ -317,7 +326,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
     GDN_BSTAMP(4);
     float* su = reinterpret_cast<float*>(smem + C::KQ_BYTES);        // [NP][128]: v, then u
     front(std::integral_constant<int, 2>(), std::integral_constant<int, 1>(), [&](int, int i, const float (&x)[4]) {
-        const float m = s_line[i] ? s_beta[i] : 0.f;
+        const float m = s_bdown[i];
         *reinterpret_cast<float4*>(su + i * DV + 4 * lane) = s_line[i] ? make_float4(m * x[0], m * x[1], m * x[2], m * x[3]) : make_float4(0.f, 0.f, 0.f, 0.f);
     });
     if (tid < DV) su[NP * DV + tid] = 0.f;
@@ -332,7 +341,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
         const bool isq = d >= NP;
         const int i = isq ? d - NP : d;
         const unsigned long long line = isq ? s_line[i] : s_line[i] & ~(1ull << i);
-        const float g = s_G[i], mul = isq ? 1.f : s_beta[i];
+        const float g = s_G[i], mul = isq ? s_up[i] : s_beta[i];
         float* dst = (isq ? sA : sL) + i;
         for (int j0 = (warp >> 2) * 16; j0 < NP; j0 += 32) {
             uint32_t r[16];
@@ -448,8 +457,8 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
 #pragma unroll
                 for (int k = 0; k < 16; k++) if (k == c) { p1 = __uint_as_float(r1[k]); p2 = __uint_as_float(r2[k]); }
                 const unsigned long long line = s_line[i];
-                const float grow = exp2f(s_G[i]);
-                float u = su[i * DV + d] - s_beta[i] * grow * p1, y = grow * p2;
+                const float grow = s_grow[i];
+                float u = su[i * DV + d] - s_bgrow[i] * p1, y = grow * p2;
                 for (unsigned long long m = line & ~(1ull << i); m; m &= m - 1) {
                     const int j = __ffsll((long long)m) - 1;
                     u = fmaf(-sL[j * NP + i], su[j * DV + d], u);
@@ -588,12 +597,21 @@ __global__ void __launch_bounds__(CM_THREADS, 2) tree_commit_kernel(const __grid
     const int* path = a.path + (size_t)b * a.E;
     const int first = tid < CM_PATH && tid < a.E ? path[tid] : 0;
     const int slot = a.slots[b], dst = a.dst_slots[b], pos = a.pos[b], n = a.n_path[b];
+    const int o0 = min(tid, a.B - 1), so0 = a.slots[o0], to0 = a.dst_slots[o0], no0 = a.n_path[o0];
     const uint2 taps = *reinterpret_cast<const uint2*>(a.conv_w[layer] + (size_t)ch * 4);
     const float A_log = a.A_log[layer][h], dt_bias = a.dt_bias[layer][h];
     bool bad = slot < 0 || slot >= a.n_slots || dst < 0 || dst >= a.n_slots || pos < 0 || n < 0 || n > a.E;
     if (!bad && n == 0 && slot == dst) return;
     if (tid < CM_PATH) s_path[tid] = first;
     bad = bad || (tid < n && tid < CM_PATH && (first < 0 || first >= a.N));
+    // another sequence that writes what this one reads or writes, or reads what it writes, would make the result a matter of order: both
+    // are refused (the pools' last slot takes the padding of a batch and is nobody's)
+    auto clash = [&](int o, int so, int to, int no) -> bool {
+        const int last = a.n_slots - 1;
+        return o != b && (so != to || no != 0) && ((to == slot && slot != last) || ((to == dst || so == dst) && dst != last));
+    };
+    bad = bad || clash(o0, so0, to0, no0);
+    for (int o = tid + CM_THREADS; o < a.B; o += CM_THREADS) bad = bad || clash(o, a.slots[o], a.dst_slots[o], a.n_path[o]);
     if (!bad)
         for (int j = CM_PATH + tid; j < n; j += CM_THREADS) bad = bad || path[j] < 0 || path[j] >= a.N;
     if (__syncthreads_or(bad)) { if (tid == 0) atomicExch(a.status, 1); return; }

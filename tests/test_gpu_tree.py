@@ -325,6 +325,28 @@ def test_deltanet_tree_malformed_trees_slots_and_masked_nans(dev):
     assert run_delta({**d, "slots": d["slots"][:0], "pos": d["pos"][:0]}, i32_dev(parents[:0], dev), d["proj"][0][:0]).shape == (0, 2048)
 
 
+@pytest.mark.parametrize("N", [12, 64])
+def test_deltanet_tree_with_decays_from_none_to_all(dev, N):
+    """Tokens that keep the state, that halve it and that wipe it out, mixed along every path: what lies between two nodes of a path counts, not
+    the sum from its root (which leaves the range in which fp32 tells a difference of 0.01 apart)."""
+    rng = np.random.default_rng(N)
+    c = delta_case(rng, 2, N, 3)
+    c["dt_bias"][:] = 0
+    c["A_log"][:] = 0
+    a = rng.choice([-6.0, -1.0, 20.0, 100.0, 30000.0], (2 * N, 16), p=[0.4, 0.3, 0.1, 0.1, 0.1])      # decays e^-log(1 + e^a): 0.998, 0.73, 2e-9, 0, 0
+    c["proj"][0, :, 8208:8224] = a
+    parents = np.stack([random_tree(rng, N, kind=kind) for kind in ("chain", "random")])
+    d = delta_dev(c, dev)
+    y = host(run_delta(d, i32_dev(parents, dev)))
+    for b in range(2):
+        s, par = int(c["slots"][b]), int(c["pos"][b]) & 1
+        ref = tree.deltanet_tree(host(d["proj"])[0, b * N:(b + 1) * N], c["conv"][0, 2 * s + par], c["conv_w"][0], c["A_log"][0], c["dt_bias"][0], c["ssm"][0, s], parents[b])
+        got = y[b * N:(b + 1) * N]
+        scale = np.abs(ref).reshape(N, 16, 128).max((0, 2)).repeat(128)
+        assert (np.abs(got - ref) <= HALF * np.abs(ref) + DELTA_ABS * scale).all(), float((np.abs(got - ref) - HALF * np.abs(ref) - DELTA_ABS * scale).max())
+    assert _lib.device_status() == 0
+
+
 def test_deltanet_tree_of_a_chain_agrees_with_deltanet_bm(dev):
     rng = np.random.default_rng(32)
     c = delta_case(rng, 2, 4, 3)
@@ -393,6 +415,65 @@ def test_deltanet_commit_skips_what_is_out_of_range(dev):
         run({**d, "conv_w": d["conv_w"].float()}, path, n)
     with pytest.raises(ValueError):
         run({**d, "proj": d["proj"][:, :11]}, path, n)
+
+
+def test_deltanet_commit_refuses_slots_that_depend_on_order(dev):
+    rng = np.random.default_rng(42)
+    c = delta_case(rng, 4, 3, 10)
+    path, n = np.tile(np.arange(3, dtype=np.int32), (4, 1)), np.array([2, 1, 3, 2], np.int32)
+
+    def run(slots, dst, n):
+        d = delta_dev(c, dev)
+        deltanet_commit(d["proj"], d["conv"], d["conv_w"], d["A_log"], d["dt_bias"], d["ssm"], i32_dev(slots, dev), d["pos"], i32_dev(path, dev), i32_dev(n, dev),
+                        dst_slots=i32_dev(dst, dev))
+        return d, host(d["ssm"])[0], _lib.device_status()
+    good, bad = [0, 1, 2, 3], 0
+    _, want, status = run(good, good, n)
+    assert status == 0
+    # (slots, destinations, sequences that are skipped)
+    for slots, dst, skipped in (([0, 1, 0, 3], [0, 1, 0, 3], [0, 2]), ([0, 1, 2, 3], [4, 1, 4, 3], [0, 2]), ([0, 1, 2, 3], [2, 1, 5, 3], [0, 2]),
+                                ([0, 1, 2, 3], [1, 2, 3, 0], [0, 1, 2, 3])):
+        _, ssm, status = run(slots, dst, n)
+        assert status == 1
+        for b in range(4):
+            if b in skipped:
+                assert np.array_equal(ssm[dst[b]], c["ssm"][0, dst[b]]), (slots, dst, b)
+            else:
+                assert np.array_equal(ssm[dst[b]], want[b])
+    # one slot read by many, untouched sequences, and padding in the last slot are all right
+    _, ssm, status = run([0, 1, 0, 3], [0 + 4, 1, 5, 3], n)
+    assert status == 0 and np.array_equal(ssm[4], want[0]) and np.array_equal(ssm[1], want[1])
+    _, ssm, status = run([0, 1, 1, 1], [0, 1, 1, 1], np.array([2, 1, 0, 0], np.int32))
+    assert status == 0 and np.array_equal(ssm[:2], want[:2])
+    _, ssm, status = run([0, 9, 9, 3], [0, 9, 9, 3], n)
+    assert status == 0 and np.array_equal(ssm[0], want[0]) and np.array_equal(ssm[3], want[3]) and np.array_equal(ssm[4:9], c["ssm"][0, 4:9])
+    d = delta_dev(c, dev)
+    with pytest.raises(ValueError, match="two layers"):
+        deltanet_commit(*[[d[k][0]] * 2 for k in ("proj", "conv", "conv_w", "A_log", "dt_bias", "ssm")], d["slots"], d["pos"], i32_dev(path, dev), i32_dev(n, dev))
+
+
+def test_more_sequences_than_a_block_has_threads(dev):
+    """300 sequences: commit's look at the others' slots, compaction and accept go past one block's threads; two of them clash."""
+    rng = np.random.default_rng(43)
+    B = 300
+    c = delta_case(rng, B, 1, B + 1)
+    slots = rng.permutation(B).astype(np.int32)
+    dup = slots.copy()
+    dup[299] = dup[3]
+    n = np.ones(B, np.int32)
+    states = []
+    for s in (slots, dup):
+        d = delta_dev(c, dev)
+        parents = torch.full((B, 1), -1, dtype=torch.int32, device=dev)
+        n_path, path = accept_tree(parents, torch.zeros_like(parents), torch.zeros_like(parents))
+        assert n_path.tolist() == n.tolist() and not path.any()
+        deltanet_commit(d["proj"], d["conv"], d["conv_w"], d["A_log"], d["dt_bias"], d["ssm"], i32_dev(s, dev), d["pos"], path, n_path)
+        states.append(host(d["ssm"])[0])
+        assert _lib.device_status() == (s is dup)
+    changed = np.array([(x != x0).any() for x, x0 in zip(states[0], c["ssm"][0])])
+    assert changed[:B].all() and not changed[B]
+    differs = np.array([(x != y).any() for x, y in zip(*states)])
+    assert sorted(np.flatnonzero(differs)) == sorted([int(slots[3]), int(slots[299])])
 
 
 # ---------------------------------------------------------------------------------------------------------------------

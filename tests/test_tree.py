@@ -65,6 +65,14 @@ def test_entry_points_refuse_before_any_launch():
     assert copy(lens=(ctypes.c_longlong * 2)(64, 66)) == -1
 
 
+def test_tree_attention_refuses_tables_beyond_32_bit_positions():
+    lib = _lib.load()
+    attn = lambda B, KV, page_size, max_pages, q=ONE: lib.gqa_tree_attn(q, ONE, ONE, ONE, ONE, ONE, ONE, ONE, ONE, ONE, 1 << 40, B, 64, 16 * KV, KV, page_size, max_pages, 1, None)  # noqa: E731
+    assert attn(1, 1, 1 << 20, 2048) == -7 and b"too long" in lib.gdn_last_error_string()      # 2^31 rows: positions
+    assert attn(256, 8, 1 << 14, 1 << 10) == -7                      # 2^24 rows: 256 sequences x 8 heads x 8 row tiles x 2^17 key tiles
+    assert attn(256, 8, 1 << 14, 1 << 9, q=None) == -8 and attn(1, 1, 1 << 14, 1 << 16, q=None) == -8      # (accepted: the next check answers)
+
+
 def _pool(n_pages, page_size=8):
     return PagePool(2, n_pages, page_size, 2, 16, device="cpu")
 
