@@ -5,10 +5,13 @@
 // per KV head; a tree has up to 64 nodes x (H / KV) query heads, so here the rows fill the 128 of a tensor-core tile and a K / V tile is
 // read once for all of them.  Bound: HBM (2 KiB per key and pair of KV heads) up to about 128 rows per KV head, the tensor pipe beyond.
 //
-// Work: a (sequence, KV head, row tile) triple is a "pair"; its keys come in 128-key tiles, the last tile holding the nodes themselves
-// (from the call's k_new / v_new).  The tiles of all pairs laid end to end are cut into equal ranges, one per SM, so that one long
-// sequence occupies the whole GPU as well as many short ones; a pair that is cut leaves fp32 partials, which a second small kernel
-// joins (overlapping its launch with this kernel's end).  Every block derives the plan from ctx_len itself.
+// Work: a (sequence, KV head) is a "pair"; its keys come in 128-key tiles, the last tile holding the nodes themselves (from the call's
+// k_new / v_new).  The tiles of all pairs laid end to end are cut into equal ranges, one per SM, so that one long sequence occupies the
+// whole GPU as well as many short ones; a pair that is cut leaves fp32 partials, which a second small kernel joins (overlapping its
+// launch with this kernel's end).  Every block derives the plan from ctx_len itself.  More than 128 rows take several row tiles: the blocks
+// then form groups, one block per row tile, that walk the same range side by side, so that one of them brings a tile out of HBM and
+// the others find it in L2 (with the row tiles one after the other in the plan, 2 x 64 nodes over 64 k tokens read everything twice:
+// 112 us against 98).
 //
 // Roles: warps 0-3 softmax (one thread per query row; warps without rows sleep), warp 4 issues the MMAs, warps 5 and 6 are the TMA
 // producers of K and V, warp 7 appends the nodes' rows to the cache.  Per tile
@@ -41,7 +44,7 @@ constexpr int TA_SLOT = 16384, TA_NK = 5, TA_NV = 5;                  // K slab:
 constexpr int TA_Q_BYTES = 65536;                                     // 128 rows, or two buffers of up to 64 rows
 constexpr int TA_SMEM = TA_Q_BYTES + (TA_NK + TA_NV) * TA_SLOT;
 constexpr uint32_t TAM_O = 0, TAM_SP0 = 256;
-constexpr int TA_TAIL = 1;                                            // plan weight of a pair's epilogue, in tiles (about 3 us against 2.7)
+constexpr int TA_TAIL = 3;                                            // plan weight of a pair's end (its nodes and epilogue, 8 us) in tiles (2.6 us)
 constexpr float TA_RAISE = 8.f;                                       // log2 units
 enum {
     AB_QFULL = 0, AB_QEMPTY = 2, AB_KFULL = 4, AB_KEMPTY = AB_KFULL + TA_NK, AB_VFULL = AB_KEMPTY + TA_NK, AB_VEMPTY = AB_VFULL + TA_NV,
@@ -52,14 +55,16 @@ struct TreeAttnPlan {
     TreeAttnArgs a;
     float* part;                 // [2 * G][64 column groups][rows][4]: partial O; then [2 * G][rows][2]: (m, l)
     float* part_ml;
-    int* info;                   // [G][2]: the pair that starts in block g and goes on in the next ones, and its number of partials (0: none)
+    int* info;                   // a cut pair's first block, the pair and its number of partials (0: not cut), in the order the merge kernel's
+                                 // grid has: by pair where there are at most G pairs (`by_pair`), by first block otherwise
+    bool by_pair;
     int G;                       // blocks
     int group, nodes, rows;      // query heads per KV head, nodes per row tile, rows per tile
     int row_tiles, q_bufs, q_slab;       // row tiles per (sequence, KV head); Q buffers; bytes of a Q slab (64 dims of all rows)
     int k_box, v_box;            // keys per copy
 };
 
-struct TreeSeg { int b, kvh, rt, t0, n, span, tiles, ctx; };          // tiles [t0, t0 + n) of a pair with `tiles` of them; span: of the plan
+struct TreeSeg { int b, kvh, t0, n, span, tiles, ctx; };          // tiles [t0, t0 + n) of a pair with `tiles` of them; span: of the plan
 
 // {i, ancestors} of nodes lane and lane + 32 of one tree, as bit masks (0 = unused); par0 / par1: their parents (-2 beyond N)
 __device__ __noinline__ void warp_lines(int par0, int par1, unsigned long long& l0, unsigned long long& l1, bool& bad) {
@@ -140,7 +145,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
     GDN_BSTAMP(0);
     // ---- plan ----
     const long long cap = (long long)a.max_pages * a.page_size;
-    const int PP = a.KV * p.row_tiles;
+    const int rt = blockIdx.x % p.row_tiles, grp = blockIdx.x / p.row_tiles;      // row tile and group of this block
     // context of sequence b as the kernel uses it, -1 = skipped (negative, or the nodes do not fit the table)
     auto context = [&](int b) -> int {
         const int ctx = a.ctx_len[b];
@@ -163,7 +168,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                 const int ctx = context(b);
                 if (ctx < 0 && blockIdx.x == 0) atomicExch(a.status, 1);
                 s_ctx[b] = ctx;
-                x = ((max(ctx, 0) + TA_TK - 1) / TA_TK + 1 + TA_TAIL) * PP;
+                x = ((max(ctx, 0) + TA_TK - 1) / TA_TK + 1 + TA_TAIL) * a.KV;
             }
             const int own = x;
 #pragma unroll
@@ -189,8 +194,8 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
     const uint32_t tb = tmem_slot;
     GDN_BSTAMP(1);
     const int N_all = s_cum[a.B];
-    const int G = min((int)gridDim.x, N_all);
-    const int lo = (int)blockIdx.x < G ? range_lo(blockIdx.x, G, N_all) : 0, hi = (int)blockIdx.x < G ? range_lo(blockIdx.x + 1, G, N_all) : 0;
+    const int G = min((int)gridDim.x / p.row_tiles, N_all);
+    const int lo = grp < G ? range_lo(grp, G, N_all) : 0, hi = grp < G ? range_lo(grp + 1, G, N_all) : 0;
 
     auto aborted = [&]() -> bool { return *(volatile int*)&s_abort != 0; };
     // bounded; a failure tells the whole block to stop computing
@@ -213,9 +218,9 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
         s.b = l;
         s.ctx = s_ctx[l];
         s.tiles = (max(s.ctx, 0) + TA_TK - 1) / TA_TK + 1;
-        const int off = x - s_cum[l], len = s.tiles + TA_TAIL, pr = off / len;
-        s.t0 = off - pr * len;
-        s.kvh = pr / p.row_tiles; s.rt = pr - s.kvh * p.row_tiles;
+        const int off = x - s_cum[l], len = s.tiles + TA_TAIL;
+        s.kvh = off / len;
+        s.t0 = off - s.kvh * len;
         s.span = min(len - s.t0, hi - x);
         s.n = min(s.tiles - s.t0, s.span);                           // (0 or less where the range starts in a pair's tail)
         return s;
@@ -224,7 +229,17 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
     // keys of tile t of a segment's pair (the last tile holds the nodes)
     auto limit_of = [&](const TreeSeg& s, int t) -> int { return t == s.tiles - 1 ? a.N : min(TA_TK, s.ctx - t * TA_TK); };
 
-    if (tid == 0) *reinterpret_cast<int2*>(p.info + 2 * blockIdx.x) = make_int2(0, 0);      // (no pair to join, as far as is known)
+    // nothing to join, as far as is known (every pair starts in exactly one block, and only that one writes its entry)
+    auto clear_info = [&]() {
+        if (!p.by_pair) { *reinterpret_cast<int2*>(p.info + 2 * blockIdx.x) = make_int2(0, 0); return; }
+#pragma unroll 1
+        for (int x = lo; x < hi;) {
+            const TreeSeg s = segment(x);
+            x += s.span;
+            if (s.t0 == 0) p.info[2 * ((s.b * a.KV + s.kvh) * p.row_tiles + rt) + 1] = 0;
+        }
+    };
+    if (tid == 0) clear_info();
     if (warp == 5 || warp == 6) {
         // ================= producers: warp 5 Q and K, warp 6 V =================
         // Lane i works out page and row of box i of a tile (a tile has at most 32 boxes where the page size is a multiple of 4); page
@@ -251,7 +266,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                 if (lane == 0) {
                     mbar_expect_tx(bar(AB_QFULL + qb), p.rows * 512);
                     for (int j = 0; j < 4; j++)
-                        tma_load_3d(sQ + qb * (TA_Q_BYTES / 2) + j * p.q_slab, &tmQ, bar(AB_QFULL + qb), 64 * j, s.kvh * p.group, s.b * a.N + s.rt * p.nodes);
+                        tma_load_3d(sQ + qb * (TA_Q_BYTES / 2) + j * p.q_slab, &tmQ, bar(AB_QFULL + qb), 64 * j, s.kvh * p.group, s.b * a.N + rt * p.nodes);
                 }
             }
             const int* table = a.block_table + (size_t)s.b * a.max_pages;
@@ -409,7 +424,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
         for (int x = lo; x < hi;) {
             const TreeSeg s = segment(x);
             x += s.span;
-            if (s.t0 != 0 || s.rt != 0 || s.ctx < 0) continue;
+            if (s.t0 != 0 || rt != 0 || s.ctx < 0) continue;
             const int* par = a.parents + (size_t)s.b * a.N;
             unsigned long long l0, l1;
             bool bad;
@@ -440,7 +455,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
             const TreeSeg s = segment(x);
             x += s.span;
             if (s.n <= 0) continue;
-            const int node = s.rt * p.nodes + local;
+            const int node = rt * p.nodes + local;
             const bool real = row < p.rows && node < a.N;
             const bool has_nodes = s.t0 + s.n == s.tiles;
             int par0 = -2, par1 = -2;                                // requested early, used at the last tile
@@ -550,20 +565,23 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                         const int slot = (nv + c) % TA_NV;
                         if (!warp_wait(AB_VFULL + slot, (nv + c) / TA_NV)) { ok = false; break; }
                         const int r0 = nodes ? 0 : limit & 31, r1 = nodes ? 32 : (r0 + 15) & ~15;
-#pragma unroll 1
+#pragma unroll 4
                         for (int i = row; i < (r1 - r0) * 32; i += n_warps * 32) {
                             const int r = r0 + (i >> 5), k = 32 * c + r, ch = i & 31;
                             uint4* at = reinterpret_cast<uint4*>(smem + TA_Q_BYTES + TA_NK * TA_SLOT + slot * TA_SLOT + (ch >> 3) * 4096 + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
                             if (!nodes || !(used >> k & 1)) { *at = make_uint4(0, 0, 0, 0); continue; }
                             const uint4 v = *at;
                             uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                            bool hit = false;
+                            // an exponent of ones in either half carries into the half's top bit
+                            const uint32_t E = 0x7f807f80u, one = 0x00800080u;
+                            if (!((((w[0] & E) + one) | ((w[1] & E) + one) | ((w[2] & E) + one) | ((w[3] & E) + one)) & 0x80008000u)) continue;
 #pragma unroll
                             for (int q = 0; q < 4; q++) {
-                                if (bf16_not_finite(w[q])) { w[q] &= 0xffff0000u; hit = true; }
-                                if (bf16_not_finite(w[q] >> 16)) { w[q] &= 0xffffu; hit = true; }
+                                if (bf16_not_finite(w[q])) w[q] &= 0xffff0000u;
+                                if (bf16_not_finite(w[q] >> 16)) w[q] &= 0xffffu;
                             }
-                            if (hit) { seen_bad |= 1ull << k; *at = make_uint4(w[0], w[1], w[2], w[3]); }
+                            seen_bad |= 1ull << k;
+                            *at = make_uint4(w[0], w[1], w[2], w[3]);
                         }
                     }
                     fence_proxy_async_smem();
@@ -641,37 +659,37 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                 // the pair that starts in this block and goes on in the next ones is joined by the merge kernel
                 int parts = 1;
 #pragma unroll 1
-                while (range_lo(blockIdx.x + parts, G, N_all) < hi - s.n + s.tiles) parts++;
-                *reinterpret_cast<int2*>(p.info + 2 * blockIdx.x) = make_int2((s.b * a.KV + s.kvh) * p.row_tiles + s.rt, parts);
+                while (range_lo(grp + parts, G, N_all) < hi - s.n + s.tiles) parts++;
+                const int pair = (s.b * a.KV + s.kvh) * p.row_tiles + rt;
+                *reinterpret_cast<int2*>(p.info + 2 * (p.by_pair ? pair : (int)blockIdx.x)) = make_int2(p.by_pair ? (int)blockIdx.x : pair, parts);
             }
             nseg++;
         }
     }
-    if (tid == 0 && aborted()) p.info[2 * blockIdx.x + 1] = 0;
+    if (tid == 0 && aborted()) clear_info();
     tc_fence_before_sync();
     __syncthreads();
     if (warp == 4) tmem_dealloc(tb, 512);
     GDN_BSTAMP(9);
 }
 
-// Joins the partials of the pair that starts in main block blockIdx.x and is cut: eight rows per block, a thread holds four columns of a row.
+// Joins the partials of a cut pair (blockIdx.x: the pair, or the main block that it starts in): eight rows per block, a thread holds four columns of a row.
 // Bound: latency (a few hundred KiB out of L2), so all a block needs is requested at once, six partials a thread.
-constexpr int TM_THREADS = 512, TM_ROWS = 8, TM_AHEAD = 6;
+constexpr int TM_ROWS = 8, TM_THREADS = 64 * TM_ROWS, TM_AHEAD = 6;
 
 __global__ void __launch_bounds__(TM_THREADS) tree_attn_merge_kernel(const __grid_constant__ TreeAttnPlan p) {
     __shared__ float s_w[148][TM_ROWS], s_l[148][TM_ROWS];
     __shared__ unsigned char s_live[TM_ROWS];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int g = blockIdx.x;
-    const int2 info = *reinterpret_cast<const int2*>(p.info + 2 * g);
-    const int pair = info.x, parts = info.y;
+    const int2 info = *reinterpret_cast<const int2*>(p.info + 2 * blockIdx.x);
+    const int first = p.by_pair ? info.x : blockIdx.x, pair = p.by_pair ? blockIdx.x : info.x, parts = info.y;
     GDN_BSTAMP(10);
     if (parts == 0) return;
     const TreeAttnArgs& a = p.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = tid & (TM_ROWS - 1), row = blockIdx.y * TM_ROWS + r, cg = tid / TM_ROWS;
     const bool in = row < p.rows;
-    auto slot = [&](int k) -> size_t { return k == 0 ? 2 * g + 1 : 2 * (g + k); };
+    auto slot = [&](int k) -> size_t { return 2 * (first + k * p.row_tiles) + (k == 0 ? 1 : 0); };
     // (requested at once: the rows' (m, l), the first partials and the tree; a dependent round trip to L2 costs most of a microsecond)
     const float4* part = reinterpret_cast<const float4*>(p.part) + (size_t)cg * p.rows + row;
     const size_t step = (size_t)64 * p.rows;                         // float4s of a slot
@@ -727,7 +745,7 @@ __global__ void __launch_bounds__(TM_THREADS) tree_attn_merge_kernel(const __gri
 }
 
 // ---- host side ----
-static int tree_sms() {
+static int tree_sms() {                                               // (at least 8, the largest number of row tiles)
     static int sms[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) { cudaGetLastError(); return 148; }
@@ -814,7 +832,9 @@ int launch_tree_attn(const TreeAttnArgs& all, void* workspace, size_t workspace_
         a.k_new += (size_t)b0 * a.N * a.KV * ATT_D; a.v_new += (size_t)b0 * a.N * a.KV * ATT_D;
         a.block_table += (size_t)b0 * a.max_pages; a.ctx_len += b0; a.parents += (size_t)b0 * a.N;
         tree_shape(p, a.N, a.H, a.KV);
-        p.G = tree_sms();
+        p.G = tree_sms() / p.row_tiles * p.row_tiles;
+        const int pairs = a.B * a.KV * p.row_tiles;
+        p.by_pair = pairs <= p.G;                                    // (fewer merge blocks that find nothing to do: each wave of them costs a microsecond)
         p.info = static_cast<int*>(workspace);
         p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + 148 * 16);
         p.part = p.part_ml + 2 * 148 * (size_t)p.rows * 2;
@@ -837,7 +857,7 @@ int launch_tree_attn(const TreeAttnArgs& all, void* workspace, size_t workspace_
         int rc = launch_pdl((const void*)tree_attn_kernel, dim3(p.G), TA_THREADS, TA_SMEM, st, args);
         if (rc) return rc;
         void* margs[] = {&p};
-        rc = launch_pdl((const void*)tree_attn_merge_kernel, dim3(p.G, (p.rows + TM_ROWS - 1) / TM_ROWS), TM_THREADS, 0, st, margs);
+        rc = launch_pdl((const void*)tree_attn_merge_kernel, dim3(p.by_pair ? pairs : p.G, (p.rows + TM_ROWS - 1) / TM_ROWS), TM_THREADS, 0, st, margs);
         if (rc) return rc;
     }
     return GDN_OK;
