@@ -674,9 +674,13 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
 }
 
 // Joins the partials of a cut pair (blockIdx.x: the pair, or the main block that it starts in): eight rows per block, a thread holds four columns of a row.
-// Bound: latency (a few hundred KiB out of L2), so all a block needs is requested at once, six partials a thread.
-constexpr int TM_ROWS = 8, TM_THREADS = 64 * TM_ROWS, TM_AHEAD = 6;
+// Bound: latency (a few hundred KiB out of L2), so what a block needs is requested at once.  Sixteen partials in flight a thread leave room for
+// one block per SM, six for two: 16 sequences (about 5 partials a pair) 43 us with six, 46 with sixteen; 2 sequences (18 a pair) 98.5 and
+// 95.6, 9 sequences (8 a pair) 27.5 and 25.7.
+constexpr int TM_ROWS = 8, TM_THREADS = 64 * TM_ROWS;
+constexpr int TM_FEW = 6, TM_MANY = 16;                              // partials requested at once where pairs have few of them, and many
 
+template <int AHEAD>
 __global__ void __launch_bounds__(TM_THREADS) tree_attn_merge_kernel(const __grid_constant__ TreeAttnPlan p) {
     __shared__ float s_w[148][TM_ROWS], s_l[148][TM_ROWS];
     __shared__ unsigned char s_live[TM_ROWS];
@@ -693,9 +697,9 @@ __global__ void __launch_bounds__(TM_THREADS) tree_attn_merge_kernel(const __gri
     // (requested at once: the rows' (m, l), the first partials and the tree; a dependent round trip to L2 costs most of a microsecond)
     const float4* part = reinterpret_cast<const float4*>(p.part) + (size_t)cg * p.rows + row;
     const size_t step = (size_t)64 * p.rows;                         // float4s of a slot
-    float4 o[TM_AHEAD];
+    float4 o[AHEAD];
 #pragma unroll
-    for (int k = 0; k < TM_AHEAD; k++)
+    for (int k = 0; k < AHEAD; k++)
         if (in && k < parts) o[k] = __ldcg(part + slot(k) * step);
     for (int k = cg; k < parts; k += TM_THREADS / TM_ROWS) {
         const float2 ml = in ? __ldcg(reinterpret_cast<const float2*>(p.part_ml + (slot(k) * p.rows + row) * 2)) : make_float2(-INFINITY, 0.f);
@@ -735,10 +739,10 @@ __global__ void __launch_bounds__(TM_THREADS) tree_attn_merge_kernel(const __gri
         acc.x = fmaf(w, x.x, acc.x); acc.y = fmaf(w, x.y, acc.y); acc.z = fmaf(w, x.z, acc.z); acc.w = fmaf(w, x.w, acc.w);
     };
 #pragma unroll
-    for (int k = 0; k < TM_AHEAD; k++)
+    for (int k = 0; k < AHEAD; k++)
         if (k < parts) add(s_w[k][r], o[k]);
-#pragma unroll 4
-    for (int k = TM_AHEAD; k < parts; k++) add(s_w[k][r], __ldcg(part + slot(k) * step));
+#pragma unroll (AHEAD / 2)
+    for (int k = AHEAD; k < parts; k++) add(s_w[k][r], __ldcg(part + slot(k) * step));
     const uint2 v = s_live[r] ? make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w)) : make_uint2(0, 0);
     *reinterpret_cast<uint2*>(a.out + (((size_t)b * a.N + node) * a.H + kvh * p.group + row % p.group) * ATT_D + 4 * cg) = v;
     GDN_BSTAMP(11);
@@ -857,7 +861,9 @@ int launch_tree_attn(const TreeAttnArgs& all, void* workspace, size_t workspace_
         int rc = launch_pdl((const void*)tree_attn_kernel, dim3(p.G), TA_THREADS, TA_SMEM, st, args);
         if (rc) return rc;
         void* margs[] = {&p};
-        rc = launch_pdl((const void*)tree_attn_merge_kernel, dim3(p.by_pair ? pairs : p.G, (p.rows + TM_ROWS - 1) / TM_ROWS), TM_THREADS, 0, st, margs);
+        // (the mean number of partials of a pair)
+        const bool few = p.G <= TM_FEW * pairs;
+        rc = launch_pdl(few ? (const void*)tree_attn_merge_kernel<TM_FEW> : (const void*)tree_attn_merge_kernel<TM_MANY>, dim3(p.by_pair ? pairs : p.G, (p.rows + TM_ROWS - 1) / TM_ROWS), TM_THREADS, 0, st, margs);
         if (rc) return rc;
     }
     return GDN_OK;
