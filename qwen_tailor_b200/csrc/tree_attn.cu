@@ -14,7 +14,7 @@
 // 112 us against 98).
 //
 // Roles: warps 0-3 softmax (one thread per query row; warps without rows sleep), warp 4 issues the MMAs, warps 5 and 6 are the TMA
-// producers of K and V, warp 7 appends the nodes' rows to the cache.  Per tile
+// producers of K and V, warp 7 appends the nodes' rows to the cache and makes their value rows fit for the product.  Per tile
 //     S [128 x 128]  = Q K^T      16 MMAs; K travels in slabs of 64 dims x 128 keys
 //     P              = 2^(S sc - m), written over S in tensor memory as bf16 hi + lo pairs (weights exact to 2^-17, as in the chained
 //                      and prefill kernels; hi alone would put an error of the size of the output's own rounding on every weight)
@@ -48,7 +48,7 @@ constexpr int TA_TAIL = 3;                                            // plan we
 constexpr float TA_RAISE = 8.f;                                       // log2 units
 enum {
     AB_QFULL = 0, AB_QEMPTY = 2, AB_KFULL = 4, AB_KEMPTY = AB_KFULL + TA_NK, AB_VFULL = AB_KEMPTY + TA_NK, AB_VEMPTY = AB_VFULL + TA_NV,
-    AB_SDONE = AB_VEMPTY + TA_NV, AB_PREADY = AB_SDONE + 2, AB_PFREE = AB_PREADY + 2, AB_ODONE = AB_PFREE + 2, AB_OFREE, AB_NODES, AB_DRAIN, AB_COUNT
+    AB_SDONE = AB_VEMPTY + TA_NV, AB_PREADY = AB_SDONE + 2, AB_PFREE = AB_PREADY + 2, AB_ODONE = AB_PFREE + 2, AB_OFREE, AB_LAST, AB_NODES, AB_DRAIN, AB_COUNT
 };
 
 struct TreeAttnPlan {
@@ -181,9 +181,8 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
     auto bar = [&](int i) -> uint32_t { return smem_addr(&bars[i]); };
     const int n_warps = (p.rows + 31) / 32;                          // softmax warps with rows
     if (tid == 32) {
-        for (int i = 0; i < AB_COUNT; i++) mbar_init(bar(i), (i >= AB_PREADY && i < AB_PREADY + 2) || i == AB_OFREE || i == AB_NODES ? n_warps : 1);
+        for (int i = 0; i < AB_COUNT; i++) mbar_init(bar(i), (i >= AB_PREADY && i < AB_PREADY + 2) || i == AB_OFREE ? n_warps : 1);
         s_abort = 0;
-        s_badv[0] = s_badv[1] = 0;
         fence_barrier_init();
         tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV); tma_prefetch_desc(&tmKn); tma_prefetch_desc(&tmVn);
     }
@@ -411,6 +410,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                     GDN_TSTAMP(n * 16 + 1);
                     if (t == s.t0 + s.n - 1) mma_commit(bar(AB_QEMPTY + qb));
                     if (p_have) ok = issue_pv(n - 1, p_limit, p_first, p_last, p_seg);
+                    if (t == s.tiles - 1) mma_commit(bar(AB_LAST));  // the chunks before the nodes' have been consumed
                     p_have = true; p_limit = limit_of(s, t); p_first = t == s.t0; p_last = t == s.t0 + s.n - 1; p_seg = nseg;
                 }
                 nseg++;
@@ -419,29 +419,110 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
             if (!ok) { mma_commit(bar(AB_DRAIN)); mbar_wait(bar(AB_DRAIN), 0, 100000u); }      // gave up: nothing may run on after the block
         }
     } else if (warp == 7) {
-        // ================= append: the nodes' rows into the cache, by the block that has a pair's first tile =================
+        // ================= nodes: their rows into the cache, by the block that has a pair's first tile; their value rows fit for the product =================
+        uint32_t nv = 0, node_tiles = 0;                             // V chunks and node tiles so far
+        bool ok = true;
 #pragma unroll 1
-        for (int x = lo; x < hi;) {
+        for (int x = lo; x < hi && ok;) {
             const TreeSeg s = segment(x);
             x += s.span;
-            if (s.t0 != 0 || rt != 0 || s.ctx < 0) continue;
-            const int* par = a.parents + (size_t)s.b * a.N;
-            unsigned long long l0, l1;
-            bool bad;
-            warp_lines(lane < a.N ? par[lane] : -2, lane + 32 < a.N ? par[lane + 32] : -2, l0, l1, bad);
-            if (bad) atomicExch(a.status, 1);
-            const unsigned long long used = __ballot_sync(0xffffffffu, l0 != 0) | (unsigned long long)__ballot_sync(0xffffffffu, l1 != 0) << 32;
-            const int* table = a.block_table + (size_t)s.b * a.max_pages;
-#pragma unroll 1
-            for (int i = 0; i < a.N; i++) {
-                if (!(used >> i & 1)) continue;
-                const int at = s.ctx + i;
-                const int page = table[at / a.page_size];
-                if (page < 0 || page >= a.n_pages) { if (lane == 0) atomicExch(a.status, 1); continue; }
-                const size_t src = (((size_t)s.b * a.N + i) * a.KV + s.kvh) * ATT_D, dst = (((size_t)page * a.KV + s.kvh) * a.page_size + at % a.page_size) * ATT_D;
-                reinterpret_cast<uint4*>(a.k_pages + dst)[lane] = reinterpret_cast<const uint4*>(a.k_new + src)[lane];
-                reinterpret_cast<uint4*>(a.v_pages + dst)[lane] = reinterpret_cast<const uint4*>(a.v_new + src)[lane];
+            if (s.n <= 0) continue;
+            const bool has_nodes = s.t0 + s.n == s.tiles, append = s.t0 == 0 && rt == 0 && s.ctx >= 0;
+            unsigned long long used = 0;
+            if (append || has_nodes) {
+                const int* par = a.parents + (size_t)s.b * a.N;
+                unsigned long long l0, l1;
+                bool bad;
+                warp_lines(s.ctx >= 0 && lane < a.N ? par[lane] : -2, s.ctx >= 0 && lane + 32 < a.N ? par[lane + 32] : -2, l0, l1, bad);
+                if (bad && append) atomicExch(a.status, 1);
+                used = __ballot_sync(0xffffffffu, l0 != 0) | (unsigned long long)__ballot_sync(0xffffffffu, l1 != 0) << 32;
             }
+            auto append_rows = [&]() {                               // four rows of K and V in flight
+                const int* table = a.block_table + (size_t)s.b * a.max_pages;
+                int page[2];
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const int i = lane + 32 * k;
+                    page[k] = used >> i & 1 ? table[(s.ctx + i) / a.page_size] : -1;
+                    if ((used >> i & 1) && (page[k] < 0 || page[k] >= a.n_pages)) { atomicExch(a.status, 1); page[k] = -1; }
+                }
+#pragma unroll 1
+                for (int i0 = 0; i0 < a.N; i0 += 4) {
+                    uint4 kr[4], vr[4];
+                    size_t dst[4];
+                    bool on[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int i = i0 + k, pg = __shfl_sync(0xffffffffu, i0 < 32 ? page[0] : page[1], i & 31);
+                        on[k] = i < a.N && pg >= 0;
+                        dst[k] = (((size_t)pg * a.KV + s.kvh) * a.page_size + (s.ctx + i) % a.page_size) * ATT_D;
+                        if (on[k]) {
+                            const size_t src = (((size_t)s.b * a.N + i) * a.KV + s.kvh) * ATT_D;
+                            kr[k] = reinterpret_cast<const uint4*>(a.k_new + src)[lane];
+                            vr[k] = reinterpret_cast<const uint4*>(a.v_new + src)[lane];
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if (on[k]) {
+                            reinterpret_cast<uint4*>(a.k_pages + dst[k])[lane] = kr[k];
+                            reinterpret_cast<uint4*>(a.v_pages + dst[k])[lane] = vr[k];
+                        }
+                }
+            };
+            // a long range has time for the copies before its nodes' tile comes up, a short one after it
+            if (append && s.n >= 4) append_rows();
+            nv += (max(min(s.ctx, (s.t0 + s.n) * TA_TK) - s.t0 * TA_TK, 0) + 31) / 32;
+            if (has_nodes) {
+                // value rows of unused nodes (and behind the last) and the non-finite values of the others are zeroed, once the chunks
+                // before these have been consumed (a parity of the ring cannot tell a phase from the one two before).  The wait lasts as
+                // long as the segment, and so does its bound.
+                int got = 0;
+                if (lane == 0) {
+                    for (long long i = 0; i < 1000000ll * (s.n + 1) && !got && !aborted(); i++) {
+                        got = mbar_test_wait(bar(AB_LAST), node_tiles & 1u);
+                        if (!got) __nanosleep(100);
+                    }
+                    if (!got && !aborted()) { s_abort = 1; atomicExch(a.status, 2); }
+                }
+                ok = __shfl_sync(0xffffffffu, got, 0) != 0;
+                unsigned long long seen_bad = 0;
+#pragma unroll 1
+                for (int c = 0; c < (a.N + 31) / 32 && ok; c++) {
+                    const uint32_t slot = (nv + c) % TA_NV;
+                    ok = warp_wait(AB_VFULL + slot, (nv + c) / TA_NV);
+                    if (!ok) break;
+                    unsigned char* chunk = smem + TA_Q_BYTES + TA_NK * TA_SLOT + slot * TA_SLOT + (lane >> 3) * 4096;      // lane = 16-byte column of a row
+#pragma unroll 4
+                    for (int r = 0; r < 32; r++) {
+                        uint4* at = reinterpret_cast<uint4*>(chunk + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+                        if (!(used >> (32 * c + r) & 1)) { *at = make_uint4(0, 0, 0, 0); continue; }
+                        const uint4 v = *at;
+                        uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                        // an exponent of ones in either half carries into the half's top bit
+                        const uint32_t E = 0x7f807f80u, one = 0x00800080u;
+                        if (!((((w[0] & E) + one) | ((w[1] & E) + one) | ((w[2] & E) + one) | ((w[3] & E) + one)) & 0x80008000u)) continue;
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            if (bf16_not_finite(w[q])) w[q] &= 0xffff0000u;
+                            if (bf16_not_finite(w[q] >> 16)) w[q] &= 0xffffu;
+                        }
+                        seen_bad |= 1ull << (32 * c + r);
+                        *at = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                if (!ok) break;
+                fence_proxy_async_smem();
+                __syncwarp();
+                const uint32_t b0 = __reduce_or_sync(0xffffffffu, (uint32_t)seen_bad), b1 = __reduce_or_sync(0xffffffffu, (uint32_t)(seen_bad >> 32));
+                if (lane == 0) {
+                    s_badv[node_tiles & 1] = b0 | (unsigned long long)b1 << 32;      // (last read before the product two node tiles ago)
+                    mbar_arrive(bar(AB_NODES));
+                }
+                node_tiles++;
+                nv += (a.N + 31) / 32;
+            }
+            if (append && s.n < 4) append_rows();
         }
     } else if (warp < n_warps) {
         // ================= softmax and epilogue: thread = row = node * group + head =================
@@ -471,18 +552,16 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                 const int limit = limit_of(s, t), chunks = (limit + 31) / 32;
                 const bool nodes = t == s.tiles - 1;
                 const uint32_t sp = tl + TAM_SP0 + (n & 1) * 128;
-                if (!warp_wait(AB_SDONE + (n & 1), n >> 1)) { ok = false; break; }
-                tc_fence_after_sync();
-                if (warp == 0) GDN_TSTAMP(n * 16 + 4);
-                unsigned long long used = 0;                         // (nodes tile) nodes in use
                 if (nodes) {                                         // the ancestors of this row's node
                     unsigned long long l0, l1;
                     bool bad;
                     warp_lines(par0, par1, l0, l1, bad);
-                    used = __ballot_sync(0xffffffffu, l0 != 0) | (unsigned long long)__ballot_sync(0xffffffffu, l1 != 0) << 32;
                     const unsigned long long x0 = shfl64(l0, node & 31), x1 = shfl64(l1, node & 31);
                     line = real ? (node < 32 ? x0 : x1) : 0;
                 }
+                if (!warp_wait(AB_SDONE + (n & 1), n >> 1)) { ok = false; break; }
+                tc_fence_after_sync();
+                if (warp == 0) GDN_TSTAMP(n * 16 + 4);
                 // Two passes over the scores, 32 columns at a time in rolled loops: the code of a tile has to stay small (unrolled over the 128
                 // columns it drove the producers' and the issuer's code out of the instruction cache, and every step of theirs took
                 // hundreds of cycles).  Masked scores are replaced by -inf.
@@ -553,49 +632,23 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                 }
                 tmem_wait_st();
                 if (warp == 0) GDN_TSTAMP(n * 16 + 6);
-                if (nodes || (limit & 15)) {
-                    // value rows that nobody may see, and a node's non-finite values, are zeroed before the product reads them.  These warps
+                if (nodes) {                                         // warp 7 has made the nodes' value rows ready
+                    if (!warp_wait(AB_NODES, node_tiles)) { ok = false; break; }
+                    badv = *(volatile unsigned long long*)&s_badv[node_tiles & 1];
+                    node_tiles++;
+                } else if (limit & 15) {
+                    // value rows behind the context are zeroed, up to the next multiple of 16 keys, before the product reads them.  These warps
                     // do not wait for every phase of the V ring, and a parity cannot tell a phase from the one two before: once the
                     // product of the tile before is done, the chunks before this tile's have all been consumed.
                     if (n > 0 && !warp_wait(AB_PFREE + ((n - 1) & 1), (n - 1) >> 1)) { ok = false; break; }
-                    unsigned long long seen_bad = 0;
-                    // (nodes: all rows of its chunks; the last context tile: the rows behind the context, up to the next multiple of 16 keys)
+                    const int slot = (nv + chunks - 1) % TA_NV, r0 = limit & 31, r1 = (r0 + 15) & ~15;
+                    if (!warp_wait(AB_VFULL + slot, (nv + chunks - 1) / TA_NV)) { ok = false; break; }
 #pragma unroll 1
-                    for (int c = nodes ? 0 : chunks - 1; c < chunks && ok; c++) {
-                        const int slot = (nv + c) % TA_NV;
-                        if (!warp_wait(AB_VFULL + slot, (nv + c) / TA_NV)) { ok = false; break; }
-                        const int r0 = nodes ? 0 : limit & 31, r1 = nodes ? 32 : (r0 + 15) & ~15;
-#pragma unroll 4
-                        for (int i = row; i < (r1 - r0) * 32; i += n_warps * 32) {
-                            const int r = r0 + (i >> 5), k = 32 * c + r, ch = i & 31;
-                            uint4* at = reinterpret_cast<uint4*>(smem + TA_Q_BYTES + TA_NK * TA_SLOT + slot * TA_SLOT + (ch >> 3) * 4096 + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
-                            if (!nodes || !(used >> k & 1)) { *at = make_uint4(0, 0, 0, 0); continue; }
-                            const uint4 v = *at;
-                            uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                            // an exponent of ones in either half carries into the half's top bit
-                            const uint32_t E = 0x7f807f80u, one = 0x00800080u;
-                            if (!((((w[0] & E) + one) | ((w[1] & E) + one) | ((w[2] & E) + one) | ((w[3] & E) + one)) & 0x80008000u)) continue;
-#pragma unroll
-                            for (int q = 0; q < 4; q++) {
-                                if (bf16_not_finite(w[q])) w[q] &= 0xffff0000u;
-                                if (bf16_not_finite(w[q] >> 16)) w[q] &= 0xffffu;
-                            }
-                            seen_bad |= 1ull << k;
-                            *at = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
+                    for (int i = row; i < (r1 - r0) * 32; i += n_warps * 32) {
+                        const int r = r0 + (i >> 5), ch = i & 31;
+                        *reinterpret_cast<uint4*>(smem + TA_Q_BYTES + TA_NK * TA_SLOT + slot * TA_SLOT + (ch >> 3) * 4096 + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
                     }
                     fence_proxy_async_smem();
-                    if (nodes) {
-                        if (seen_bad) atomicOr(&s_badv[node_tiles & 1], seen_bad);
-                        __threadfence_block();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(bar(AB_NODES));
-                        ok = warp_wait(AB_NODES, node_tiles) && ok;
-                        badv = *(volatile unsigned long long*)&s_badv[node_tiles & 1];
-                        if (tid == 0) s_badv[(node_tiles + 1) & 1] = 0;      // (last read before this barrier)
-                        node_tiles++;
-                    }
-                    if (!ok) break;
                 }
                 nv += chunks;
                 tc_fence_before_sync();
