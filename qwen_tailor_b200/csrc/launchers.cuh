@@ -169,6 +169,7 @@ struct TreeCommitArgs {
     const int *slots, *dst_slots, *pos, *path, *n_path;      // [B] each, path [B, E]
     int* status;
     int B, N, E, n_slots;
+    int ahead;                                               // layers between a block and the one it prefetches for
 };
 int launch_tree_commit(const TreeCommitArgs& a, int n_layers, cudaStream_t st);
 int launch_tree_accept(const int* parents, const int* toks, const int* ids, int* path, int* n_path, int* status, int B, int N, cudaStream_t st);

@@ -571,15 +571,18 @@ int launch_tree_accept(const int* parents, const int* toks, const int* ids, int*
 }
 
 // ----------------------------------------------------------------------------------------------------------------------
-// commit: one block per (layer, sequence, head), two per SM.  Bound: HBM, the state once in and once out (2 MiB per layer and
-// sequence), and behind it the issue slots (about 10 k instructions a head and four tokens).  The state lies in registers, a row on 8
-// lanes of 4 float4 each, so that a quarter warp reads 128 contiguous bytes.  Two levels of loads, each all at once, because a load
-// costs microseconds while the states stream: first the indices, the path and the weights, then everything they point to; the
-// conv / norm / gate work of the path's tokens runs while the state arrives.  24 sequences x 18 layers: 253 us (3.8 TB/s); measured
-// and not kept: half heads on four blocks per SM (305), 512 threads a head (309), the next states prefetched into L2 (268), persistent
-// blocks with a bulk-copy ring, preparing warps and eight tokens at a time (225 .. 380 by variant, 25 against 16 us for one sequence).
+// commit: one block per (layer, sequence, head), two per SM.  Bound: HBM, the state once in and once out (2 MiB per layer and sequence).
+// One bulk copy brings a head's state into shared memory while the path's tokens go through conv, norm and gates; then half of it at a time
+// lies in registers, a row on 8 lanes of 4 float4 each, so that a quarter warp reads and writes 128 contiguous bytes.  While the states
+// stream, a load that misses L2 takes 5 us, so a block asks L2 for the rows that a block of a later layer will need (32 KiB against its 128
+// of state, and the states are marked to leave L2 first).  24 sequences x 18 layers, accept and compaction included: 200 us (4.8 TB/s),
+// without the prefetch 249, two layers ahead instead of one 202.  Measured and not kept: state by plain loads (256), three blocks per SM with 80
+// registers (204 .. 215), half heads on four blocks (305), 512 threads a head (309), persistent blocks with a ring of bulk copies (225 .. 380,
+// 25 against 14 us for one sequence).
 // ----------------------------------------------------------------------------------------------------------------------
-constexpr int CM_THREADS = 256, CM_STEPS = 16;                       // tokens of the path prepared at a time
+constexpr int CM_THREADS = 256, CM_STEPS = 8;                        // tokens of the path prepared at a time
+constexpr int STATE_BYTES = DV * DK * 4;
+constexpr int CM_GENERATION = 300;                                   // blocks between a prefetch and its use: as many as are resident
 constexpr int CM_PATH = 64, CM_AHEAD = 8;                            // path entries kept in shared memory; raw rows in flight
 
 // silu to a few fp32 ulp: expf's own error and an approximate division
@@ -587,6 +590,8 @@ __device__ __forceinline__ float silu_ulp(float x) { return __fdividef(x, 1.f + 
 __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) { f32x2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 
 __global__ void __launch_bounds__(CM_THREADS, 2) tree_commit_kernel(const __grid_constant__ TreeCommitArgs a) {
+    extern __shared__ __align__(1024) unsigned char smem[];          // the state as it comes in
+    __shared__ uint64_t s_bar;
     __shared__ __align__(16) float s_k[CM_STEPS][DK];
     __shared__ float s_v[CM_STEPS][DV], s_g[CM_STEPS], s_beta[CM_STEPS], s_red[CM_STEPS][4];
     __shared__ int s_path[CM_PATH];
@@ -602,6 +607,18 @@ __global__ void __launch_bounds__(CM_THREADS, 2) tree_commit_kernel(const __grid
     const float A_log = a.A_log[layer][h], dt_bias = a.dt_bias[layer][h];
     bool bad = slot < 0 || slot >= a.n_slots || dst < 0 || dst >= a.n_slots || pos < 0 || n < 0 || n > a.E;
     if (!bad && n == 0 && slot == dst) return;
+    const uint32_t landed = smem_addr(&s_bar);
+    const bool loads = !bad;                                         // (uniform)
+    if (tid == 0 && loads) {
+        mbar_init(landed, 1);
+        fence_barrier_init();
+        mbar_expect_tx(landed, STATE_BYTES);
+        const char* src = reinterpret_cast<const char*>(a.ssm_pool[layer] + (size_t)slot * STATE_ELEMS + (size_t)h * DV * DK);
+        uint64_t once;                                               // (read once: first to leave L2)
+        asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;"
+                     ::"r"(smem_addr(smem)), "l"(src), "r"(STATE_BYTES), "r"(landed), "l"(once) : "memory");
+    }
     if (tid < CM_PATH) s_path[tid] = first;
     bad = bad || (tid < n && tid < CM_PATH && (first < 0 || first >= a.N));
     // another sequence that writes what this one reads or writes, or reads what it writes, would make the result a matter of order: both
@@ -614,10 +631,26 @@ __global__ void __launch_bounds__(CM_THREADS, 2) tree_commit_kernel(const __grid
     for (int o = tid + CM_THREADS; o < a.B; o += CM_THREADS) bad = bad || clash(o, a.slots[o], a.dst_slots[o], a.n_path[o]);
     if (!bad)
         for (int j = CM_PATH + tid; j < n; j += CM_THREADS) bad = bad || path[j] < 0 || path[j] >= a.N;
-    if (__syncthreads_or(bad)) { if (tid == 0) atomicExch(a.status, 1); return; }
+    if (__syncthreads_or(bad)) {
+        if (tid == 0) { atomicExch(a.status, 1); if (loads) mbar_wait(landed, 0); }      // (nothing may land after the block)
+        return;
+    }
     auto node = [&](int j) -> int { return j < CM_PATH ? s_path[j] : path[j]; };
     const __nv_bfloat16* rows = a.proj[layer] + (size_t)b * a.N * a.row_stride;
     const __nv_bfloat16* win = a.conv_pool[layer] + ((size_t)slot * 2 + (pos & 1)) * 3 * CD;
+    // A load that misses L2 while the states stream takes 5 us, one that hits 0.8: the rows that this sequence's block of a later layer
+    // will read (about one generation of blocks ahead) are asked for now.
+    const int later = layer + a.ahead;
+    if (later < gridDim.y) {
+        const __nv_bfloat16* rows2 = a.proj[later] + (size_t)b * a.N * a.row_stride;
+        const __nv_bfloat16* win2 = a.conv_pool[later] + ((size_t)slot * 2 + (pos & 1)) * 3 * CD;
+        for (int i = tid; i < (n + 3) * 8; i += CM_THREADS) {
+            const int r = i >> 3, part = (i & 7) >> 1;               // parts: q, k, v (two lines each), gates
+            const __nv_bfloat16* base = r < 3 ? win2 + (size_t)r * CD : rows2 + (size_t)node(r - 3) * a.row_stride;
+            const __nv_bfloat16* line = part < 3 ? base + part * KD + h * DK + (i & 1) * 64 : base + CD + KD;
+            if (part == 0 ? r >= n : part < 3 || (r >= 3 && !(i & 1))) asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
+        }
+    }
     // raw row r of the sequence: 0..2 the window, 3 + j the path's tokens
     auto raw = [&](int r, int chan) -> __nv_bfloat16 { return r < 3 ? win[(size_t)r * CD + chan] : rows[(size_t)node(r - 3) * a.row_stride + chan]; };
     __nv_bfloat16 x0 = win[ch], x1 = win[CD + ch], x2 = win[2 * CD + ch], q0, q1, q2;
@@ -635,18 +668,31 @@ __global__ void __launch_bounds__(CM_THREADS, 2) tree_commit_kernel(const __grid
         raw_b = r[0]; raw_a = r[HV];
     };
     if (tid < min(n, CM_STEPS)) fetch_gates(tid);
-    // ---- the state ----
-    const int row = warp * 16 + (lane >> 3), col = (lane & 7) * 4;   // rows row + 4 i, columns col + 32 m
-    const size_t at = (size_t)h * DV * DK + (size_t)row * DK + col;
-    const float* src = a.ssm_pool[layer] + (size_t)slot * STATE_ELEMS + at;
-    ulonglong2 S[4][4];
+    // this thread's part of the state, in two halves: rows row + 8 half + 4 i, columns col + 32 m
+    const int row = warp * 16 + (lane >> 3), col = (lane & 7) * 4;
+    float* out = a.ssm_pool[layer] + (size_t)dst * STATE_ELEMS + (size_t)h * DV * DK;
+    bool ok = true;
+    ulonglong2 S[2][4];
+    auto take = [&](int half) {
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+        for (int i = 0; i < 2; i++)
 #pragma unroll
-        for (int m = 0; m < 4; m++) {
-            const float4 v = __ldcs(reinterpret_cast<const float4*>(src + 4 * i * DK + 32 * m));
-            S[i][m] = make_ulonglong2(pack2(v.x, v.y), pack2(v.z, v.w));
-        }
+            for (int m = 0; m < 4; m++) S[i][m] = *reinterpret_cast<const ulonglong2*>(smem + ((row + 8 * half + 4 * i) * DK + col + 32 * m) * 4);
+    };
+    auto put = [&](int half, bool last) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int m = 0; m < 4; m++) {
+                const int e = (row + 8 * half + 4 * i) * DK + col + 32 * m;
+                if (last) {
+                    const float2 lo = unpack2(S[i][m].x), hi = unpack2(S[i][m].y);
+                    __stcs(reinterpret_cast<float4*>(out + e), make_float4(lo.x, lo.y, hi.x, hi.y));
+                } else {
+                    *reinterpret_cast<ulonglong2*>(smem + e * 4) = S[i][m];
+                }
+            }
+    };
     float w[4];
     unpack_bf16x4(taps, w);
     for (int j0 = 0; j0 < n; j0 += CM_STEPS) {
@@ -676,50 +722,52 @@ __global__ void __launch_bounds__(CM_THREADS, 2) tree_commit_kernel(const __grid
             }
         }
         __syncthreads();
-        for (int j = 0; j < cnt; j++) {
-            // k is used as it left the conv; its length enters the two places where k does
-            const float r = rsqrtf((s_red[j][0] + s_red[j][1]) + (s_red[j][2] + s_red[j][3]) + 1e-6f);
-            const float g = s_g[j], beta = s_beta[j];
-            const f32x2 gg = pack2(g, g);
-            ulonglong2 k[4];
+        if (j0 == 0 && !mbar_wait(landed, 0)) { ok = false; break; }
+#pragma unroll 1
+        for (int half = 0; half < 2; half++) {
+            take(half);
+            for (int j = 0; j < cnt; j++) {
+                // k is used as it left the conv; its length enters the two places where k does
+                const float r = rsqrtf((s_red[j][0] + s_red[j][1]) + (s_red[j][2] + s_red[j][3]) + 1e-6f);
+                const float g = s_g[j], beta = s_beta[j];
+                const f32x2 gg = pack2(g, g);
+                ulonglong2 k[4];
 #pragma unroll
-            for (int m = 0; m < 4; m++) k[m] = *reinterpret_cast<const ulonglong2*>(&s_k[j][col + 32 * m]);
-            float p[4];
+                for (int m = 0; m < 4; m++) k[m] = *reinterpret_cast<const ulonglong2*>(&s_k[j][col + 32 * m]);
+                float p[2];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                f32x2 p0 = 0, p1 = 0;
+                for (int i = 0; i < 2; i++) {
+                    f32x2 p0 = 0, p1 = 0;
 #pragma unroll
-                for (int m = 0; m < 4; m++) {
-                    S[i][m].x = mul2(S[i][m].x, gg); S[i][m].y = mul2(S[i][m].y, gg);
-                    fma2(p0, S[i][m].x, k[m].x); fma2(p1, S[i][m].y, k[m].y);
+                    for (int m = 0; m < 4; m++) {
+                        S[i][m].x = mul2(S[i][m].x, gg); S[i][m].y = mul2(S[i][m].y, gg);
+                        fma2(p0, S[i][m].x, k[m].x); fma2(p1, S[i][m].y, k[m].y);
+                    }
+                    const float2 a0 = unpack2(p0), a1 = unpack2(p1);
+                    p[i] = (a0.x + a0.y) + (a1.x + a1.y);
                 }
-                const float2 a0 = unpack2(p0), a1 = unpack2(p1);
-                p[i] = (a0.x + a0.y) + (a1.x + a1.y);
-            }
-            // the four rows' sums over their eight lanes: two exchanges leave lane l with row l & 3's, one more completes it
-            const bool o1 = lane & 1, o2 = lane & 2;
-            const float t0 = (o1 ? p[1] : p[0]) + __shfl_xor_sync(0xffffffffu, o1 ? p[0] : p[1], 1);
-            const float t1 = (o1 ? p[3] : p[2]) + __shfl_xor_sync(0xffffffffu, o1 ? p[2] : p[3], 1);
-            float s = (o2 ? t1 : t0) + __shfl_xor_sync(0xffffffffu, o2 ? t0 : t1, 2);
-            s += __shfl_xor_sync(0xffffffffu, s, 4);
-            const float u = (s_v[j][row + 4 * (lane & 3)] - s * r) * beta * r;      // of row `row + 4 (lane & 3)`
+                // the two rows' sums over their eight lanes: one exchange leaves lane l with row l & 1's, two more complete it
+                const bool odd = lane & 1;
+                float x = (odd ? p[1] : p[0]) + __shfl_xor_sync(0xffffffffu, odd ? p[0] : p[1], 1);
+                x += __shfl_xor_sync(0xffffffffu, x, 2);
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                const float u = (s_v[j][row + 8 * half + 4 * (lane & 1)] - x * r) * beta * r;      // of row `row + 8 half + 4 (lane & 1)`
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float ui = __shfl_sync(0xffffffffu, u, (lane & 24) + i);
-                const f32x2 uu = pack2(ui, ui);
+                for (int i = 0; i < 2; i++) {
+                    const float ui = __shfl_sync(0xffffffffu, u, (lane & 24) + i);
+                    const f32x2 uu = pack2(ui, ui);
 #pragma unroll
-                for (int m = 0; m < 4; m++) { fma2(S[i][m].x, uu, k[m].x); fma2(S[i][m].y, uu, k[m].y); }
+                    for (int m = 0; m < 4; m++) { fma2(S[i][m].x, uu, k[m].x); fma2(S[i][m].y, uu, k[m].y); }
+                }
             }
+            put(half, j0 + cnt >= n);
         }
     }
-    float* out = a.ssm_pool[layer] + (size_t)dst * STATE_ELEMS + at;
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int m = 0; m < 4; m++) {
-            const float2 lo = unpack2(S[i][m].x), hi = unpack2(S[i][m].y);
-            __stcs(reinterpret_cast<float4*>(out + 4 * i * DK + 32 * m), make_float4(lo.x, lo.y, hi.x, hi.y));
-        }
+    if (n == 0) {
+        ok = mbar_wait(landed, 0);
+        if (ok) for (int half = 0; half < 2; half++) { take(half); put(half, true); }
+    }
+    if (!ok) { atomicExch(a.status, 2); return; }
     // a window buffer that is read and written in one call (n even): every channel has been read by the thread that writes it
     __nv_bfloat16* wout = a.conv_pool[layer] + ((size_t)dst * 2 + (((unsigned)pos + (unsigned)n) & 1)) * 3 * CD;
     wout[ch] = x0; wout[CD + ch] = x1; wout[2 * CD + ch] = x2;
@@ -728,7 +776,16 @@ __global__ void __launch_bounds__(CM_THREADS, 2) tree_commit_kernel(const __grid
 
 int launch_tree_commit(const TreeCommitArgs& a, int n_layers, cudaStream_t st) {
     if (a.B <= 0 || n_layers <= 0) return GDN_OK;
-    tree_commit_kernel<<<dim3((unsigned)(a.B * HV), n_layers), CM_THREADS, 0, st>>>(a);
+    static bool attr_set[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 0 && dev < 64 && !attr_set[dev]) {
+        if (cudaFuncSetAttribute(tree_commit_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, STATE_BYTES) != cudaSuccess) return check_launch("tree_commit smem attribute");
+        attr_set[dev] = true;
+    }
+    TreeCommitArgs with = a;
+    with.ahead = (CM_GENERATION + a.B * HV - 1) / (a.B * HV);
+    tree_commit_kernel<<<dim3((unsigned)(a.B * HV), n_layers), CM_THREADS, STATE_BYTES, st>>>(with);
     return check_launch("tree_commit");
 }
 
