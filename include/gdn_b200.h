@@ -293,7 +293,7 @@ GDN_API int gdn_rows_compact(void* const* pools_host, int n_pools, int n_pages, 
                      const int* dst_table, int max_pages, const int* base, const int* keep, const int* n_keep, int B, int L, void* stream);
 
 /* Entry dst_host[i] <- entry src_host[i] of every pool [n_entries][n_sub][sub_bytes]; of each sub-block the first len_host[i] bytes (NULL: all).
- * Indices are host arrays.  No dst may equal another dst or any src (unchecked here; the copies are unordered).  Sizes are even. */
+ * Indices are host arrays.  No dst may equal another dst or any src (GDN_E_INDEX: the copies are unordered).  Sizes are even. */
 GDN_API int gdn_entries_copy(void* const* pools_host, int n_pools, long long n_entries, int n_sub, long long sub_bytes, const int* dst_host,
                      const int* src_host, const long long* len_host, int n_pairs, void* stream);
 

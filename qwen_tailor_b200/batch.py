@@ -203,7 +203,7 @@ def copy_entries(pools: Sequence[torch.Tensor], dst: Sequence[int], src: Sequenc
     pools: contiguous tensors [n_entries, ...] of one shape and type (bf16 or fp32); stacked=True: each has a leading layer dimension.
     dst, src: host integers.  One source may be copied to many entries; no dst may repeat or be a src (ValueError).
     rows (an int, or one per pair): only the first rows of every head of pages [n_entries, heads, page_size, dim] are copied.
-    Every 160 pairs take one launch."""
+    Every 512 pairs take one launch."""
     first, shape, ptrs = _pool_ptrs("copy_entries", pools, stacked)
     d, s = array("i", dst), array("i", src)
     n = len(d)
@@ -211,26 +211,26 @@ def copy_entries(pools: Sequence[torch.Tensor], dst: Sequence[int], src: Sequenc
         raise ValueError(f"copy_entries: {n} destinations for {len(s)} sources")
     if n == 0:
         return
-    targets, sources = set(d), set(s)
-    if min(targets) < 0 or min(sources) < 0 or max(targets) >= shape[0] or max(sources) >= shape[0]:
-        raise ValueError(f"copy_entries: an entry outside [0, {shape[0]})")
-    if len(targets) < n or not targets.isdisjoint(sources):
-        raise ValueError("copy_entries: a destination is named twice, or is a source too")
     item, lens = first.element_size(), None
     n_sub, sub_bytes = 1, prod(shape[1:]) * item
     if rows is not None:
         if len(shape) != 4:
             raise ValueError(f"copy_entries: rows needs pools [n_entries, heads, page_size, dim], got entries of {tuple(shape[1:])}")
-        r = array("q", [rows] * n if isinstance(rows, Integral) else rows)
-        if len(r) != n or min(r) < 0 or max(r) > shape[2]:
+        row, one = shape[3] * item, isinstance(rows, Integral)
+        r = (int(rows),) if one else array("q", rows)
+        if (not one and len(r) != n) or min(r) < 0 or max(r) > shape[2]:
             raise ValueError(f"copy_entries: rows must be one number or {n}, from 0 to {shape[2]}")
-        n_sub, sub_bytes = shape[1], shape[2] * shape[3] * item
-        row = shape[3] * item
+        n_sub, sub_bytes = shape[1], shape[2] * row
         lens = array("q", [x * row for x in r])
+        if one:
+            lens *= n
     dev = first.device
     with on_device(dev):
-        check(_lib.load().gdn_entries_copy(_address(ptrs), len(ptrs), shape[0], n_sub, sub_bytes, _address(d), _address(s), _address(lens) if lens is not None else None, n,
-                                           raw_stream(dev)), "copy_entries")
+        rc = _lib.load().gdn_entries_copy(_address(ptrs), len(ptrs), shape[0], n_sub, sub_bytes, _address(d), _address(s), _address(lens) if lens is not None else None, n,
+                                          raw_stream(dev))
+    if rc == -4:                                                     # an entry out of range, named twice as a destination, or both source and destination
+        raise ValueError(_lib.load().gdn_last_error_string().decode())
+    check(rc, "copy_entries")
 
 
 def compact_rows(pools: Sequence[torch.Tensor], block_table, base, keep, n_keep, dst_table=None, stacked=False):

@@ -5,6 +5,8 @@
 
 #include <cstdarg>
 #include <cstdio>
+#include <cstdlib>
+#include <cstring>
 
 namespace gdn {
 
@@ -475,29 +477,57 @@ int gdn_entries_copy(void* const* pools_host, int n_pools, long long n_entries, 
     if (n_pools == 0 || n_pairs == 0) return GDN_OK;
     REQUIRE(pools_host && dst_host && src_host, GDN_E_NULL, "gdn_entries_copy: null pointer");
     for (int p = 0; p < n_pools; p++) REQUIRE(pools_host[p] && (uintptr_t)pools_host[p] % 2 == 0, GDN_E_NULL, "gdn_entries_copy: null or odd pool %d", p);
-    for (int i = 0; i < n_pairs; i++) {
-        REQUIRE(dst_host[i] >= 0 && dst_host[i] < n_entries && src_host[i] >= 0 && src_host[i] < n_entries, GDN_E_INDEX,
-                "gdn_entries_copy: pair %d copies entry %d to %d of %lld", i, src_host[i], dst_host[i], n_entries);
-        REQUIRE(!len_host || (len_host[i] >= 0 && len_host[i] <= sub_bytes && len_host[i] % 2 == 0), GDN_E_SHAPE, "gdn_entries_copy: pair %d: %lld of %lld bytes", i,
-                len_host[i], sub_bytes);
+    const bool whole = !len_host;
+    bool same = true;                                                // every pair copies the same number of bytes
+    REQUIRE(whole || sub_bytes / 2 <= 0xffffffffll, GDN_E_UNSUPPORTED, "gdn_entries_copy: parts of sub-blocks of %lld bytes", sub_bytes);
+    // which entries are destinations; a source or a second destination among them would make the result a matter of order
+    unsigned char few[1024] = {}, *mark = few;
+    if (n_entries > 8 * (long long)sizeof(few)) {
+        mark = static_cast<unsigned char*>(calloc((size_t)(n_entries + 7) / 8, 1));
+        REQUIRE(mark, GDN_E_UNSUPPORTED, "gdn_entries_copy: no memory to check %lld entries", n_entries);
     }
+    int rc = GDN_OK;
+    for (int i = 0; i < n_pairs && !rc; i++) {
+        const int d = dst_host[i], e = src_host[i];
+        if (d < 0 || d >= n_entries || e < 0 || e >= n_entries) {
+            set_error("gdn_entries_copy: pair %d copies entry %d to %d of %lld", i, e, d, n_entries);
+            rc = GDN_E_INDEX;
+        } else if (mark[d >> 3] >> (d & 7) & 1) {
+            set_error("gdn_entries_copy: entry %d is named twice as a destination", d);
+            rc = GDN_E_INDEX;
+        } else if (!whole && (len_host[i] < 0 || len_host[i] > sub_bytes || len_host[i] % 2)) {
+            set_error("gdn_entries_copy: pair %d: %lld of %lld bytes", i, len_host[i], sub_bytes);
+            rc = GDN_E_SHAPE;
+        } else {
+            mark[d >> 3] |= 1u << (d & 7);
+            same = same && (whole || len_host[i] == len_host[0]);
+        }
+    }
+    for (int i = 0; i < n_pairs && !rc; i++) {
+        const int e = src_host[i];
+        if (mark[e >> 3] >> (e & 7) & 1) {
+            set_error("gdn_entries_copy: entry %d is a source and a destination", e);
+            rc = GDN_E_INDEX;
+        }
+    }
+    if (mark != few) free(mark);
+    if (rc) return rc;
     for (int p0 = 0; p0 < n_pools; p0 += EC_MAX_POOLS)
         for (int i0 = 0; i0 < n_pairs; i0 += EC_MAX_PAIRS) {
-            EntriesArgs a{};
+            EntriesArgs a;
             const int pools = n_pools - p0 < EC_MAX_POOLS ? n_pools - p0 : EC_MAX_POOLS;
             a.n_pairs = n_pairs - i0 < EC_MAX_PAIRS ? n_pairs - i0 : EC_MAX_PAIRS;
             for (int p = 0; p < pools; p++) a.pool[p] = pools_host[p0 + p];
-            for (int i = 0; i < a.n_pairs; i++) {
-                a.dst[i] = dst_host[i0 + i]; a.src[i] = src_host[i0 + i];
-                a.len[i] = len_host ? len_host[i0 + i] : sub_bytes;
-            }
+            memcpy(a.dst, dst_host + i0, a.n_pairs * sizeof(int));
+            memcpy(a.src, src_host + i0, a.n_pairs * sizeof(int));
+            a.per_pair = !same;
+            for (int i = 0; i < a.n_pairs && a.per_pair; i++) a.len[i] = (unsigned)(len_host[i0 + i] / 2);
             // whole entries are one run of bytes
-            a.entry_bytes = n_sub * sub_bytes; a.sub_bytes = sub_bytes; a.n_sub = n_sub;
-            if (!len_host) {
-                a.n_sub = 1; a.sub_bytes = a.entry_bytes;
-                for (int i = 0; i < a.n_pairs; i++) a.len[i] = a.entry_bytes;
-            }
-            const int rc = launch_entries_copy(a, pools, static_cast<cudaStream_t>(stream));
+            a.entry_bytes = n_sub * sub_bytes;
+            a.n_sub = whole ? 1 : n_sub;
+            a.sub_bytes = whole ? a.entry_bytes : sub_bytes;
+            a.len_all = whole ? a.entry_bytes : len_host[0];
+            rc = launch_entries_copy(a, pools, static_cast<cudaStream_t>(stream));
             if (rc) return rc;
         }
     return GDN_OK;

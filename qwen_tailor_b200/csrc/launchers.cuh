@@ -121,12 +121,14 @@ int launch_hrec(void* hist, const void* rows, const int* slots, const int* pos, 
 int launch_state_copy(void* dst, const void* src, int elem_size, long long n, long long d0, long long s0, int ny, long long dstride,
                       long long sstride, cudaStream_t st);
 
-constexpr int EC_MAX_POOLS = 64, EC_MAX_PAIRS = 160;              // per launch: the arguments fit the 4 KiB every launch may carry
+constexpr int EC_MAX_POOLS = 64, EC_MAX_PAIRS = 512;              // per launch (the arguments travel with it: 6.7 KiB)
 struct EntriesArgs {
     void* pool[EC_MAX_POOLS];
     int dst[EC_MAX_PAIRS], src[EC_MAX_PAIRS];
-    long long len[EC_MAX_PAIRS];      // bytes of each sub-block to copy
+    unsigned len[EC_MAX_PAIRS];       // bytes of each sub-block to copy, halved (`per_pair`), or
+    long long len_all;                // the same number of bytes for every pair
     long long entry_bytes, sub_bytes; // an entry = n_sub sub-blocks
+    bool per_pair;
     int n_sub, n_pairs;
 };
 int launch_entries_copy(const EntriesArgs& a, int n_pools, cudaStream_t st);

@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(EC_THREADS) entries_copy_kernel(const __grid_c
     const long long rest = blockIdx.x / a.n_pairs;
     const long long chunk = rest % chunks;
     const int sub = (int)(rest / chunks);
-    const long long len = a.len[pair] / (long long)sizeof(T);
+    const long long len = (a.per_pair ? 2ll * a.len[pair] : a.len_all) / (long long)sizeof(T);
     const long long i0 = chunk * (EC_THREADS * EC_PER) + threadIdx.x;
     if (i0 >= len) return;
     char* pool = static_cast<char*>(a.pool[blockIdx.y]);
@@ -95,11 +95,11 @@ __global__ void __launch_bounds__(EC_THREADS) entries_copy_kernel(const __grid_c
 }
 
 int launch_entries_copy(const EntriesArgs& a, int n_pools, cudaStream_t st) {
-    long long longest = 0;
-    bool vec = a.entry_bytes % 16 == 0 && a.sub_bytes % 16 == 0;
-    for (int i = 0; i < a.n_pairs; i++) {
-        longest = a.len[i] > longest ? a.len[i] : longest;
-        vec = vec && a.len[i] % 16 == 0;
+    long long longest = a.per_pair ? 0 : a.len_all;
+    bool vec = a.entry_bytes % 16 == 0 && a.sub_bytes % 16 == 0 && longest % 16 == 0;
+    for (int i = 0; i < a.n_pairs && a.per_pair; i++) {
+        longest = 2ll * a.len[i] > longest ? 2ll * a.len[i] : longest;
+        vec = vec && a.len[i] % 8 == 0;
     }
     for (int i = 0; i < n_pools; i++) vec = vec && reinterpret_cast<uintptr_t>(a.pool[i]) % 16 == 0;
     if (n_pools <= 0 || a.n_pairs <= 0 || longest <= 0) return GDN_OK;

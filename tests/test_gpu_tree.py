@@ -575,6 +575,24 @@ def test_copy_entries(dev, shape, dtype, rows, stacked):
     assert all(torch.equal(p, X) for p, X in zip(pools, want))
 
 
+@pytest.mark.parametrize("entries,n,rows", [(1400, 600, "each"), (20000, 1030, 3)])
+def test_copy_entries_beyond_one_launch(dev, entries, n, rows):
+    rng = np.random.default_rng(n)
+    order = rng.permutation(entries)
+    dst, src = order[:n], order[n:2 * n]
+    p = torch.randn(entries, 2, 4, 8, device=dev)
+    each = rng.integers(0, 5, n) if rows == "each" else np.full(n, rows)
+    want = p.cpu().clone()
+    for d, s, r in zip(dst, src, each):
+        want[d, :, :r] = want[s, :, :r]
+    copy_entries([p], dst.tolist(), src.tolist(), rows=each.tolist() if rows == "each" else rows)
+    assert torch.equal(p.cpu(), want)
+    for d, s in ((dst.tolist() + [int(dst[5])], src.tolist() + [int(src[5])]), (dst.tolist() + [int(src[7])], src.tolist() + [int(order[-1])])):
+        with pytest.raises(ValueError, match="entry"):
+            copy_entries([p], d, s)
+    assert torch.equal(p.cpu(), want)
+
+
 def test_copy_entries_refusals(dev):
     p = torch.zeros(6, 2, 4, 8, device=dev)
     copy_entries([p], [], [])
