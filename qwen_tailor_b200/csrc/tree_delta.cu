@@ -263,11 +263,13 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
                 for (int g = 0; g < GROUPS; g++) put(g, i0 + 8 * n, x[n][g]);
         }
     };
+    // (a warp's nodes are 8 apart, so the swizzle of its rows is one)
+    const uint32_t put_at = (lane >> 4) * C::SLAB + ((((lane >> 1) & 7) ^ warp) << 4) + (lane & 1) * 8;
     auto put_kq = [&](int row, const float (&x)[4]) {                // rows 0 .. NP - 1: K, then Q
         uint2 hi, lo;
         split_bf16(x[0], x[1], hi.x, lo.x);
         split_bf16(x[2], x[3], hi.y, lo.y);
-        const uint32_t at = (lane >> 4) * C::SLAB + row * 128 + ((((lane >> 1) & 7) ^ (row & 7)) << 4) + (lane & 1) * 8;
+        const uint32_t at = put_at + row * 128;
         *reinterpret_cast<uint2*>(smem + at) = hi;
         *reinterpret_cast<uint2*>(smem + 2 * C::SLAB + at) = lo;
     };
