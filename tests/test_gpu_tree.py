@@ -110,6 +110,33 @@ def test_attn_tree_peaked_scores_and_many_sequences(dev):
     assert _lib.device_status() == 0
 
 
+@pytest.mark.parametrize("B,N,page", [(80, 40, 64), (300, 3, 16)])
+def test_attn_tree_more_pairs_than_blocks(dev, B, N, page):
+    """80 sequences with two row tiles each (pairs are joined by the block they start in), and more sequences than one launch takes."""
+    rng = np.random.default_rng(B)
+    ctx = rng.integers(0, 150, B)
+    ctx[[0, B // 2, B - 1]] = [600, 0, 700]
+    c = attn_case(rng, ctx, N, page)
+    parents = np.stack([random_tree(rng, N, max(1, N - b % 3)) for b in range(B)])
+    d = to_dev(c, dev)
+    out = host(run_attn(d, i32_dev(parents, dev)))
+    check_attn(c, parents, out, host(d["k_pages"]), host(d["v_pages"]))
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("H,KV,N", [(32, 2, 64), (10, 2, 64), (24, 2, 50), (7, 1, 64), (13, 1, 37)])
+def test_attn_tree_row_tiles(dev, H, KV, N):
+    """Eight, three, five, four and five row tiles of a range side by side (5, 12, 7 and 13 heads on one leave rows of the tile empty)."""
+    rng = np.random.default_rng(H * N)
+    ctx = [140, 0, 2200]
+    c = attn_case(rng, ctx, N, 64, H, KV)
+    parents = np.stack([random_tree(rng, N, N - b) for b in range(3)])
+    d = to_dev(c, dev)
+    out = host(run_attn(d, i32_dev(parents, dev)))
+    check_attn(c, parents, out, host(d["k_pages"]), host(d["v_pages"]))
+    assert _lib.device_status() == 0
+
+
 @pytest.mark.parametrize("N", [3, 40])
 def test_attn_tree_nothing_leaks_from_masked_places(dev, N):
     """NaN and infinities behind the context in its last page, in unused pages, in unused nodes and in siblings change nothing where
@@ -669,4 +696,86 @@ def test_rounds_of_tree_speculation_on_paged_pools(dev):
     for s in seqs:
         pools.release(s)
     assert pools.pages.available() == pools.pages.n_pages - 1
+    assert _lib.device_status() == 0
+
+
+def test_a_round_captured_replayed_and_padded(dev):
+    """Verify, accept, commit and compaction in one captured graph, replayed on fresh contents: what eager calls give; idle rows of the batch (trash
+    slot, no nodes) change nothing; two such rounds on two streams do not disturb each other."""
+    rng = np.random.default_rng(91)
+    cfg = Cfg(layers=4)
+    nl, N, live, S = cfg.n_linear, 7, 3, 5
+    c = delta_case(rng, live, 1, S + 1, nl)
+    f = lambda *s: synth.bf16r(rng.standard_normal(s))  # noqa: E731
+    weights = list(bf16_dev(c["conv_w"], dev)), list(f32_dev(c["A_log"], dev)), list(f32_dev(c["dt_bias"], dev))
+    lengths = [61, 64, 3]
+
+    def fresh():
+        pools = PagedPools(cfg, S, 256, n_pages=20)
+        for l in range(nl):
+            pools.ssm[l].copy_(f32_dev(c["ssm"][l], dev))
+            pools.conv[l].copy_(bf16_dev(c["conv"][l], dev))
+        for X, Y in zip(pools.pages.K + pools.pages.V, kv):
+            X.copy_(Y)
+        for s in range(live):
+            pools.reserve(s, lengths[s] + N)
+        return pools
+
+    kv = [bf16_dev(f(20, 2, 64, 256), dev) for _ in range(2)]
+    rounds = []
+    for _ in range(2):
+        parents = np.stack([random_tree(rng, N, N - b) for b in range(live)])
+        rounds.append(dict(parents=parents, proj=f(nl, live * N, 8224), q=f(live * N, 8, 256), k=f(live * N, 2, 256), v=f(live * N, 2, 256),
+                           toks=rng.integers(0, 2, (live, N)), ids=rng.integers(0, 2, (live, N))))
+
+    def inputs(r, B):
+        pad = lambda x, n, fill: np.concatenate([x, np.full((n, *x.shape[1:]), fill, x.dtype)])  # noqa: E731
+        rows, seqs = (B - live) * N, B - live
+        return dict(parents=i32_dev(pad(r["parents"], seqs, -2), dev), toks=i32_dev(pad(r["toks"], seqs, 0), dev), ids=i32_dev(pad(r["ids"], seqs, 0), dev),
+                    q=bf16_dev(pad(r["q"], rows, np.nan), dev), k=bf16_dev(pad(r["k"], rows, np.nan), dev), v=bf16_dev(pad(r["v"], rows, np.nan), dev),
+                    projs=[bf16_dev(pad(x, rows, np.nan), dev) for x in r["proj"]], slots=i32_dev(list(range(live)) + [S] * seqs, dev), pos=i32_dev(lengths + [0] * seqs, dev))
+
+    def step(pools, i):
+        ys = [pools.deltanet_tree(l, i["projs"][l], weights[0][l], weights[1][l], weights[2][l], i["slots"], i["pos"], i["parents"]) for l in range(nl)]
+        o = pools.attn_tree(0, i["q"], i["k"], i["v"], i["slots"], i["pos"], i["parents"])
+        n_path, path = accept_tree(i["parents"], i["toks"], i["ids"])
+        pools.commit_tree(i["projs"], *weights, i["slots"], i["pos"], path, n_path)
+        return [*ys, o, n_path, path]
+
+    caches = lambda pools: [*pools.ssm, *pools.conv, *pools.pages.K, *pools.pages.V]  # noqa: E731
+    start = [x.clone() for x in caches(fresh())]
+    want = []
+    for r in rounds:
+        pools = fresh()
+        out = step(pools, inputs(r, live))
+        want.append((out, [x.clone() for x in caches(pools)]))
+    assert _lib.device_status() == 0
+
+    B = live + 2
+    per_round = []
+    for r in rounds:                                                 # one graph per round, pools and inputs of its own
+        pools, i = fresh(), inputs(r, B)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(pools, i)
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(pools, i)
+        per_round.append((g, pools, out, torch.cuda.Stream(), i))    # (a graph does not keep its inputs alive)
+    for _ in range(3):
+        for g, pools, _, _, _ in per_round:
+            for x, x0 in zip(caches(pools), start):
+                x.copy_(x0)
+        torch.cuda.synchronize()
+        for g, _, _, stream, _ in per_round:                            # both at once
+            with torch.cuda.stream(stream):
+                g.replay()
+        torch.cuda.synchronize()
+        for (g, pools, out, _, _), (ref, after) in zip(per_round, want):
+            for x, y in zip(out, ref):
+                assert torch.equal(x[:len(y)], y) and not (x[len(y):].float() * (x[len(y):] != -1)).any(), "idle rows: zeros, and -1 in the path"
+            for x, y in zip(caches(pools), after):
+                assert torch.equal(x, y)
     assert _lib.device_status() == 0
