@@ -726,17 +726,21 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
     GDN_BSTAMP(9);
 }
 
-// Joins the partials of a cut pair (blockIdx.x: the pair, or the main block that it starts in): eight rows per block, a thread holds four columns of a row.
-// Bound: latency (a few hundred KiB out of L2), so what a block needs is requested at once.  Sixteen partials in flight a thread leave room for
-// one block per SM, six for two: 16 sequences (about 5 partials a pair) 43 us with six, 46 with sixteen; 2 sequences (18 a pair) 98.5 and
-// 95.6, 9 sequences (8 a pair) 27.5 and 25.7.
-constexpr int TM_ROWS = 8, TM_THREADS = 64 * TM_ROWS;
+// Joins the partials of a cut pair (blockIdx.x: the pair, or the main block that it starts in): a thread holds four columns of a row, or of every
+// 2nd or 4th partial of it.  Bound: latency (a few hundred KiB out of L2), so what a block needs is requested at once, and where rows are few
+// several threads share one: one sequence with 16 k cached tokens and 16 nodes 36 -> 28 us (74 partials a pair, four threads a row), with 64
+// nodes 37.5 -> 33.3, four sequences with 8 k 31.3 -> 28.3 (two threads a row).  Sixteen partials in flight a thread leave room for one block
+// per SM, six for two: 16 sequences (about 5 partials a pair) 43 us with six, 46 with sixteen; 2 sequences x 64 nodes (18 a pair) 98.5 and 95.6,
+// 9 sequences (8 a pair) 27.5 and 25.7.
+constexpr int TM_THREADS = 512;
 constexpr int TM_FEW = 6, TM_MANY = 16;                              // partials requested at once where pairs have few of them, and many
 
-template <int AHEAD>
+template <int ROWS, int AHEAD>
 __global__ void __launch_bounds__(TM_THREADS) tree_attn_merge_kernel(const __grid_constant__ TreeAttnPlan p) {
-    __shared__ float s_w[148][TM_ROWS], s_l[148][TM_ROWS];
-    __shared__ unsigned char s_live[TM_ROWS];
+    constexpr int GROUPS = TM_THREADS / (64 * ROWS);                 // threads that share a row's columns: each takes every GROUPS-th partial
+    __shared__ float s_w[148][ROWS], s_l[148][ROWS];
+    __shared__ unsigned char s_live[ROWS];
+    __shared__ float4 s_acc[GROUPS][64 * ROWS];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int2 info = *reinterpret_cast<const int2*>(p.info + 2 * blockIdx.x);
@@ -744,7 +748,7 @@ __global__ void __launch_bounds__(TM_THREADS) tree_attn_merge_kernel(const __gri
     GDN_BSTAMP(10);
     if (parts == 0) return;
     const TreeAttnArgs& a = p.a;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = tid & (TM_ROWS - 1), row = blockIdx.y * TM_ROWS + r, cg = tid / TM_ROWS;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = tid & (ROWS - 1), row = blockIdx.y * ROWS + r, cg = tid / ROWS % 64, grp = tid / (64 * ROWS);
     const bool in = row < p.rows;
     auto slot = [&](int k) -> size_t { return 2 * (first + k * p.row_tiles) + (k == 0 ? 1 : 0); };
     // (requested at once: the rows' (m, l), the first partials and the tree; a dependent round trip to L2 costs most of a microsecond)
@@ -753,24 +757,24 @@ __global__ void __launch_bounds__(TM_THREADS) tree_attn_merge_kernel(const __gri
     float4 o[AHEAD];
 #pragma unroll
     for (int k = 0; k < AHEAD; k++)
-        if (in && k < parts) o[k] = __ldcg(part + slot(k) * step);
-    for (int k = cg; k < parts; k += TM_THREADS / TM_ROWS) {
+        if (in && grp + k * GROUPS < parts) o[k] = __ldcg(part + slot(grp + k * GROUPS) * step);
+    for (int k = tid / ROWS; k < parts; k += TM_THREADS / ROWS) {
         const float2 ml = in ? __ldcg(reinterpret_cast<const float2*>(p.part_ml + (slot(k) * p.rows + row) * 2)) : make_float2(-INFINITY, 0.f);
         s_w[k][r] = ml.x;
         s_l[k][r] = ml.y;
     }
     const int rt = pair % p.row_tiles, kvh = pair / p.row_tiles % a.KV, b = pair / p.row_tiles / a.KV;
-    if (warp == TM_ROWS) {                                           // which of the rows belong to nodes in use
+    if (warp == 8) {                                                 // which of the rows belong to nodes in use
         unsigned long long l0, l1;
         bool bad;
         const int* par = a.parents + (size_t)b * a.N;
         warp_lines(lane < a.N ? par[lane] : -2, lane + 32 < a.N ? par[lane + 32] : -2, l0, l1, bad);
-        const int node = rt * p.nodes + (blockIdx.y * TM_ROWS + (lane & (TM_ROWS - 1))) / p.group;
+        const int node = rt * p.nodes + (blockIdx.y * ROWS + (lane & (ROWS - 1))) / p.group;
         const unsigned long long x0 = shfl64(l0, node & 31), x1 = shfl64(l1, node & 31);
-        if (lane < TM_ROWS) s_live[lane] = node < a.N && (node < 32 ? x0 : x1) != 0;
+        if (lane < ROWS) s_live[lane] = node < a.N && (node < 32 ? x0 : x1) != 0;
     }
     __syncthreads();
-    if (warp < TM_ROWS) {                                            // the row's common maximum; weights over the row's sum
+    if (warp < ROWS) {                                               // the row's common maximum; weights over the row's sum
         float mx = -INFINITY, sum = 0.f;
         for (int k = lane; k < parts; k += 32) mx = fmaxf(mx, s_w[k][warp]);
 #pragma unroll
@@ -785,17 +789,25 @@ __global__ void __launch_bounds__(TM_THREADS) tree_attn_merge_kernel(const __gri
         for (int k = lane; k < parts; k += 32) s_w[k][warp] *= inv;
     }
     __syncthreads();
-    const int node = rt * p.nodes + row / p.group;
-    if (!in || node >= a.N) return;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     auto add = [&](float w, float4 x) {
         acc.x = fmaf(w, x.x, acc.x); acc.y = fmaf(w, x.y, acc.y); acc.z = fmaf(w, x.z, acc.z); acc.w = fmaf(w, x.w, acc.w);
     };
 #pragma unroll
     for (int k = 0; k < AHEAD; k++)
-        if (k < parts) add(s_w[k][r], o[k]);
+        if (in && grp + k * GROUPS < parts) add(s_w[grp + k * GROUPS][r], o[k]);
+    if (in)
 #pragma unroll (AHEAD / 2)
-    for (int k = AHEAD; k < parts; k++) add(s_w[k][r], __ldcg(part + slot(k) * step));
+        for (int k = grp + AHEAD * GROUPS; k < parts; k += GROUPS) add(s_w[k][r], __ldcg(part + slot(k) * step));
+    if (GROUPS > 1) {
+        s_acc[grp][cg * ROWS + r] = acc;
+        __syncthreads();
+        if (grp > 0) return;
+#pragma unroll
+        for (int g = 1; g < GROUPS; g++) add(1.f, s_acc[g][cg * ROWS + r]);
+    }
+    const int node = rt * p.nodes + row / p.group;
+    if (!in || node >= a.N) return;
     const uint2 v = s_live[r] ? make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w)) : make_uint2(0, 0);
     *reinterpret_cast<uint2*>(a.out + (((size_t)b * a.N + node) * a.H + kvh * p.group + row % p.group) * ATT_D + 4 * cg) = v;
     GDN_BSTAMP(11);
@@ -914,9 +926,12 @@ int launch_tree_attn(const TreeAttnArgs& all, void* workspace, size_t workspace_
         int rc = launch_pdl((const void*)tree_attn_kernel, dim3(p.G), TA_THREADS, TA_SMEM, st, args);
         if (rc) return rc;
         void* margs[] = {&p};
-        // (the mean number of partials of a pair)
-        const bool few = p.G <= TM_FEW * pairs;
-        rc = launch_pdl(few ? (const void*)tree_attn_merge_kernel<TM_FEW> : (const void*)tree_attn_merge_kernel<TM_MANY>, dim3(p.by_pair ? pairs : p.G, (p.rows + TM_ROWS - 1) / TM_ROWS), TM_THREADS, 0, st, margs);
+        // as few rows a block as leave it an SM of its own; with eight, by the mean number of partials of a pair
+        const int eights = pairs * ((p.rows + 7) / 8), rows = eights * 4 <= p.G ? 2 : eights * 2 <= p.G ? 4 : 8;
+        const void* merge = rows == 2 ? (const void*)tree_attn_merge_kernel<2, TM_MANY>
+                            : rows == 4 ? (const void*)tree_attn_merge_kernel<4, TM_MANY>
+                            : p.G > TM_FEW * pairs ? (const void*)tree_attn_merge_kernel<8, TM_MANY> : (const void*)tree_attn_merge_kernel<8, TM_FEW>;
+        rc = launch_pdl(merge, dim3(p.by_pair ? pairs : p.G, (p.rows + rows - 1) / rows), TM_THREADS, 0, st, margs);
         if (rc) return rc;
     }
     return GDN_OK;
