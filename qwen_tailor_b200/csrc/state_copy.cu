@@ -69,7 +69,8 @@ int launch_hrec(void* hist, const void* rows, const int* slots, const int* pos, 
 // states, conv windows).  An entry is n_sub sub-blocks of sub_bytes; the first `len` bytes of each are copied (len is per pair: the
 // filled rows of a page).  Pool pointers and pairs travel as kernel arguments, so nothing is uploaded and a call can be captured.
 // Bound: HBM (every byte once in, once out).  A block moves one 16 KiB chunk with four independent 16-byte accesses per thread; the
-// pairs are the fastest index of the grid, so that the copies of one source (a fork) find its chunk in L2.
+// pairs are the fastest index of the grid, so that the copies of one source (a fork) find its chunk in L2.  300 pages in 12 pools 74 us
+// (6.4 TB/s read and write); a slot's states, windows and last pages into seven others, three launches, 31 us.
 // ----------------------------------------------------------------------------------------------------------------------
 constexpr int EC_THREADS = 256, EC_PER = 4;
 
@@ -118,7 +119,7 @@ int launch_entries_copy(const EntriesArgs& a, int n_pools, cudaStream_t st) {
 // and head.  keep is strictly ascending, so keep[j] >= j and a row is only ever overwritten after it was read: a thread owns a
 // 16-byte column of a (pool, sequence, head) and walks the rows in order, eight loads in flight before their eight stores.  Bound:
 // latency (a round keeps a handful of rows); the index words of 32 rows are fetched by the 32 lanes at once, so that the dependent
-// chain is keep -> page -> row whatever the number of rows.
+// chain is keep -> page -> row whatever the number of rows.  24 sequences, 12 pools, one to seven rows: 3.0 us.
 // ----------------------------------------------------------------------------------------------------------------------
 constexpr int RC_WARPS = 4, RC_ROWS = 8;
 
