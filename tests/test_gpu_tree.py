@@ -779,3 +779,46 @@ def test_a_round_captured_replayed_and_padded(dev):
             for x, y in zip(caches(pools), after):
                 assert torch.equal(x, y)
     assert _lib.device_status() == 0
+
+
+def test_pools_beyond_32_bit_offsets(dev):
+    """Pages and slots that lie more than 2^31 elements into their pools give what the same contents give at the front."""
+    rng = np.random.default_rng(5)
+    c = attn_case(rng, [300, 64], 20, 64)
+    parents = i32_dev(np.stack([random_tree(rng, 20) for _ in range(2)]), dev)
+    d = to_dev(c, dev)
+    near = run_attn(d, parents)
+    used = c["k_pages"].shape[0]
+    total = 2 ** 31 // (2 * 64 * 256) + used + 1                     # the last `used` pages start behind element 2^31
+    K, V = (torch.empty(total, 2, 64, 256, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    first = total - used
+    for X, name in ((K, "k_pages"), (V, "v_pages")):
+        X[first:] = bf16_dev(c[name], dev)
+    table = d["table"] + first
+    assert torch.equal(attn_tree(d["q"], d["k_new"], d["v_new"], K, V, table, d["ctx"], parents), near)
+    assert torch.equal(K[first:], d["k_pages"]) and torch.equal(V[first:], d["v_pages"]), "the appended rows too"
+    keep, n_keep = i32_dev([[0, 3, 7, 19], [1, 2, 5, 6]], dev), i32_dev([4, 3], dev)
+    compact_rows([d["k_pages"], d["v_pages"]], d["table"], d["ctx"], keep, n_keep)
+    compact_rows([K, V], table, d["ctx"], keep, n_keep)
+    assert torch.equal(K[first:], d["k_pages"]) and torch.equal(V[first:], d["v_pages"])
+    copy_entries([K, V], [0, total - 1], [first + 1, 1], rows=33)
+    assert torch.equal(K[0, :, :33], K[first + 1, :, :33]) and torch.equal(V[total - 1, :, :33], V[1, :, :33])
+    del K, V
+
+    c = delta_case(rng, 2, 9, 2)
+    c["slots"][:] = [0, 1]
+    d = delta_dev(c, dev)
+    parents = i32_dev(np.stack([random_tree(rng, 9) for _ in range(2)]), dev)
+    path, n = i32_dev([[0, 1, 4], [0, 2, -1]], dev), i32_dev([3, 2], dev)
+    far = 2 ** 31 // (16 * 128 * 128) + 1
+    ssm = torch.empty(1, far + 5, 16, 128, 128, device=dev)
+    conv = torch.empty(1, 2 * (far + 5), 3, 6144, dtype=torch.bfloat16, device=dev)
+    ssm[:, far:far + 2], conv[:, 2 * far:2 * far + 4] = d["ssm"], d["conv"]
+    e = {**d, "ssm": ssm, "conv": conv, "slots": d["slots"] + far}
+    assert torch.equal(run_delta(e, parents), run_delta(d, parents))
+    for x in (d, e):
+        deltanet_commit(x["proj"], x["conv"], x["conv_w"], x["A_log"], x["dt_bias"], x["ssm"], x["slots"], x["pos"], path, n)
+    assert torch.equal(ssm[:, far:far + 2], d["ssm"]) and torch.equal(conv[:, 2 * far:2 * far + 4], d["conv"])
+    copy_entries([ssm], [far + 3], [far + 1], stacked=True)
+    assert torch.equal(ssm[0, far + 3], ssm[0, far + 1])
+    assert _lib.device_status() == 0
