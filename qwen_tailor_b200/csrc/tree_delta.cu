@@ -41,15 +41,17 @@ __device__ __forceinline__ unsigned long long tree_line(const int* par, int i, b
 
 // ----------------------------------------------------------------------------------------------------------------------
 // verify: one block per (sequence, head), two blocks per SM.  NP = nodes padded to 16, 32 or 64.  Bound: issue slots and latency
-// (46 k warp instructions a head at 64 nodes, half of the slots used; the state alone would take a quarter of the time).  Measured: 64 sequences
-// x 64 nodes 90 us, 16 x 27 14.5 us, one sequence x 8 nodes 8.2 us.
+// (some 40 k warp instructions a head at 64 nodes, half of the slots used; the state alone would take a quarter of the time).  Measured: 64
+// sequences x 64 nodes 86 us, 16 x 27 14.4 us, one sequence x 8 nodes 8.0 us.
 //     [P1 | P2] = S0 [K; Q]^T     on the tensor cores, rows = value rows d: S0 in tensor memory, [K; Q] in shared memory
 //     G         = [K; Q] K^T      on the tensor cores
 // each operand as bf16 hi + lo and the three products that matter (what is dropped is 2^-16 of the factors; K and Q rounded to bf16
 // alone would put an error of the size of y's own rounding on every product).  The rest is fp32: thread d of four warps solves
 //     u_i = beta_i (v_i - e^G_i P1_i) - sum_j L_ij u_j
-// for its value row in blocks of 16 nodes, thread d of the other four follows with y_i = e^G_i P2_i + sum_j A_ij u_j.  L and A are
-// dense with zeros outside the ancestors; zeros do not stop NaN, so a head with a non-finite q, k, v or gate takes the sums over the
+// for its value row in blocks of 16 nodes.  Up to 32 nodes thread d of the other four follows a block behind with
+//     y_i = e^G_i P2_i + sum_j A_ij u_j;
+// with 64 this sum is another product, u and A as hi + lo (86 us against 90; the product's latency is what fewer nodes would add).  L and A
+// are dense with zeros outside the ancestors; zeros do not stop NaN, so a head with a non-finite q, k, v or gate takes the sums over the
 // ancestors one by one instead.
 // M_ij is 2 to the difference of two sums G, which can be far larger than their difference (a path through tokens that wipe the state out).
 // G is summed in 64 bits and split into hi = fp32(G) and lo; with u'_i = 2^-lo_i u_i in place of u the solve needs 2^(hi_i - hi_j) only, and
@@ -68,6 +70,8 @@ template <int NP> struct TreeVerify {
     static constexpr int ST_BYTES = 65536 / HALVES;
     static constexpr int SMEM = KQ_BYTES + ST_BYTES + DV * 4;        // + a row of zeros behind the last u
     static constexpr uint32_t TM_HI = 0, TM_LO = 64, TM_P = 128, TM_G = 0;       // G replaces S0 (products of one thread run in order)
+    static constexpr bool Y_MMA = NP == 64;                          // y's sums on the tensor cores
+    static constexpr uint32_t TM_UHI = 0, TM_ULO = 32, TM_Y = 64;    // u and y replace G and the rest of S0
 };
 
 __device__ __forceinline__ void split_bf16(float x, float y, uint32_t& hi, uint32_t& lo) {
@@ -82,6 +86,11 @@ __device__ __forceinline__ float2 unpack2(f32x2 v) { float2 r; asm("mov.b64 {%0,
 __device__ __forceinline__ void fma2(f32x2& x, f32x2 a, f32x2 b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(x) : "l"(a), "l"(b)); }
 // the fast approximations of exp and of the division are good to a few fp32 ulp, far below y's rounding to bf16
 __device__ __forceinline__ float silu_fast(float x) { return __fdividef(x, 1.f + __expf(-x)); }
+
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
 
 template <int NP>
 __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDeltaArgs a, const __grid_constant__ CUtensorMap tmS) {
@@ -346,28 +355,49 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
         const unsigned long long line = isq ? s_line[i] : s_line[i] & ~(1ull << i);
         const float g = s_G[i], mul = isq ? s_up[i] : s_beta[i];
         float* dst = (isq ? sA : sL) + i;
+        unsigned char* arow = reinterpret_cast<unsigned char*>(sA) + i * 128;        // Y_MMA: A's rows as operand images, hi and (8 KiB on) lo
         for (int j0 = (warp >> 2) * 16; j0 < NP; j0 += 32) {
             uint32_t r[16];
             tmem_ld16(tl + C::TM_G + j0, r);
             tmem_wait_ld();
             const uint32_t on = (uint32_t)(line >> j0);
+            float m[16];
 #pragma unroll
             for (int c = 0; c < 16; c++) {
                 float e;
                 asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g - s_G[j0 + c]));
-                dst[(j0 + c) * NP] = on >> c & 1 ? mul * e * __uint_as_float(r[c]) : 0.f;
+                m[c] = on >> c & 1 ? mul * e * __uint_as_float(r[c]) : 0.f;
+            }
+            if (C::Y_MMA && isq) {
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    uint4 hi, lo;
+                    split_bf16(m[8 * q], m[8 * q + 1], hi.x, lo.x);
+                    split_bf16(m[8 * q + 2], m[8 * q + 3], hi.y, lo.y);
+                    split_bf16(m[8 * q + 4], m[8 * q + 5], hi.z, lo.z);
+                    split_bf16(m[8 * q + 6], m[8 * q + 7], hi.w, lo.w);
+                    const int at = ((j0 / 8 + q) ^ (i & 7)) << 4;
+                    *reinterpret_cast<uint4*>(arow + at) = hi;
+                    *reinterpret_cast<uint4*>(arow + 8192 + at) = lo;
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < 16; c++) dst[(j0 + c) * NP] = m[c];
             }
         }
     }
+    if (C::Y_MMA) fence_proxy_async_smem();
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
     GDN_BSTAMP(7);
     const bool solver = warp < 4;
     __nv_bfloat16* out = a.y + (size_t)b * N * KD + h * DV + d;
-    if (!s_odd) {
+    const bool plain = !s_odd;
+    if (plain) {
 #pragma unroll 1
         for (int I = 0; I < NP / 16; I++) {
+            if (C::Y_MMA && !solver) break;
             f32x2 x[8];                                              // nodes 16 I + 2 k, + 1
             {
                 uint32_t r[16];
@@ -409,10 +439,12 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
                 for (int q = 0; q < 4; q++) add(js >> 8 * q & 255, u[q]);
             }
             if (solver) {
+                float us[16];
 #pragma unroll
                 for (int c = 0; c < 16; c++) {                       // (entries up to c are zero)
                     const float2 p = unpack2(x[c / 2]);
                     const float u = c & 1 ? p.y : p.x;
+                    us[c] = u;
                     su[(16 * I + c) * DV + d] = u;
                     const f32x2 uu = pack2(-u, -u);
                     const ulonglong2* row = reinterpret_cast<const ulonglong2*>(coef + (16 * I + c) * NP);
@@ -423,8 +455,16 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
                         if (4 * q + 3 > c) fma2(x[2 * q + 1], m.y, uu);
                     }
                 }
-                __threadfence_block();
-                asm volatile("bar.arrive %0, 256;" ::"r"(1 + I) : "memory");
+                if (C::Y_MMA) {
+                    uint32_t hi[8], lo[8];
+#pragma unroll
+                    for (int q = 0; q < 8; q++) split_bf16(us[2 * q], us[2 * q + 1], hi[q], lo[q]);
+                    tmem_st8(tl + C::TM_UHI + 8 * I, hi);
+                    tmem_st8(tl + C::TM_ULO + 8 * I, lo);
+                } else {
+                    __threadfence_block();
+                    asm volatile("bar.arrive %0, 256;" ::"r"(1 + I) : "memory");
+                }
             } else {
                 asm volatile("bar.sync %0, 256;" ::"r"(1 + I) : "memory");
 #pragma unroll
@@ -447,7 +487,50 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
                 }
             }
         }
+        if constexpr (C::Y_MMA) {
+            // y = e^G P2 + U A^T, rows = value rows: u as hi + lo out of tensor memory, A as hi + lo out of shared memory
+            float f[32];
+            const int i0 = 32 * (warp >> 2);
+            {
+                uint32_t r[32];
+                tmem_ld32(tl + C::TM_P + NP + i0, r);
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 32; c++) f[c] = s_grow[i0 + c] * __uint_as_float(r[c]);
+            }
+            tmem_wait_st();
+            tc_fence_before_sync();
+            __syncthreads();
+            if (tid == TV_THREADS - 32) {
+                tc_fence_after_sync();
+                constexpr uint32_t HI = smem_desc_hi_sw128(1024), I_Y = idesc_bf16(128, NP, 0, 0);
+                const uint32_t ah = smem_desc_lo(sKQ + NP * NP * 4, 16), al = ah + (8192 >> 4);
+#pragma unroll
+                for (int ks = 0; ks < NP / 16; ks++) {
+                    if (ks == 0) mma_ts_w<false>(tb + C::TM_Y, tb + C::TM_UHI, ah, HI, I_Y);
+                    else mma_ts_w<true>(tb + C::TM_Y, tb + C::TM_UHI + 8 * ks, ah + 2 * ks, HI, I_Y);
+                    mma_ts_w<true>(tb + C::TM_Y, tb + C::TM_UHI + 8 * ks, al + 2 * ks, HI, I_Y);
+                    mma_ts_w<true>(tb + C::TM_Y, tb + C::TM_ULO + 8 * ks, ah + 2 * ks, HI, I_Y);
+                }
+                mma_commit(b_mma);
+            }
+            if (!mbar_wait(b_mma, 1)) { s_fail = 1; atomicExch(a.status, 2); }
+            tc_fence_after_sync();
+            uint32_t r[32];
+            tmem_ld32(tl + C::TM_Y + i0, r);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 32; c++)
+                if (i0 + c < N) out[(size_t)(i0 + c) * KD] = __float2bfloat16_rn(f[c] + __uint_as_float(r[c]));
+        }
     } else if (solver) {
+        // A's entries: as they are, or from their operand images (of a non-finite one hi alone)
+        auto coef_a = [&](int j, int i) -> float {
+            if (!C::Y_MMA) return sA[j * NP + i];
+            const unsigned char* at = reinterpret_cast<const unsigned char*>(sA) + i * 128 + (((j >> 3) ^ (i & 7)) << 4) + (j & 7) * 2;
+            const float hi = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(at)), lo = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(at + 8192));
+            return isfinite(hi) ? hi + lo : hi;
+        };
         // a non-finite value somewhere: only what lies on a node's own path enters its sums
         for (int i0 = 0; i0 < NP; i0 += 16) {
             uint32_t r1[16], r2[16];
@@ -465,9 +548,9 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
                 for (unsigned long long m = line & ~(1ull << i); m; m &= m - 1) {
                     const int j = __ffsll((long long)m) - 1;
                     u = fmaf(-sL[j * NP + i], su[j * DV + d], u);
-                    y = fmaf(sA[j * NP + i], su[j * DV + d], y);
+                    y = fmaf(coef_a(j, i), su[j * DV + d], y);
                 }
-                y = fmaf(sA[i * NP + i], u, y);
+                y = fmaf(coef_a(i, i), u, y);
                 su[i * DV + d] = u;                                  // (column d is this thread's)
                 out[(size_t)i * KD] = __float2bfloat16_rn(line ? y : 0.f);
             }
@@ -477,7 +560,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
     tc_fence_before_sync();
     __syncthreads();
     GDN_BSTAMP(9);
-    if (s_fail && tid == 0) { mbar_wait(b_state, C::HALVES - 1, 100000u); mbar_wait(b_mma, 0, 100000u); }      // copies and products in flight end first
+    if (s_fail && tid == 0) { mbar_wait(b_state, C::HALVES - 1, 100000u); mbar_wait(b_mma, C::Y_MMA && plain ? 1 : 0, 100000u); }      // copies and products in flight end first
     __syncthreads();
     if (warp == 7) tmem_dealloc(tb, 256);
 }
