@@ -48,10 +48,10 @@ __device__ __forceinline__ unsigned long long tree_line(const int* par, int i, b
 // each operand as bf16 hi + lo and the three products that matter (what is dropped is 2^-16 of the factors; K and Q rounded to bf16
 // alone would put an error of the size of y's own rounding on every product).  The rest is fp32: thread d of four warps solves
 //     u_i = beta_i (v_i - e^G_i P1_i) - sum_j L_ij u_j
-// for its value row in blocks of 16 nodes.  Up to 32 nodes thread d of the other four follows a block behind with
+// for its value row in blocks of 16 nodes.  Up to 16 nodes thread d of the other four follows with
 //     y_i = e^G_i P2_i + sum_j A_ij u_j;
-// with 64 this sum is another product, u and A as hi + lo (86 us against 90; the product's latency is what fewer nodes would add).  L and A
-// are dense with zeros outside the ancestors; zeros do not stop NaN, so a head with a non-finite q, k, v or gate takes the sums over the
+// with more, where it would follow block by block, this sum is another product, u and A as hi + lo (64 sequences x 64 nodes 86 us against
+// 90, x 32 nodes 52.8 against 54.1, one sequence x 32 nodes 11.1 either way).  L and A are dense with zeros outside the ancestors; zeros do not stop NaN, so a head with a non-finite q, k, v or gate takes the sums over the
 // ancestors one by one instead.
 // M_ij is 2 to the difference of two sums G, which can be far larger than their difference (a path through tokens that wipe the state out).
 // G is summed in 64 bits and split into hi = fp32(G) and lo; with u'_i = 2^-lo_i u_i in place of u the solve needs 2^(hi_i - hi_j) only, and
@@ -70,7 +70,8 @@ template <int NP> struct TreeVerify {
     static constexpr int ST_BYTES = 65536 / HALVES;
     static constexpr int SMEM = KQ_BYTES + ST_BYTES + DV * 4;        // + a row of zeros behind the last u
     static constexpr uint32_t TM_HI = 0, TM_LO = 64, TM_P = 128, TM_G = 0;       // G replaces S0 (products of one thread run in order)
-    static constexpr bool Y_MMA = NP == 64;                          // y's sums on the tensor cores
+    static constexpr bool Y_MMA = NP >= 32;                          // y's sums on the tensor cores
+    static constexpr int A_LO = NP * 128;                            // (A as operand: hi, then lo)
     static constexpr uint32_t TM_UHI = 0, TM_ULO = 32, TM_Y = 64;    // u and y replace G and the rest of S0
 };
 
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
         const unsigned long long line = isq ? s_line[i] : s_line[i] & ~(1ull << i);
         const float g = s_G[i], mul = isq ? s_up[i] : s_beta[i];
         float* dst = (isq ? sA : sL) + i;
-        unsigned char* arow = reinterpret_cast<unsigned char*>(sA) + i * 128;        // Y_MMA: A's rows as operand images, hi and (8 KiB on) lo
+        unsigned char* arow = reinterpret_cast<unsigned char*>(sA) + i * 128;        // Y_MMA: A's rows as operand images, hi and lo
         for (int j0 = (warp >> 2) * 16; j0 < NP; j0 += 32) {
             uint32_t r[16];
             tmem_ld16(tl + C::TM_G + j0, r);
@@ -378,7 +379,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
                     split_bf16(m[8 * q + 6], m[8 * q + 7], hi.w, lo.w);
                     const int at = ((j0 / 8 + q) ^ (i & 7)) << 4;
                     *reinterpret_cast<uint4*>(arow + at) = hi;
-                    *reinterpret_cast<uint4*>(arow + 8192 + at) = lo;
+                    *reinterpret_cast<uint4*>(arow + C::A_LO + at) = lo;
                 }
             } else {
 #pragma unroll
@@ -489,22 +490,25 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
         }
         if constexpr (C::Y_MMA) {
             // y = e^G P2 + U A^T, rows = value rows: u as hi + lo out of tensor memory, A as hi + lo out of shared memory
-            float f[32];
-            const int i0 = 32 * (warp >> 2);
-            {
-                uint32_t r[32];
-                tmem_ld32(tl + C::TM_P + NP + i0, r);
+            constexpr int MINE = NP / 2;                             // nodes whose y this warp's group writes
+            auto load = [&](uint32_t col, uint32_t (&r)[MINE]) {
+                if constexpr (MINE == 32) tmem_ld32(tl + col, r);
+                else tmem_ld16(tl + col, r);
                 tmem_wait_ld();
+            };
+            float f[MINE];
+            uint32_t r[MINE];
+            const int i0 = MINE * (warp >> 2);
+            load(C::TM_P + NP + i0, r);
 #pragma unroll
-                for (int c = 0; c < 32; c++) f[c] = s_grow[i0 + c] * __uint_as_float(r[c]);
-            }
+            for (int c = 0; c < MINE; c++) f[c] = s_grow[i0 + c] * __uint_as_float(r[c]);
             tmem_wait_st();
             tc_fence_before_sync();
             __syncthreads();
             if (tid == TV_THREADS - 32) {
                 tc_fence_after_sync();
                 constexpr uint32_t HI = smem_desc_hi_sw128(1024), I_Y = idesc_bf16(128, NP, 0, 0);
-                const uint32_t ah = smem_desc_lo(sKQ + NP * NP * 4, 16), al = ah + (8192 >> 4);
+                const uint32_t ah = smem_desc_lo(sKQ + NP * NP * 4, 16), al = ah + (C::A_LO >> 4);
 #pragma unroll
                 for (int ks = 0; ks < NP / 16; ks++) {
                     if (ks == 0) mma_ts_w<false>(tb + C::TM_Y, tb + C::TM_UHI, ah, HI, I_Y);
@@ -516,11 +520,9 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
             }
             if (!mbar_wait(b_mma, 1)) { s_fail = 1; atomicExch(a.status, 2); }
             tc_fence_after_sync();
-            uint32_t r[32];
-            tmem_ld32(tl + C::TM_Y + i0, r);
-            tmem_wait_ld();
+            load(C::TM_Y + i0, r);
 #pragma unroll
-            for (int c = 0; c < 32; c++)
+            for (int c = 0; c < MINE; c++)
                 if (i0 + c < N) out[(size_t)(i0 + c) * KD] = __float2bfloat16_rn(f[c] + __uint_as_float(r[c]));
         }
     } else if (solver) {
@@ -528,7 +530,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
         auto coef_a = [&](int j, int i) -> float {
             if (!C::Y_MMA) return sA[j * NP + i];
             const unsigned char* at = reinterpret_cast<const unsigned char*>(sA) + i * 128 + (((j >> 3) ^ (i & 7)) << 4) + (j & 7) * 2;
-            const float hi = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(at)), lo = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(at + 8192));
+            const float hi = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(at)), lo = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(at + C::A_LO));
             return isfinite(hi) ? hi + lo : hi;
         };
         // a non-finite value somewhere: only what lies on a node's own path enters its sums
