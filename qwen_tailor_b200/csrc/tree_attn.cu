@@ -610,6 +610,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                         tmem_wait_st();
                     }
                 }
+                __syncwarp();                                        // (each lane chose its own factor; tensor-memory accesses take a converged warp)
                 // p = 2^(s sc - m) (a masked score gives 0) as bf16 hi + lo, written over the scores group by group: the 32 score
                 // columns of keys 32 g .. 32 g + 31 become 16 columns of hi pairs and 16 columns of lo pairs
                 const float nm = (m_run == -INFINITY) ? 0.f : -m_run;
@@ -671,6 +672,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
 #pragma unroll 1
             for (int c0 = 0; c0 < 256; c0 += 32) {
                 uint32_t u[32];
+                __syncwarp();                                        // (rows add and store different things below; the load takes a converged warp)
                 tmem_ld32(tl + TAM_O + c0, u);
                 tmem_wait_ld();
                 if (add) {
@@ -722,7 +724,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
     if (tid == 0 && aborted()) clear_info();
     tc_fence_before_sync();
     __syncthreads();
-    if (warp == 4) tmem_dealloc(tb, 512);
+    if (warp == 4) { __syncwarp(); tmem_dealloc(tb, 512); }          // (one lane of it was the issuer)
     GDN_BSTAMP(9);
 }
 

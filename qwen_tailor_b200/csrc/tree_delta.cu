@@ -147,7 +147,8 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
         fence_barrier_init();
         load_state(0);
     }
-    if (warp == 7) { tmem_alloc(smem_addr(&s_tmem), 256); tmem_relinquish(); }
+    // (tensor memory is allocated, read and written by converged warps: wherever lanes may have parted before, they meet first)
+    if (warp == 7) { __syncwarp(); tmem_alloc(smem_addr(&s_tmem), 256); tmem_relinquish(); }
     if (tid < NP) { s_par[tid] = par; s_lg[tid] = lg; }
     tc_fence_before_sync();
     __syncthreads();
@@ -294,6 +295,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
     for (int k = 0; k < 2; k++) {
         const int box = 2 * k + (warp >> 2);
         if ((k == 0 || C::HALVES == 2) && !mbar_wait(b_state, k)) { s_fail = 1; atomicExch(a.status, 2); }
+        __syncwarp();                                                // (lanes poll on their own)
         const unsigned char* src = smem + C::KQ_BYTES + (C::HALVES == 2 ? box & 1 : box) * 16384 + d * 128;
         uint32_t hi[16], lo[16];
 #pragma unroll
@@ -345,6 +347,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
     if (tid < DV) su[NP * DV + tid] = 0.f;
     GDN_BSTAMP(5);
     if (!mbar_wait(b_mma, 0)) { s_fail = 1; atomicExch(a.status, 2); }
+    __syncwarp();
     tc_fence_after_sync();
     GDN_BSTAMP(6);
     // ---- L[j][i] = beta_i M_ij (k_i . k_j) and A[j][i] = M_ij (q_i . k_j), j along rows, so that a thread reads them for four i at a time ----
@@ -359,6 +362,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
         unsigned char* arow = reinterpret_cast<unsigned char*>(sA) + i * 128;        // Y_MMA: A's rows as operand images, hi and lo
         for (int j0 = (warp >> 2) * 16; j0 < NP; j0 += 32) {
             uint32_t r[16];
+            __syncwarp();
             tmem_ld16(tl + C::TM_G + j0, r);
             tmem_wait_ld();
             const uint32_t on = (uint32_t)(line >> j0);
@@ -519,6 +523,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
                 mma_commit(b_mma);
             }
             if (!mbar_wait(b_mma, 1)) { s_fail = 1; atomicExch(a.status, 2); }
+            __syncwarp();
             tc_fence_after_sync();
             load(C::TM_Y + i0, r);
 #pragma unroll
@@ -536,6 +541,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
         // a non-finite value somewhere: only what lies on a node's own path enters its sums
         for (int i0 = 0; i0 < NP; i0 += 16) {
             uint32_t r1[16], r2[16];
+            __syncwarp();
             tmem_ld16(tl + C::TM_P + i0, r1);
             tmem_ld16(tl + C::TM_P + NP + i0, r2);
             tmem_wait_ld();
@@ -564,7 +570,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
     GDN_BSTAMP(9);
     if (s_fail && tid == 0) { mbar_wait(b_state, C::HALVES - 1, 100000u); mbar_wait(b_mma, C::Y_MMA && plain ? 1 : 0, 100000u); }      // copies and products in flight end first
     __syncthreads();
-    if (warp == 7) tmem_dealloc(tb, 256);
+    if (warp == 7) { __syncwarp(); tmem_dealloc(tb, 256); }
 }
 
 typedef CUresult (*StateEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,

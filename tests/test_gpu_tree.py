@@ -175,6 +175,30 @@ def test_attn_tree_nothing_leaks_from_masked_places(dev, N):
     assert _lib.device_status() == 0
 
 
+@pytest.mark.parametrize("N,H,KV", [(13, 8, 2), (40, 8, 2), (9, 24, 2)])
+def test_attn_tree_rows_of_a_warp_see_different_values(dev, N, H, KV):
+    """Infinities and NaN in the values of several nodes of a random tree: the rows of one warp add different numbers of them between two loads from
+    tensor memory, and some of its rows are no node's.  Every output is what the definition gives, infinities with their sign."""
+    rng = np.random.default_rng(N + H)
+    ctx = [70, 900, 0]
+    c = attn_case(rng, ctx, N, 64, H, KV)
+    parents = np.stack([random_tree(rng, N, N - b) for b in range(3)])
+    for b in range(3):
+        for i in range(1, N, 2):
+            c["v_new"][b * N + i, :, rng.integers(0, 256, 6)] = rng.choice([np.inf, -np.inf, np.nan], (6, KV))
+    d = to_dev(c, dev)
+    out = host(run_attn(d, i32_dev(parents, dev)))
+    for b in range(3):
+        r = slice(b * N, (b + 1) * N)
+        with np.errstate(invalid="ignore"):
+            ref, mag = tree.attn_tree(c["q"][r], c["k_new"][r], c["v_new"][r], context(c, b, c["k_pages"]), context(c, b, c["v_pages"]), parents[b])
+        fin = np.isfinite(ref)
+        assert fin.any() and not fin.all()
+        assert np.array_equal(out[r][~fin], ref[~fin].astype(np.float32), equal_nan=True)
+        assert (np.abs(out[r][fin] - ref[fin]) <= HALF * np.abs(ref[fin]) + ATTN_ABS * mag[fin] + 1e-30).all()
+    assert _lib.device_status() == 0
+
+
 def test_attn_tree_reports_and_skips_what_is_malformed(dev):
     rng = np.random.default_rng(7)
     ctx = [40, 50, 60, 70]
