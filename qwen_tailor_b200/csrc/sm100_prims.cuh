@@ -36,10 +36,16 @@ __device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
+// Polls after which a wait gives up.  A build with -DGDN_WAIT_POLLS=0 gives up wherever it would have to wait, which is how the way out is
+// tested.  What a block has in flight when it gives up is waited for with a limit of its own.
+#ifndef GDN_WAIT_POLLS
+#define GDN_WAIT_POLLS 2000000u
+#endif
+constexpr uint32_t WAIT_POLLS = GDN_WAIT_POLLS, DRAIN_POLLS = 2000000u;
 // Bounded wait: non-blocking polls with a ~20 ns pause in between (back-to-back polls would take issue slots from the warps that
 // do the work); gives up after `limit` polls and returns false.  The caller records the failure and leaves the kernel instead
 // of spinning for ever on a shared GPU.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t limit = 2000000u) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t limit = WAIT_POLLS) {
     for (uint32_t i = 0; i < limit; i++) {
         if (mbar_test_wait(bar, parity)) return true;
         __nanosleep(20);

@@ -29,7 +29,8 @@
 // Masked places never reach the sums: scores are replaced, not multiplied; value rows behind the context and of unused nodes are zeroed in
 // shared memory; non-finite values of a node are zeroed there too (their weight is 0 for nodes that do not see it, and 0 x NaN is NaN)
 // and added back in the epilogue of the rows that do see it.
-// Every wait is bounded; one that gives up sets the device status word and the block runs out its loops.
+// Every wait is bounded; one that gives up sets the device status word and the block runs out its loops.  No block leaves before the copies and
+// products that it issued are over, whichever role gave up.
 #include <cstring>
 #include "gqa_common.cuh"
 #include "sm100_prims.cuh"
@@ -114,7 +115,7 @@ __device__ __forceinline__ int range_lo(int g, int G, int N) { const int q = N /
 // The rest of a bounded wait whose first poll failed; out of line, because a wait is needed in two dozen places and the code of the
 // roles' loops has to stay small (they run side by side out of one instruction cache).
 __device__ __noinline__ bool tree_wait_slow(uint32_t addr, uint32_t parity, volatile int* abort, int* status) {
-    for (uint32_t i = 0; i < 2000000u; i++) {
+    for (uint32_t i = 0; i < WAIT_POLLS; i++) {
         if (mbar_test_wait(addr, parity)) return true;
         if ((i & 63u) == 63u && *abort) return false;
         __nanosleep(20);
@@ -252,7 +253,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
         uint64_t stream_policy;                                      // the cache is read once per row tile: first to leave L2 unless a second row tile follows
         if (p.row_tiles == 1) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(stream_policy));
         else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(stream_policy));
-        uint32_t nr = 0, nseg = 0;                                   // slots filled so far
+        uint32_t nr = 0, nq = 0, nseg = 0, part = 0;                 // slots and Q buffers filled so far; lanes that filled one of a tile given up
         bool okp = true;
 #pragma unroll 1
         for (int x = lo; x < hi && okp;) {
@@ -267,6 +268,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                     for (int j = 0; j < 4; j++)
                         tma_load_3d(sQ + qb * (TA_Q_BYTES / 2) + j * p.q_slab, &tmQ, bar(AB_QFULL + qb), 64 * j, s.kvh * p.group, s.b * a.N + rt * p.nodes);
                 }
+                nq++;
             }
             const int* table = a.block_table + (size_t)s.b * a.max_pages;
             const int entries = s.ctx > 0 ? (s.ctx - 1) / a.page_size + 1 : 0;      // those that hold context
@@ -327,10 +329,11 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                     } else if (todo) {
                         __nanosleep(20);
                     }
-                    if ((polls & 63u) == 63u && __any_sync(0xffffffffu, aborted() || polls > 2000000u)) { okp = false; break; }
+                    if ((polls & 63u) == 63u && __any_sync(0xffffffffu, aborted() || polls > WAIT_POLLS)) { okp = false; break; }
                 }
                 if (!okp) {
                     if (lane == 0 && !aborted()) { s_abort = 1; atomicExch(a.status, 2); }
+                    part = __ballot_sync(0xffffffffu, lane < steps && !todo);
                     break;
                 }
                 nr += steps;
@@ -338,10 +341,13 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
             }
             nseg++;
         }
-        if (!okp && lane == 0) {                                     // gave up: the copies in flight have to land before the block leaves
-            for (int i = 0; i < ring; i++) if (nr > (uint32_t)i) mbar_wait(bar(first_full + i), ((nr - 1 - i) / ring) & 1, 100000u);
-            if (isk) for (int i = 0; i < p.q_bufs; i++) if (nseg + 1 > (uint32_t)i) mbar_wait(bar(AB_QFULL + i), ((nseg - i) / p.q_bufs) & 1, 100000u);
-        }
+        // Every copy has to land before the block leaves, also where another role gives up: lane i sees to the last one into slot i (a
+        // tile fills at most `ring` slots, so a tile given up added at most one), lanes behind it to the Q buffers.
+        const uint32_t first_use = lane < ring ? lane : lane - ring, every = lane < ring ? ring : p.q_bufs;
+        uint32_t uses = lane < ring ? nr : isk && lane < ring + p.q_bufs ? nq : 0;
+        uses = uses > first_use ? (uses - 1 - first_use) / every + 1 : 0;
+        if (lane < ring && (part >> (lane + ring - nr % ring) % ring & 1)) uses++;
+        if (uses) mbar_wait(bar(lane < ring ? first_full + lane : AB_QFULL + first_use), (uses - 1) & 1u, DRAIN_POLLS);
     } else if (warp == 4) {
         // ================= MMA issuer =================
         if (lane == 0) {
@@ -416,7 +422,8 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                 nseg++;
             }
             if (ok && p_have) ok = issue_pv(n - 1, p_limit, p_first, p_last, p_seg);
-            if (!ok) { mma_commit(bar(AB_DRAIN)); mbar_wait(bar(AB_DRAIN), 0, 100000u); }      // gave up: nothing may run on after the block
+            mma_commit(bar(AB_DRAIN));                               // no product may run on after the block, whichever role gave up
+            mbar_wait(bar(AB_DRAIN), 0, DRAIN_POLLS);
         }
     } else if (warp == 7) {
         // ================= nodes: their rows into the cache, by the block that has a pair's first tile; their value rows fit for the product =================
@@ -479,7 +486,7 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
                 // long as the segment, and so does its bound.
                 int got = 0;
                 if (lane == 0) {
-                    for (long long i = 0; i < 1000000ll * (s.n + 1) && !got && !aborted(); i++) {
+                    for (long long i = 0; i < (long long)(WAIT_POLLS / 2) * (s.n + 1) && !got && !aborted(); i++) {
                         got = mbar_test_wait(bar(AB_LAST), node_tiles & 1u);
                         if (!got) __nanosleep(100);
                     }
@@ -721,9 +728,9 @@ tree_attn_kernel(const __grid_constant__ TreeAttnPlan p, const __grid_constant__
             nseg++;
         }
     }
-    if (tid == 0 && aborted()) clear_info();
     tc_fence_before_sync();
     __syncthreads();
+    if (tid == 0 && aborted()) clear_info();                         // (every role is through: what gave up shows)
     if (warp == 4) { __syncwarp(); tmem_dealloc(tb, 512); }          // (one lane of it was the issuer)
     GDN_BSTAMP(9);
 }

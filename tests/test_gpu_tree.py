@@ -9,6 +9,7 @@ from qwen_tailor_b200 import Cfg, _lib, synth
 from qwen_tailor_b200.batch import attn_paged, attn_tree, compact_rows, copy_entries
 from qwen_tailor_b200.batch_spec import accept_tree, deltanet_bm, deltanet_commit, deltanet_tree
 from qwen_tailor_b200.paged_pools import PagedPools
+from short_waits import compile_library, operators_use
 
 pytestmark = pytest.mark.gpu
 
@@ -294,6 +295,26 @@ def test_attn_tree_captured_on_other_streams_and_repeatable(dev):
     for g, h, ref in zip(got, here, refs):
         assert torch.equal(g, ref) and torch.equal(h, ref)
     assert _lib.device_status() == 0
+
+
+@pytest.fixture(scope="module")
+def short_waits(tmp_path_factory):
+    return compile_library(tmp_path_factory.mktemp("short_waits"))
+
+
+def test_attn_tree_gives_up_in_order(dev, short_waits):
+    """Waits that run out are reported (status 2), nothing is left in flight, and the next calls are right."""
+    rng = np.random.default_rng(20)
+    for ctx, N, H, page in (([3000, 70, 0], 12, 8, 64), ([2000], 40, 8, 48), ([900, 1500], 3, 24, 5)):
+        c = attn_case(rng, ctx, N, page, H)
+        d, p = to_dev(c, dev), i32_dev(np.stack([random_tree(rng, N) for _ in ctx]), dev)
+        ref = run_attn(d, p)
+        assert _lib.device_status() == 0
+        with operators_use(short_waits):
+            for _ in range(20):
+                run_attn(d, p)
+                assert _lib.device_status() == 2
+        assert torch.equal(run_attn(d, p), ref) and _lib.device_status() == 0
 
 
 # ---------------------------------------------------------------------------------------------------------------------
