@@ -63,6 +63,9 @@ using namespace sm100;
 
 constexpr int TV_THREADS = 256;
 constexpr float LOG2E = 1.4426950408889634f, TV_WIPED = -160.f;      // 2^-160 is below the smallest fp32 number
+// Waits of verify that gave up.  A copy or product is only issued when the waits before it were not among them (as seen behind a barrier, so that
+// all threads see the same); y is unspecified then, and the block leaves when what was issued is over.
+enum { FAIL_STATE0 = 1, FAIL_STATE1 = 2, FAIL_PRODUCT = 4, FAIL_Y = 8 };
 template <int NP> struct TreeVerify {
     static constexpr int HALVES = NP == 64 ? 2 : 1;                  // pieces the state arrives in
     static constexpr int SLAB = 2 * NP * 128;                        // bytes of 64 dims of [K; Q]
@@ -107,7 +110,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
     __shared__ __align__(4) unsigned char s_list[NP / 16][NP];       // per block of 16 nodes: their ancestors in earlier blocks,
     __shared__ int s_cnt[NP / 16];                                   // in fours (filled up with NP, the row of zeros)
     __shared__ uint32_t s_tmem;
-    __shared__ int s_odd, s_fail;                                    // a non-finite value in this head; a wait gave up
+    __shared__ int s_odd, s_fail;                                    // a non-finite value in this head; waits that gave up (FAIL_*)
     const int N = a.N, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int b = blockIdx.x / HV, h = blockIdx.x % HV;
     const uint32_t sKQ = smem_addr(smem), sST = sKQ + C::KQ_BYTES;
@@ -291,10 +294,13 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
     // ---- the state into tensor memory as hi + lo: lane = value row, warps 0-3 and 4-7 take every other box of 32 key columns ----
     const uint32_t tl = tb + ((uint32_t)((warp & 3) * 32) << 16);
     const int d = (warp & 3) * 32 + lane;
+    auto gave_up = [&](int which) { atomicOr(&s_fail, which); atomicExch(a.status, 2); };
+    bool whole = C::HALVES == 1;                                     // the last piece of the state is on its way
 #pragma unroll 1
     for (int k = 0; k < 2; k++) {
         const int box = 2 * k + (warp >> 2);
-        if ((k == 0 || C::HALVES == 2) && !mbar_wait(b_state, k)) { s_fail = 1; atomicExch(a.status, 2); }
+        if (k == 0) { if (!mbar_wait(b_state, 0)) gave_up(FAIL_STATE0); }
+        else if (C::HALVES == 2 && whole) { if (!mbar_wait(b_state, 1)) gave_up(FAIL_STATE1); }
         __syncwarp();                                                // (lanes poll on their own)
         const unsigned char* src = smem + C::KQ_BYTES + (C::HALVES == 2 ? box & 1 : box) * 16384 + d * 128;
         uint32_t hi[16], lo[16];
@@ -308,14 +314,16 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
         tmem_st16(tl + C::TM_LO + 16 * box, lo);
         if (k == 0 && C::HALVES == 2) {
             __syncthreads();                                         // the first half has been read
-            if (tid == 0) load_state(1);
+            whole = !(s_fail & FAIL_STATE0);
+            if (tid == 0 && whole) load_state(1);
         }
     }
     tmem_wait_st();
     tc_fence_before_sync();
     __syncthreads();
     GDN_BSTAMP(3);
-    if (tid == TV_THREADS - 32) {
+    const bool product = !(s_fail & (FAIL_STATE0 | FAIL_STATE1));
+    if (tid == TV_THREADS - 32 && product) {
         tc_fence_after_sync();
         constexpr uint32_t HI = smem_desc_hi_sw128(1024);
         constexpr uint32_t I_P = idesc_bf16(128, 2 * NP, 0, 0), I_G = idesc_bf16(128, NP, 0, 0);
@@ -346,7 +354,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
     });
     if (tid < DV) su[NP * DV + tid] = 0.f;
     GDN_BSTAMP(5);
-    if (!mbar_wait(b_mma, 0)) { s_fail = 1; atomicExch(a.status, 2); }
+    if (product && !mbar_wait(b_mma, 0)) gave_up(FAIL_PRODUCT);
     __syncwarp();
     tc_fence_after_sync();
     GDN_BSTAMP(6);
@@ -398,7 +406,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
     GDN_BSTAMP(7);
     const bool solver = warp < 4;
     __nv_bfloat16* out = a.y + (size_t)b * N * KD + h * DV + d;
-    const bool plain = !s_odd;
+    const bool plain = !s_odd, y_product = C::Y_MMA && plain && product && !(s_fail & FAIL_PRODUCT);
     if (plain) {
 #pragma unroll 1
         for (int I = 0; I < NP / 16; I++) {
@@ -509,7 +517,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
             tmem_wait_st();
             tc_fence_before_sync();
             __syncthreads();
-            if (tid == TV_THREADS - 32) {
+            if (tid == TV_THREADS - 32 && y_product) {
                 tc_fence_after_sync();
                 constexpr uint32_t HI = smem_desc_hi_sw128(1024), I_Y = idesc_bf16(128, NP, 0, 0);
                 const uint32_t ah = smem_desc_lo(sKQ + NP * NP * 4, 16), al = ah + (C::A_LO >> 4);
@@ -522,7 +530,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
                 }
                 mma_commit(b_mma);
             }
-            if (!mbar_wait(b_mma, 1)) { s_fail = 1; atomicExch(a.status, 2); }
+            if (y_product && !mbar_wait(b_mma, 1)) gave_up(FAIL_Y);
             __syncwarp();
             tc_fence_after_sync();
             load(C::TM_Y + i0, r);
@@ -568,7 +576,10 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
     tc_fence_before_sync();
     __syncthreads();
     GDN_BSTAMP(9);
-    if (s_fail && tid == 0) { mbar_wait(b_state, C::HALVES - 1, 100000u); mbar_wait(b_mma, C::Y_MMA && plain ? 1 : 0, 100000u); }      // copies and products in flight end first
+    if (s_fail && tid == 0) {                                        // copies and products in flight end first
+        mbar_wait(b_state, C::HALVES == 2 && whole, DRAIN_POLLS);
+        if (product) mbar_wait(b_mma, y_product, DRAIN_POLLS);
+    }
     __syncthreads();
     if (warp == 7) { __syncwarp(); tmem_dealloc(tb, 256); }
 }

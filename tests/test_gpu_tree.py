@@ -419,6 +419,21 @@ def test_deltanet_tree_with_decays_from_none_to_all(dev, N):
     assert _lib.device_status() == 0
 
 
+def test_deltanet_tree_gives_up_in_order(dev, short_waits):
+    """Waits that run out are reported (status 2), nothing is left in flight, and the next calls are right."""
+    rng = np.random.default_rng(21)
+    for B, N in ((20, 5), (20, 27), (30, 64)):
+        c = delta_case(rng, B, N, B)
+        d, p = delta_dev(c, dev), i32_dev(np.stack([random_tree(rng, N) for _ in range(B)]), dev)
+        ref = run_delta(d, p)
+        assert _lib.device_status() == 0
+        with operators_use(short_waits):
+            for _ in range(20):
+                run_delta(d, p)
+                assert _lib.device_status() == 2
+        assert torch.equal(run_delta(d, p), ref) and _lib.device_status() == 0
+
+
 def test_deltanet_tree_of_a_chain_agrees_with_deltanet_bm(dev):
     rng = np.random.default_rng(32)
     c = delta_case(rng, 2, 4, 3)
