@@ -738,7 +738,7 @@ __global__ void __launch_bounds__(CM_THREADS, 2) tree_commit_kernel(const __grid
     if (!bad)
         for (int j = CM_PATH + tid; j < n; j += CM_THREADS) bad = bad || path[j] < 0 || path[j] >= a.N;
     if (__syncthreads_or(bad)) {
-        if (tid == 0) { atomicExch(a.status, 1); if (loads) mbar_wait(landed, 0); }      // (nothing may land after the block)
+        if (tid == 0) { atomicExch(a.status, 1); if (loads) mbar_wait(landed, 0, DRAIN_POLLS); }      // (nothing may land after the block)
         return;
     }
     auto node = [&](int j) -> int { return j < CM_PATH ? s_path[j] : path[j]; };
@@ -777,7 +777,12 @@ __global__ void __launch_bounds__(CM_THREADS, 2) tree_commit_kernel(const __grid
     // this thread's part of the state, in two halves: rows row + 8 half + 4 i, columns col + 32 m
     const int row = warp * 16 + (lane >> 3), col = (lane & 7) * 4;
     float* out = a.ssm_pool[layer] + (size_t)dst * STATE_ELEMS + (size_t)h * DV * DK;
-    bool ok = true;
+    // The state has landed?  Decided for the whole block: one that gives up writes nothing, and waits for the copy before it leaves.
+    auto state_is_here = [&]() -> bool {
+        if (!__syncthreads_or(!mbar_wait(landed, 0))) return true;
+        if (tid == 0) { atomicExch(a.status, 2); mbar_wait(landed, 0, DRAIN_POLLS); }
+        return false;
+    };
     ulonglong2 S[2][4];
     auto take = [&](int half) {
 #pragma unroll
@@ -827,8 +832,11 @@ __global__ void __launch_bounds__(CM_THREADS, 2) tree_commit_kernel(const __grid
                 }
             }
         }
-        __syncthreads();
-        if (j0 == 0 && !mbar_wait(landed, 0)) { ok = false; break; }
+        if (j0 == 0) {                                               // (a barrier, which the rows above need too)
+            if (!state_is_here()) return;
+        } else {
+            __syncthreads();
+        }
 #pragma unroll 1
         for (int half = 0; half < 2; half++) {
             take(half);
@@ -870,10 +878,9 @@ __global__ void __launch_bounds__(CM_THREADS, 2) tree_commit_kernel(const __grid
         }
     }
     if (n == 0) {
-        ok = mbar_wait(landed, 0);
-        if (ok) for (int half = 0; half < 2; half++) { take(half); put(half, true); }
+        if (!state_is_here()) return;
+        for (int half = 0; half < 2; half++) { take(half); put(half, true); }
     }
-    if (!ok) { atomicExch(a.status, 2); return; }
     // a window buffer that is read and written in one call (n even): every channel has been read by the thread that writes it
     __nv_bfloat16* wout = a.conv_pool[layer] + ((size_t)dst * 2 + (((unsigned)pos + (unsigned)n) & 1)) * 3 * CD;
     wout[ch] = x0; wout[CD + ch] = x1; wout[2 * CD + ch] = x2;

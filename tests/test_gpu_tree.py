@@ -504,6 +504,23 @@ def test_deltanet_commit_skips_what_is_out_of_range(dev):
         run({**d, "proj": d["proj"][:, :11]}, path, n)
 
 
+def test_deltanet_commit_gives_up_in_order(dev, short_waits):
+    """A block whose wait for its state runs out reports it (status 2) and writes nothing, in place or elsewhere, with and without a path."""
+    rng = np.random.default_rng(22)
+    c = delta_case(rng, 24, 10, 49, 4)
+    n = rng.integers(0, 11, 24).astype(np.int32)
+    path = i32_dev(np.tile(np.arange(10), (24, 1)), dev)
+    free = np.setdiff1d(np.arange(48), c["slots"])[:24].astype(np.int32)
+    for dst in (None, i32_dev(free, dev)):
+        d = delta_dev(c, dev)
+        with operators_use(short_waits):
+            for _ in range(20):
+                deltanet_commit(*(d[k] for k in ("proj", "conv", "conv_w", "A_log", "dt_bias", "ssm")), d["slots"], d["pos"], path, i32_dev(n, dev), dst_slots=dst)
+                assert _lib.device_status() == 2
+        assert np.array_equal(host(d["ssm"]), c["ssm"]) and np.array_equal(host(d["conv"]), c["conv"])
+    assert _lib.device_status() == 0
+
+
 def test_deltanet_commit_refuses_slots_that_depend_on_order(dev):
     rng = np.random.default_rng(42)
     c = delta_case(rng, 4, 3, 10)
