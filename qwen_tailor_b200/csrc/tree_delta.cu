@@ -407,6 +407,8 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
     const bool solver = warp < 4;
     __nv_bfloat16* out = a.y + (size_t)b * N * KD + h * DV + d;
     const bool plain = !s_odd, y_product = C::Y_MMA && plain && product && !(s_fail & FAIL_PRODUCT);
+    // which of the 32 nodes from i0 on are in use: the sums of the others are zeros times whatever the state holds, and 0 x NaN is NaN
+    auto used_from = [&](int i0) -> uint32_t { return __ballot_sync(0xffffffffu, i0 + lane < NP && s_line[i0 + lane < NP ? i0 + lane : 0]); };
     if (plain) {
 #pragma unroll 1
         for (int I = 0; I < NP / 16; I++) {
@@ -480,6 +482,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
                 }
             } else {
                 asm volatile("bar.sync %0, 256;" ::"r"(1 + I) : "memory");
+                const uint32_t used = used_from(16 * I);
 #pragma unroll
                 for (int c = 0; c < 16; c++) {                       // (entries before c are zero)
                     const float u = su[(16 * I + c) * DV + d];
@@ -495,8 +498,8 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
                     const float2 v = unpack2(x[k]);
-                    if (16 * I + 2 * k < N) out[(size_t)(16 * I + 2 * k) * KD] = __float2bfloat16_rn(v.x);
-                    if (16 * I + 2 * k + 1 < N) out[(size_t)(16 * I + 2 * k + 1) * KD] = __float2bfloat16_rn(v.y);
+                    if (16 * I + 2 * k < N) out[(size_t)(16 * I + 2 * k) * KD] = __float2bfloat16_rn(used >> 2 * k & 1 ? v.x : 0.f);
+                    if (16 * I + 2 * k + 1 < N) out[(size_t)(16 * I + 2 * k + 1) * KD] = __float2bfloat16_rn(used >> (2 * k + 1) & 1 ? v.y : 0.f);
                 }
             }
         }
@@ -511,6 +514,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
             float f[MINE];
             uint32_t r[MINE];
             const int i0 = MINE * (warp >> 2);
+            const uint32_t used = used_from(i0);
             load(C::TM_P + NP + i0, r);
 #pragma unroll
             for (int c = 0; c < MINE; c++) f[c] = s_grow[i0 + c] * __uint_as_float(r[c]);
@@ -536,7 +540,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tree_verify_kernel(const TreeDe
             load(C::TM_Y + i0, r);
 #pragma unroll
             for (int c = 0; c < MINE; c++)
-                if (i0 + c < N) out[(size_t)(i0 + c) * KD] = __float2bfloat16_rn(f[c] + __uint_as_float(r[c]));
+                if (i0 + c < N) out[(size_t)(i0 + c) * KD] = __float2bfloat16_rn(used >> c & 1 ? f[c] + __uint_as_float(r[c]) : 0.f);
         }
     } else if (solver) {
         // A's entries: as they are, or from their operand images (of a non-finite one hi alone)

@@ -419,6 +419,35 @@ def test_deltanet_tree_with_decays_from_none_to_all(dev, N):
     assert _lib.device_status() == 0
 
 
+@pytest.mark.parametrize("N", [6, 16, 20, 32, 64])
+def test_deltanet_tree_over_a_state_that_is_not_finite(dev, N):
+    """NaN and infinities in some value rows of a slot's state, and everywhere in the trash slot's: rows of unused nodes are zero all the same, used
+    nodes get NaN in those value rows, as the rule gives it (an infinite S k meets itself with the other sign in S + beta (v - S k) k^T), and no others."""
+    rng = np.random.default_rng(N)
+    c = delta_case(rng, 4, N, 5)
+    c["slots"][:] = [2, 0, 3, 4]
+    c["ssm"][0, 0, 3, 17, 5] = np.nan
+    c["ssm"][0, 0, 3, 90, 127] = np.inf
+    c["ssm"][0, 0, 11, 64, 0] = -np.inf
+    c["ssm"][0, 4] = rng.choice([np.nan, np.inf, -np.inf], (16, 128, 128))
+    parents = np.stack([random_tree(rng, N, N - 2 - b) for b in range(4)])
+    parents[1, 1], parents[3] = -2, -2                               # an unused node between used ones (and what hangs below it); an idle row of the batch
+    d = delta_dev(c, dev)
+    y = host(run_delta(d, i32_dev(parents, dev))).reshape(4, N, -1)
+    for b in range(3):
+        s, par = int(c["slots"][b]), int(c["pos"][b]) & 1
+        with np.errstate(invalid="ignore"):
+            ref = tree.deltanet_tree(c["proj"][0, b * N:(b + 1) * N], c["conv"][0, 2 * s + par], c["conv_w"][0], c["A_log"][0], c["dt_bias"][0], c["ssm"][0, s], parents[b])
+        used = np.array([bool(line) for line in tree.lines(parents[b])])
+        assert not y[b, ~used].any() and (~used).sum() >= 2 + b
+        assert np.array_equal(np.isnan(y[b]), np.isnan(ref)) and np.isnan(ref).sum() == (3 * used.sum() if b == 1 else 0)
+        ref = np.nan_to_num(ref)
+        scale = np.abs(ref).reshape(N, 16, 128).max((0, 2)).repeat(128)
+        assert (np.abs(np.nan_to_num(y[b]) - ref) <= HALF * np.abs(ref) + DELTA_ABS * scale).all()
+    assert not y[3].any(), "an idle row, whatever the trash slot holds"
+    assert _lib.device_status() == (1 if any(p == 1 for p in parents[1]) else 0)      # (a used node below an unused one is malformed)
+
+
 def test_deltanet_tree_gives_up_in_order(dev, short_waits):
     """Waits that run out are reported (status 2), nothing is left in flight, and the next calls are right."""
     rng = np.random.default_rng(21)
