@@ -419,6 +419,33 @@ def test_deltanet_tree_with_decays_from_none_to_all(dev, N):
     assert _lib.device_status() == 0
 
 
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+@pytest.mark.parametrize("N", [6, 16, 27, 32, 50, 64])
+def test_deltanet_tree_with_a_node_that_is_not_finite(dev, N, value):
+    """A q, k, v or gate of one head of an inner node is NaN or infinite: that head sums over ancestors one by one.  Element by element the result is
+    finite where the rule's is, and right there: nodes that do not hang below it, those that hang below a q far enough, the other heads."""
+    rng = np.random.default_rng(N)
+    c = delta_case(rng, 5, N, 5)
+    parents = np.stack([random_tree(rng, N, N - b % 2) for b in range(5)])
+    heads = [0, 5, 15, 7, 2]
+    for b, (channel, h) in enumerate(zip((128 * 0 + 3, 2048 + 127, 4096 + 64, 0, 0), heads)):
+        at = channel + 128 * h if b < 3 else 8192 + h if b == 3 else 8208 + h      # q, k, v; beta; decay
+        c["proj"][0, b * N + N // 3, at] = value if b < 3 else np.nan
+    d = delta_dev(c, dev)
+    y = host(run_delta(d, i32_dev(parents, dev))).reshape(5, N, -1)
+    for b, h in enumerate(heads):
+        s, par = int(c["slots"][b]), int(c["pos"][b]) & 1
+        with np.errstate(invalid="ignore", over="ignore"):
+            ref = tree.deltanet_tree(c["proj"][0, b * N:(b + 1) * N], c["conv"][0, 2 * s + par], c["conv_w"][0], c["A_log"][0], c["dt_bias"][0], c["ssm"][0, s], parents[b])
+        fin = np.isfinite(ref)
+        assert fin[:, :128 * h].all() and fin[:, 128 * h + 128:].all() and not fin[N // 3].all() and fin[0].all()
+        assert np.array_equal(np.isfinite(y[b]), fin), b
+        ref, got = np.where(fin, ref, 0), np.where(fin, y[b], 0)
+        scale = np.abs(ref).reshape(N, 16, 128).max((0, 2)).repeat(128)
+        assert (np.abs(got - ref) <= HALF * np.abs(ref) + DELTA_ABS * scale).all(), (b, float((np.abs(got - ref) - HALF * np.abs(ref)).max()))
+    assert _lib.device_status() == 0
+
+
 @pytest.mark.parametrize("N", [6, 16, 20, 32, 64])
 def test_deltanet_tree_over_a_state_that_is_not_finite(dev, N):
     """NaN and infinities in some value rows of a slot's state, and everywhere in the trash slot's: rows of unused nodes are zero all the same, used
