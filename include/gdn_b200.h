@@ -280,7 +280,7 @@ GDN_API int gdn_tree_accept(const int* parents, const int* toks, const int* ids,
  * so are sequences of which one writes a slot that another reads or writes (the result would depend on the order), the pools' last slot
  * excepted: padding goes there, and its content is unspecified.  n_path[b] = 0 with dst_slots[b] = slots[b] touches nothing.
  *   The `_host` arrays hold one device pointer per layer: proj bf16 [B*N, row_stride], conv_pool, conv_w, A_log, dt_bias, ssm_pool as for
- *   gdn_deltanet_b.   path int32 [B, E]: nodes of the tree, 0 <= path < N */
+ *   gdn_deltanet_b; no conv or ssm pool stands for two layers.   path int32 [B, E]: nodes of the tree, 0 <= path < N */
 GDN_API int gdn_tree_commit(const void* const* proj_host, long long row_stride, void* const* conv_pool_host, const void* const* conv_w_host,
                     const void* const* A_log_host, const void* const* dt_bias_host, void* const* ssm_pool_host, int n_layers, const int* slots,
                     const int* dst_slots, const int* pos, const int* path, const int* n_path, int n_slots, int B, int N, int E, void* stream);

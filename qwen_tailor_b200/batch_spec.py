@@ -177,8 +177,9 @@ def deltanet_commit(projs, conv_pools, conv_ws, A_logs, dt_biases, ssm_pools, sl
     N = row[0] // B if B else 1
     if B and (N < 1 or row[0] != B * N):
         raise ValueError(f"{who}: proj has {row[0]} rows for {B} sequences")
-    if L > 1 and len(set(ptrs[5 * L:])) < L:
-        raise ValueError(f"{who}: one ssm pool for two layers")
+    for name, at in (("conv", L), ("ssm", 5 * L)):                   # (written: the layers run side by side)
+        if L > 1 and len(set(ptrs[at:at + L])) < L:
+            raise ValueError(f"{who}: one {name} pool for two layers")
     base = ptrs.buffer_info()[0]
     at = [base + 8 * L * i for i in range(6)]
     with on_device(dev):

@@ -639,6 +639,21 @@ def test_more_sequences_than_a_block_has_threads(dev):
 # ---------------------------------------------------------------------------------------------------------------------
 # accepting and copying
 # ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("field", ["conv", "ssm"])
+def test_deltanet_commit_refuses_one_pool_for_two_layers(dev, field):
+    rng = np.random.default_rng(44)
+    c = delta_case(rng, 2, 3, 4, 2)
+    d = delta_dev(c, dev)
+    layers = {k: list(d[k]) for k in ("proj", "conv", "conv_w", "A_log", "dt_bias", "ssm")}
+    layers[field][1] = layers[field][0]
+    with pytest.raises(ValueError, match=f"one {field} pool for two layers"):
+        deltanet_commit(*layers.values(), d["slots"], d["pos"], i32_dev([[0, 1, 2]] * 2, dev), i32_dev([2, 1], dev))
+    assert np.array_equal(host(d["ssm"]), c["ssm"]) and np.array_equal(host(d["conv"]), c["conv"])
+    shared = {k: (list(d[k]) if k in ("conv", "ssm") else [d[k][0]] * 2) for k in layers}      # weights and rows may be shared
+    deltanet_commit(*shared.values(), d["slots"], d["pos"], i32_dev([[0, 1, 2]] * 2, dev), i32_dev([2, 1], dev))
+    assert _lib.device_status() == 0
+
+
 @pytest.mark.parametrize("N,kind", [(1, "chain"), (7, "random"), (32, "star"), (33, "forest"), (64, "random"), (64, "chain")])
 def test_accept_tree(dev, N, kind):
     rng = np.random.default_rng(N)
