@@ -81,7 +81,14 @@ class PagePool:
                 self.free.append(int(p))
 
     def copy_pages(self, dst: Sequence[int], src: Sequence[int], n_rows: int):
-        """Rows [0, n_rows) of every (layer, K/V, head) of page src[i] -> page dst[i], for all i in one launch."""
+        """Rows [0, n_rows) of every (layer, K/V, head) of page src[i] -> page dst[i], for all i in one launch (a page onto itself, or no
+        rows: nothing happens)."""
+        if len(dst) != len(src):
+            raise ValueError(f"copy_pages: {len(dst)} destinations for {len(src)} sources")
+        pairs = [(d, s) for d, s in zip(dst, src) if d != s]
+        if n_rows <= 0 or not pairs:
+            return
+        dst, src = zip(*pairs)
         if self.K[0].is_cuda:
             from .batch import copy_entries
             copy_entries(self.K + self.V, dst, src, rows=None if n_rows == self.page_size else n_rows)

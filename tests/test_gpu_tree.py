@@ -9,6 +9,7 @@ from qwen_tailor_b200 import Cfg, _lib, synth
 from qwen_tailor_b200.batch import attn_paged, attn_tree, compact_rows, copy_entries
 from qwen_tailor_b200.batch_spec import accept_tree, deltanet_bm, deltanet_commit, deltanet_tree
 from qwen_tailor_b200.paged_pools import PagedPools
+from qwen_tailor_b200.prefix_cache import PagePool
 from short_waits import compile_library, operators_use
 
 pytestmark = pytest.mark.gpu
@@ -780,6 +781,25 @@ def test_copy_entries_refusals(dev):
     with pytest.raises(ValueError):
         copy_entries([p.view(6, 64)], [1], [0], rows=1)
     assert not p.any()
+
+
+def test_page_copies_onto_themselves_and_of_no_rows_change_nothing(dev):
+    pool = PagePool(2, 6, 8, 2, 16, device=dev)
+    for X in pool.K + pool.V:
+        X.copy_(torch.randn(X.shape, device=dev))
+    before = [X.clone() for X in pool.K + pool.V]
+    pool.copy_rows(3, 3, 5)
+    pool.copy_rows(3, 3, 8)
+    pool.copy_rows(2, 1, 0)
+    pool.copy_rows(2, 1, -1)
+    pool.copy_pages([1, 4], [1, 4], 8)
+    assert all(torch.equal(X, X0) for X, X0 in zip(pool.K + pool.V, before))
+    pool.copy_pages([1, 4, 5], [1, 2, 5], 3)
+    for X, X0 in zip(pool.K + pool.V, before):
+        X0[4, :, :3] = X0[2, :, :3]
+        assert torch.equal(X, X0)
+    with pytest.raises(ValueError):
+        pool.copy_pages([1, 2], [3], 8)
 
 
 # ---------------------------------------------------------------------------------------------------------------------
