@@ -80,7 +80,9 @@ def deltanet_tree(proj, conv_pool, conv_w, A_log, dt_bias, ssm_pool, slots, pos,
     its parent leaves.  Returns y [B*N, 2048] bf16; rows of unused nodes are zero.  Conv, silu, norms and gates are computed in fp32
     and rounded nowhere before y; the chained kernels round to bf16 after each step, so the two agree to bf16 rounding."""
     dev = require_same_device(proj, conv_pool, conv_w, A_log, dt_bias, ssm_pool, slots, pos, parents, out)
-    proj, stride = _rows(proj)
+    if proj.dtype != torch.bfloat16 or proj.dim() != 2 or proj.shape[1] < PW or proj.stride(1) != 1:
+        raise ValueError(f"deltanet_tree: proj must be bf16 [rows, >= 8224] with unit inner stride, got {tuple(proj.shape)} {proj.dtype}")
+    stride = proj.stride(0)
     if parents.dtype != torch.int32 or parents.dim() != 2 or not parents.is_contiguous():
         raise ValueError("deltanet_tree: parents must be contiguous int32 [B, N]")
     B, N = parents.shape

@@ -398,6 +398,20 @@ def test_deltanet_tree_malformed_trees_slots_and_masked_nans(dev):
     assert run_delta({**d, "slots": d["slots"][:0], "pos": d["pos"][:0]}, i32_dev(parents[:0], dev), d["proj"][0][:0]).shape == (0, 2048)
 
 
+def test_deltanet_tree_refuses_rows_of_another_form(dev):
+    rng = np.random.default_rng(33)
+    d = delta_dev(delta_case(rng, 2, 3, 2), dev)
+    p = i32_dev(np.stack([random_tree(rng, 3)] * 2), dev)
+    proj = d["proj"][0]
+    wide = torch.zeros(6, 2 * 8224, dtype=torch.bfloat16, device=dev)
+    odd = torch.zeros(6 * 8224 + 1, dtype=torch.bfloat16, device=dev)[1:].view(6, 8224)
+    for bad in (proj.float(), proj[:, :8223], proj[:5], proj.view(-1), wide[:, ::2], odd, proj.view(2, 3, 8224), torch.zeros(6, 8226, dtype=torch.bfloat16, device=dev)):
+        with pytest.raises(ValueError):
+            run_delta(d, p, bad)
+    run_delta(d, p, torch.zeros(6, 8228, dtype=torch.bfloat16, device=dev))
+    assert _lib.device_status() == 0
+
+
 @pytest.mark.parametrize("N", [12, 64])
 def test_deltanet_tree_with_decays_from_none_to_all(dev, N):
     """Tokens that keep the state, that halve it and that wipe it out, mixed along every path: what lies between two nodes of a path counts, not
