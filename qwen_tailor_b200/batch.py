@@ -205,7 +205,11 @@ def copy_entries(pools: Sequence[torch.Tensor], dst: Sequence[int], src: Sequenc
     rows (an int, or one per pair): only the first rows of every head of pages [n_entries, heads, page_size, dim] are copied.
     Every 512 pairs take one launch."""
     first, shape, ptrs = _pool_ptrs("copy_entries", pools, stacked)
-    d, s = array("i", dst), array("i", src)
+    try:
+        d, s = array("i", dst), array("i", src)
+        each = None if rows is None or isinstance(rows, Integral) else array("q", rows)
+    except OverflowError as e:
+        raise ValueError(f"copy_entries: entries and rows are 32-bit numbers ({e})") from None
     n = len(d)
     if n != len(s):
         raise ValueError(f"copy_entries: {n} destinations for {len(s)} sources")
@@ -216,8 +220,8 @@ def copy_entries(pools: Sequence[torch.Tensor], dst: Sequence[int], src: Sequenc
     if rows is not None:
         if len(shape) != 4:
             raise ValueError(f"copy_entries: rows needs pools [n_entries, heads, page_size, dim], got entries of {tuple(shape[1:])}")
-        row, one = shape[3] * item, isinstance(rows, Integral)
-        r = (int(rows),) if one else array("q", rows)
+        row, one = shape[3] * item, each is None
+        r = (int(rows),) if one else each
         if (not one and len(r) != n) or min(r) < 0 or max(r) > shape[2]:
             raise ValueError(f"copy_entries: rows must be one number or {n}, from 0 to {shape[2]}")
         n_sub, sub_bytes = shape[1], shape[2] * row

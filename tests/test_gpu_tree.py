@@ -797,6 +797,13 @@ def test_copy_entries_refusals(dev):
     assert not p.any()
 
 
+@pytest.mark.parametrize("dst,src,rows", [([2 ** 31], [0], None), ([0], [-2 ** 31 - 1], None), ([2 ** 40], [0], 1), ([1], [0], [2 ** 63])])
+def test_copy_entries_refuses_numbers_beyond_32_bits(dev, dst, src, rows):
+    p = torch.zeros(6, 2, 4, 8, device=dev)
+    with pytest.raises(ValueError):
+        copy_entries([p], dst, src, rows=rows)
+
+
 def test_page_copies_onto_themselves_and_of_no_rows_change_nothing(dev):
     pool = PagePool(2, 6, 8, 2, 16, device=dev)
     for X in pool.K + pool.V:
