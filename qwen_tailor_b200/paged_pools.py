@@ -146,7 +146,8 @@ class PagedPools:
         return deltanet_tree(proj, self.conv[layer], conv_w, A_log, dt_bias, self.ssm[layer], slots, pos, parents, out=out)
 
     def attn_tree(self, layer: int, q, k_new, v_new, slots: torch.Tensor, ctx_len: torch.Tensor, parents: torch.Tensor, out=None):
-        """``batch.attn_tree`` of full-attention layer ``layer``.  ``reserve`` must have made room for ctx_len + N tokens."""
+        """``batch.attn_tree`` of full-attention layer ``layer``.  ``reserve`` must have made room for min(ctx_len + N, max_len) tokens; nodes
+        from max_len - ctx_len on have to be unused."""
         table = self.table.index_select(0, slots.long())
         return attn_tree(q, k_new, v_new, self.pages.K[layer], self.pages.V[layer], table, ctx_len, parents, out=out)
 

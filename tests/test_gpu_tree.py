@@ -970,6 +970,58 @@ def test_a_round_captured_replayed_and_padded(dev):
     assert _lib.device_status() == 0
 
 
+@pytest.mark.parametrize("max_len,page", [(128, 64), (100, 64), (70, 7)])
+def test_a_round_at_the_end_of_a_sequence(dev, max_len, page):
+    """The last round before max_len, as documented: room for what fits, the nodes behind it unused.  A tree that fits to the last row, one of which two nodes
+    fit, and a full sequence."""
+    rng = np.random.default_rng(max_len)
+    cfg = Cfg(layers=4)
+    N, lengths = 6, [max_len - 6, max_len - 2, max_len]
+    pools = PagedPools(cfg, 3, max_len, n_pages=3 * -(-max_len // page) + 1, page_size=page)
+    c = delta_case(rng, 3, N, 4, cfg.n_linear)
+    for l in range(cfg.n_linear):
+        pools.ssm[l].copy_(f32_dev(c["ssm"][l], dev))
+        pools.conv[l].copy_(bf16_dev(c["conv"][l], dev))
+    r = lambda *s: synth.bf16r(rng.standard_normal(s))  # noqa: E731
+    kv = [r(2, 2, n, 256) for n in lengths]
+    for s, n in enumerate(lengths):
+        pools.reserve(s, n)
+        pools.length[s] = n
+        for X, x in zip((pools.pages.K[0], pools.pages.V[0]), kv[s]):
+            for i, pg in enumerate(pools.owned[s]):
+                rows = x[:, i * page:(i + 1) * page]
+                X[pg, :, :rows.shape[1]] = bf16_dev(rows, dev)
+        pools.reserve(s, min(n + N, pools.Lmax))
+    parents = np.stack([random_tree(rng, N, min(N, max_len - n)) for n in lengths])
+    q, k, v = (r(3 * N, h, 256) for h in (8, 2, 2))
+    slots, pos, p = i32_dev([0, 1, 2], dev), i32_dev(lengths, dev), i32_dev(parents, dev)
+    projs, w = [bf16_dev(x, dev) for x in c["proj"]], (list(bf16_dev(c["conv_w"], dev)), list(f32_dev(c["A_log"], dev)), list(f32_dev(c["dt_bias"], dev)))
+    ys = [host(pools.deltanet_tree(l, projs[l], w[0][l], w[1][l], w[2][l], slots, pos, p)).reshape(3, N, -1) for l in range(cfg.n_linear)]
+    o = host(pools.attn_tree(0, bf16_dev(q, dev), bf16_dev(k, dev), bf16_dev(v, dev), slots, pos, p)).reshape(3, N, 8, 256)
+    ids = np.zeros((3, N), np.int32)
+    n_path, path = accept_tree(p, i32_dev(ids, dev), i32_dev(ids, dev))
+    pools.commit_tree(projs, *w, slots, pos, path, n_path)
+    for s, n in enumerate(lengths):
+        want = tree.accept(parents[s], ids[s], ids[s])
+        assert len(want) == int(n_path[s]) and (len(want) > 0) == (s < 2)
+        ref, mag = tree.attn_tree(q[s * N:(s + 1) * N], k[s * N:(s + 1) * N], v[s * N:(s + 1) * N], *kv[s], parents[s])
+        assert (np.abs(o[s] - ref) <= HALF * np.abs(ref) + ATTN_ABS * mag + 1e-30).all()
+        pools.advance(s, len(want))
+        pools.trim(s)
+        for X, x, new in zip((pools.pages.K[0], pools.pages.V[0]), kv[s], (k, v)):
+            rows = np.concatenate([host(X[pg]) for pg in pools.owned[s]], 1)[:, :n + len(want)]
+            assert np.array_equal(rows, np.concatenate([x, new[s * N:(s + 1) * N][want].transpose(1, 0, 2)], 1))
+        for l in range(cfg.n_linear):
+            win = c["conv"][l, 2 * s + (n & 1)]
+            ref = tree.deltanet_tree(c["proj"][l, s * N:(s + 1) * N], win, c["conv_w"][l], c["A_log"][l], c["dt_bias"][l], c["ssm"][l, s], parents[s])
+            scale = np.abs(ref).reshape(N, 16, 128).max((0, 2)).repeat(128)
+            assert (np.abs(ys[l][s] - ref) <= HALF * np.abs(ref) + DELTA_ABS * scale).all()
+            S, win = tree.commit(c["proj"][l, s * N:(s + 1) * N], win, c["conv_w"][l], c["A_log"][l], c["dt_bias"][l], c["ssm"][l, s], want)
+            assert np.abs(host(pools.ssm[l][s]) - S).max() <= 2.0 ** -16 * np.abs(S).max()
+            assert np.array_equal(host(pools.conv[l][2 * s + (n + len(want)) % 2]), win)
+    assert _lib.device_status() == 0
+
+
 def test_pools_beyond_32_bit_offsets(dev):
     """Pages and slots that lie more than 2^31 elements into their pools give what the same contents give at the front."""
     rng = np.random.default_rng(5)
