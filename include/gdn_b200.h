@@ -245,7 +245,7 @@ GDN_API int gdn_hrec(void* hist, const void* rows, const int* slots, const int* 
 /* ---- speculative decoding with a tree of drafted tokens, and copies over many pools (no counterpart in the reference, whose
  *      speculative mode verifies one chain) ----
  * A tree: parents int32 [B, N], N <= 64.  Node i of sequence b hangs below node parents[b][i] < i; -1 = below the sequence's last
- * cached token (a root; several are allowed); a smaller value = an unused node.  A parent that does not precede its child, or that
+ * cached token (a root; there may be several, but the accepted path starts at the first); a smaller value = an unused node.  A parent that does not precede its child, or that
  * is unused, makes the node (and what hangs below it) unused and sets device status 1. */
 
 /* Attention of all nodes of the trees over a paged KV cache: node i attends the cached keys 0 .. ctx_len[b]-1, itself and its
@@ -288,7 +288,8 @@ GDN_API int gdn_tree_commit(const void* const* proj_host, long long row_stride, 
 /* Compaction of cached rows in n_pools pools [n_pages, heads, page_size, row_bytes]: row base[b] + keep[b][j] of sequence b (through
  * block_table) moves to row base[b] + j (through dst_table), j < n_keep[b].  keep is strictly ascending; from the first entry that is not, or
  * that is out of range, the rest of that sequence stays as it is (status 1).  dst_table equals block_table (in place), or the pages it
- * names for the written rows are not read by the call.   block_table, dst_table int32 [B, max_pages];  keep int32 [B, L] */
+ * names for the written rows are not read by the call.  Pages that are written belong to one sequence of the call; whoever shares one sees
+ * it change.   block_table, dst_table int32 [B, max_pages];  keep int32 [B, L] */
 GDN_API int gdn_rows_compact(void* const* pools_host, int n_pools, int n_pages, int heads, int page_size, long long row_bytes, const int* block_table,
                      const int* dst_table, int max_pages, const int* base, const int* keep, const int* n_keep, int B, int L, void* stream);
 

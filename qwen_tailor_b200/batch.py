@@ -99,8 +99,8 @@ def attn_tree(q, k_new, v_new, k_pages, v_pages, block_table, ctx_len, parents, 
     """GQA attention of a TREE of drafted tokens over a paged KV cache: the verify step of tree speculation, as ``attn_paged`` with M > 1
     is that of a chain (no counterpart in the reference).
 
-    parents int32 [B, N], N <= 64: node i of sequence b hangs below node parents[b, i] < i; -1 = below the last cached token (a root,
-    several are allowed); a smaller value = an unused node.  q [B*N, H, 256], k_new / v_new [B*N, KV, 256] bf16 (normed and roped at
+    parents int32 [B, N], N <= 64: node i of sequence b hangs below node parents[b, i] < i; -1 = below the last cached token (a root;
+    there may be several, but ``accept_tree`` only follows the first); a smaller value = an unused node.  q [B*N, H, 256], k_new / v_new [B*N, KV, 256] bf16 (normed and roped at
     position ctx_len[b] + depth of the node), pages [n_pages, KV, page_size, 256] (any page size), block_table int32 [B, max_pages],
     ctx_len int32 [B].  H is a multiple of KV, at most 16 query heads share one.
     Node i attends the cached keys of its sequence, its ancestors and itself; its k / v rows are appended at ctx_len[b] + i (in place;
@@ -245,7 +245,10 @@ def compact_rows(pools: Sequence[torch.Tensor], block_table, base, keep, n_keep,
     pools: page pools [n_pages, heads, page_size, dim] (bf16 or fp32; K and V of all layers), stacked=True: with a leading layer
     dimension.  block_table int32 [B, max_pages]; base, n_keep int32 [B]; keep int32 [B, L], strictly ascending.  All on the device.
     dst_table: the rows are written through this table instead (pages that the call does not read, or the same table): the
-    source keeps its rows.  From the first keep entry that is out of order or range the rest of a sequence is left alone and
+    source keeps its rows.
+    The pages that rows are written to belong to one sequence: a page that another one shares (``PagePool.fork``, a checkpoint) changes
+    for both, so with base = 0 only sequences of their own pages move in place, and no two sequences of a call write the same page.  One warp
+    walks the rows of a sequence in a pool and head: made for the handful that a round keeps.  From the first keep entry that is out of order or range the rest of a sequence is left alone and
     ``_lib.device_status()`` reports it."""
     first, shape, ptrs = _pool_ptrs("compact_rows", pools, stacked)
     dst_table = block_table if dst_table is None else dst_table

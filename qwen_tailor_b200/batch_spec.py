@@ -50,7 +50,8 @@ def accept_length(toks, ids):
 
 def accept_tree(parents, toks, ids):
     """The path of a tree that the target confirms, found on the device (``accept_length`` for trees): from the first root, as long as
-    there is one, to the lowest-numbered child whose token the target chose after its parent.
+    there is one, to the lowest-numbered child whose token the target chose after its parent.  The root is the token that the last round
+    confirmed; other roots and what hangs below them are never on the path (nothing here says what the target chose before them).
 
     parents int32 [B, N] as for ``attn_tree``, N <= 64; toks int32 [B, N] the nodes' tokens (those of roots are taken as confirmed); ids
     int32 [B, N] the target's token after every node.  Returns n_path int32 [B] and path int32 [B, N] (the path's nodes in order, then

@@ -154,7 +154,8 @@ class PagedPools:
     def commit_tree(self, projs, conv_ws, A_logs, dt_biases, slots: torch.Tensor, pos: torch.Tensor, path: torch.Tensor, n_path: torch.Tensor):
         """Settles a round on the device, all layers in two launches: states and conv windows advance along the accepted path
         (``deltanet_commit``, per-layer arguments as there), the K/V rows of the path move together behind the context
-        (``compact_rows``).  pos int32 [B] = tokens cached before the round.  The host follows with ``advance(slot, n_path)``."""
+        (``compact_rows``).  pos int32 [B] = tokens cached before the round.  The host follows with ``advance(slot, n_path)``.  No slot but
+        the trash slot stands twice in ``slots`` (its states would stay as they are, status 1, and its rows move twice)."""
         deltanet_commit(projs, self.conv, conv_ws, A_logs, dt_biases, self.ssm, slots, pos, path, n_path)
         compact_rows(self.pages.K + self.pages.V, self.table.index_select(0, slots.long()), pos, path, n_path)
 
