@@ -263,8 +263,8 @@ GDN_API int gqa_tree_attn(const void* q, const void* k_new, const void* v_new, v
 GDN_API size_t gqa_tree_attn_workspace_bytes(int B, int N, int H, int KV);
 
 /* Gated delta rule for all nodes of the trees: node i continues the conv window and the state that its parent leaves (a root: those of
- * the slot).  Only y is written (rows of unused nodes and of sequences with a bad slot: zero).  Conv, norms and gates in fp32, one
- * rounding (y).
+ * the slot).  Only y is written (rows of unused nodes and of sequences with a bad slot: zero).  Conv, norms, gates and the solve in
+ * fp32; operands of products as sums of two bf16 numbers (2^-16 of the factors left out); y is rounded once.
  *   proj bf16 [B*N, row_stride >= 8224];  conv_pool, ssm_pool, slots, pos as for gdn_deltanet_b;  y bf16 [B*N, 2048] */
 GDN_API int gdn_tree_verify(const void* proj, long long row_stride, const void* conv_pool, const void* conv_w, const float* A_log, const float* dt_bias,
                     const float* ssm_pool, const int* slots, const int* pos, const int* parents, int n_slots, void* y, int B, int N, void* stream);

@@ -78,8 +78,9 @@ def deltanet_tree(proj, conv_pool, conv_w, A_log, dt_bias, ssm_pool, slots, pos,
 
     proj [B*N, 8224] bf16 (row b*N+i = node i of sequence b, row stride a multiple of 4 elements); parents int32 [B, N] as for
     ``attn_tree``, N <= 64; conv_pool, ssm_pool, slots, pos as for ``deltanet_b``.  Node i continues the conv window and the state that
-    its parent leaves.  Returns y [B*N, 2048] bf16; rows of unused nodes are zero.  Conv, silu, norms and gates are computed in fp32
-    and rounded nowhere before y; the chained kernels round to bf16 after each step, so the two agree to bf16 rounding."""
+    its parent leaves.  Returns y [B*N, 2048] bf16; rows of unused nodes are zero.  Conv, silu, norms, gates and the solve are
+    computed in fp32; the operands of tensor-core products are sums of two bf16 numbers (what is left out is 2^-16 of the factors); y is rounded once.
+    The chained kernels round to bf16 after each step, so the two agree to bf16 rounding."""
     dev = require_same_device(proj, conv_pool, conv_w, A_log, dt_bias, ssm_pool, slots, pos, parents, out)
     if proj.dtype != torch.bfloat16 or proj.dim() != 2 or proj.shape[1] < PW or proj.stride(1) != 1:
         raise ValueError(f"deltanet_tree: proj must be bf16 [rows, >= 8224] with unit inner stride, got {tuple(proj.shape)} {proj.dtype}")

@@ -9,9 +9,10 @@
 // so the state is read once whatever the tree's size.  After the target has chosen, `commit` advances state and conv window along the
 // accepted path, for all layers in one launch.
 //
-// Conv, silu, norm and gates stay in fp32 here, and nothing is rounded before y (bf16) or the state (fp32): the single-token and
-// chained kernels round to bf16 after each of these operations as the reference's graph does, so results agree with them to
-// bf16 rounding, not bit for bit.
+// Conv, silu, norm, gates and the solve stay in fp32 here until y (bf16) or the state (fp32) is stored.  The operands of verify's tensor-core products -- S0, K
+// and Q, with 17 nodes and more also u and A -- are each the sum of two bf16 numbers hi + lo (exact to 2^-17), and lo x lo is left out (2^-16 of the
+// factors at most).  The single-token and chained kernels round to bf16 after each of these operations as the reference's graph does, so
+// results agree with them to bf16 rounding, not bit for bit.
 #include <cuda.h>
 #include <type_traits>
 #include "gdn_common.cuh"
@@ -46,7 +47,7 @@ __device__ __forceinline__ unsigned long long tree_line(const int* par, int i, b
 //     [P1 | P2] = S0 [K; Q]^T     on the tensor cores, rows = value rows d: S0 in tensor memory, [K; Q] in shared memory
 //     G         = [K; Q] K^T      on the tensor cores
 // each operand as bf16 hi + lo and the three products that matter (what is dropped is 2^-16 of the factors; K and Q rounded to bf16
-// alone would put an error of the size of y's own rounding on every product).  The rest is fp32: thread d of four warps solves
+// alone would put an error of the size of y's own rounding on every product).  The solve is fp32: thread d of four warps solves
 //     u_i = beta_i (v_i - e^G_i P1_i) - sum_j L_ij u_j
 // for its value row in blocks of 16 nodes.  Up to 16 nodes thread d of the other four follows with
 //     y_i = e^G_i P2_i + sum_j A_ij u_j;
@@ -88,7 +89,8 @@ typedef unsigned long long f32x2;
 __device__ __forceinline__ f32x2 pack2(float x, float y) { f32x2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y)); return r; }
 __device__ __forceinline__ float2 unpack2(f32x2 v) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v)); return r; }
 __device__ __forceinline__ void fma2(f32x2& x, f32x2 a, f32x2 b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(x) : "l"(a), "l"(b)); }
-// the fast approximations of exp and of the division are good to a few fp32 ulp, far below y's rounding to bf16
+// The documented errors of the fast exp, 2 + 1.173 |x| ulp, and of the fast division, 2 ulp, make 2^-18 of the value up to |x| = 40 (below -40 the value is
+// smaller than 2^-52), 2^-9 of y's rounding to bf16.
 __device__ __forceinline__ float silu_fast(float x) { return __fdividef(x, 1.f + __expf(-x)); }
 
 __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
