@@ -43,7 +43,7 @@ __device__ __forceinline__ unsigned long long tree_line(const int* par, int i, b
 // ----------------------------------------------------------------------------------------------------------------------
 // verify: one block per (sequence, head), two blocks per SM.  NP = nodes padded to 16, 32 or 64.  Bound: issue slots and latency
 // (some 40 k warp instructions a head at 64 nodes, half of the slots used; the state alone would take a quarter of the time).  Measured: 64
-// sequences x 64 nodes 86 us, 16 x 27 14.4 us, one sequence x 8 nodes 8.0 us.
+// sequences x 64 nodes 87 us, 16 x 27 16.5 us, one sequence x 8 nodes 9.0 us (states that L2 does not hold).
 //     [P1 | P2] = S0 [K; Q]^T     on the tensor cores, rows = value rows d: S0 in tensor memory, [K; Q] in shared memory
 //     G         = [K; Q] K^T      on the tensor cores
 // each operand as bf16 hi + lo and the three products that matter (what is dropped is 2^-16 of the factors; K and Q rounded to bf16
@@ -51,9 +51,10 @@ __device__ __forceinline__ unsigned long long tree_line(const int* par, int i, b
 //     u_i = beta_i (v_i - e^G_i P1_i) - sum_j L_ij u_j
 // for its value row in blocks of 16 nodes.  Up to 16 nodes thread d of the other four follows with
 //     y_i = e^G_i P2_i + sum_j A_ij u_j;
-// with more, where it would follow block by block, this sum is another product, u and A as hi + lo (64 sequences x 64 nodes 86 us against
-// 90, x 32 nodes 52.8 against 54.1, one sequence x 32 nodes 11.1 either way).  L and A are dense with zeros outside the ancestors; zeros do not stop NaN, so a head with a non-finite q, k, v or gate takes the sums over the
-// ancestors one by one instead.
+// with more, where it would follow block by block, this sum is another product, u and A as hi + lo (when it was made one, 64 sequences x 64
+// nodes 86 us against 90, x 32 nodes 52.8 against 54.1, one sequence x 32 nodes 11.1 either way).  L and A are dense with zeros outside the
+// ancestors; zeros do not stop NaN, so a head with a non-finite q, k, v or gate takes the sums over the ancestors one by one instead, and y's rows of
+// unused nodes are selected, whatever the state holds.
 // M_ij is 2 to the difference of two sums G, which can be far larger than their difference (a path through tokens that wipe the state out).
 // G is summed in 64 bits and split into hi = fp32(G) and lo; with u'_i = 2^-lo_i u_i in place of u the solve needs 2^(hi_i - hi_j) only, and
 // lo enters factors of single nodes: beta_i 2^-lo_i on v, 2^lo_i on A's row.
@@ -687,8 +688,8 @@ int launch_tree_accept(const int* parents, const int* toks, const int* ids, int*
 // One bulk copy brings a head's state into shared memory while the path's tokens go through conv, norm and gates; then half of it at a time
 // lies in registers, a row on 8 lanes of 4 float4 each, so that a quarter warp reads and writes 128 contiguous bytes.  While the states
 // stream, a load that misses L2 takes 5 us, so a block asks L2 for the rows that a block of a later layer will need (32 KiB against its 128
-// of state, and the states are marked to leave L2 first).  24 sequences x 18 layers, accept and compaction included: 200 us (commit
-// alone 194, 5.0 TB/s), without the prefetch 249, two layers ahead instead of one 202.  Measured and not kept: state by plain loads (256), three blocks per SM with 80
+// of state, and the states are marked to leave L2 first).  24 sequences x 18 layers, accept and compaction included: 203 us (commit
+// alone 199, 4.8 TB/s), without the prefetch 249, two layers ahead instead of one 202 (against 200 then).  Measured and not kept: state by plain loads (256), three blocks per SM with 80
 // registers (204 .. 215), half heads on four blocks (305), 512 threads a head (309), persistent blocks with a ring of bulk copies (225 .. 380,
 // 25 against 14 us for one sequence).
 // ----------------------------------------------------------------------------------------------------------------------
