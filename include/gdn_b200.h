@@ -52,7 +52,7 @@ GDN_API const char* gdn_last_error_string(void);
  *   0  every device-side check passed since the last call
  *   1  a slot / snapshot / page index or a cu_seqlens entry was out of range: that row (sequence) was skipped, or, for a page
  *      index inside a context, page 0 was read in its place and that sequence's attention output is undefined
- *   2  a bounded wait inside the decode or attention kernel gave up (its copies never arrived); the block left early
+ *   2  a bounded wait inside a decode, attention or tree kernel gave up (its copies never arrived); the block left early
  *   3  a bounded wait inside a prefill kernel gave up; the block left early
  *   4  a kernel found its dynamic shared memory not 1024-byte aligned and did nothing
  * None of these faults the device: the context stays usable and the affected outputs are left unwritten or undefined. */

@@ -134,7 +134,8 @@ _HERE = contextlib.nullcontext()
 
 
 def device_status() -> int:
-    """Read and clear the device status word (1 = a kernel skipped a row because of an out-of-range index)."""
+    """Read and clear the status word of the current device (1 = a kernel skipped a row because of an out-of-range index, 2 or 3 = a
+    bounded wait gave up and the outputs of that call are unspecified)."""
     out = c_int(0)
     check(load().gdn_device_status(ctypes.byref(out)), "gdn_device_status")
     return out.value

@@ -91,7 +91,7 @@ __device__ __forceinline__ f32x2 pack2(float x, float y) { f32x2 r; asm("mov.b64
 __device__ __forceinline__ float2 unpack2(f32x2 v) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v)); return r; }
 __device__ __forceinline__ void fma2(f32x2& x, f32x2 a, f32x2 b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(x) : "l"(a), "l"(b)); }
 // The documented errors of the fast exp, 2 + 1.173 |x| ulp, and of the fast division, 2 ulp, make 2^-18 of the value up to |x| = 40 (below -40 the value is
-// smaller than 2^-52), 2^-9 of y's rounding to bf16.
+// smaller than 2^-52), a thousandth of y's rounding to bf16.
 __device__ __forceinline__ float silu_fast(float x) { return __fdividef(x, 1.f + __expf(-x)); }
 
 __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
